@@ -71,7 +71,7 @@ def draw(rng):
         per = max(2, _size(rng, 8, 512) // groups)
         E = groups * per
         group_k = rng.randint(1, groups)
-        k = rng.randint(1, min(20, per * group_k))
+        k = rng.randint(2 if op.endswith("train") else 1, min(20, per * group_k))   # one weight of one has no gradient
         return {"op": op, "T": _size(rng, 1, 4000000 // E), "E": E, "k": k, "scores": rng.choice(["softmax", "sigmoid"]),
                 "bias": rng.random() < 0.5, "groups": groups, "group_k": group_k, "renorm": rng.random() < 0.7,
                 "scale": rng.choice([1.0, 2.5]), "dtype": rng.choice(["f32", "bf16", "f16"]),
