@@ -161,7 +161,7 @@ def _quantized(x, fmt, dims):
     """x (float32) with each block, `dims` of x, in 8-bit floats with a power-of-two scale: the values they stand for"""
     m, e = torch.frexp(x.abs().amax(dim=dims, keepdim=True))
     e = e - (9 if fmt == "e4m3" else 16) + (m > 0.875).int()      # 448 = 0.875 * 2^9, 57344 = 0.875 * 2^16
-    e = torch.where(m == 0, torch.zeros_like(e), e).clamp(min=-120)
+    e = torch.where(m == 0, torch.zeros_like(e), e).clamp(min=-110)
     q = (x * _power(-e)).to(torch.float8_e4m3fn if fmt == "e4m3" else torch.float8_e5m2)
     return q.float() * _power(e)
 
@@ -375,7 +375,7 @@ def _exact_blocks(v, fmt):
         t = e + shift
         fits = big <= top * torch.exp2(t)
         e = torch.where(fits if shift < 0 else ~(big <= top * torch.exp2(e)), t, e)
-    scale = torch.where(big > 0, torch.exp2(e.clamp(min=-120)), torch.ones_like(big))
+    scale = torch.where(big > 0, torch.exp2(e.clamp(min=-110)), torch.ones_like(big))
     a = v / scale
     octave = torch.floor(torch.log2(a.abs().clamp(min=2.0 ** least)))
     octave = torch.where(torch.exp2(octave) > a.abs().clamp(min=2.0 ** least), octave - 1, octave)
