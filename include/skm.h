@@ -414,6 +414,108 @@ int skm_reduce_scatter_f64(void *comm, void *const *send_dev, void *const *recv_
 int skm_allgather_bytes(void *comm, void *const *send_dev, void *const *recv_dev, size_t send_bytes,
                         void *const *streams);
 
+/* ------------------------------------------------------------------ routing and 8-bit products (next row) ---- */
+/* The reference has posteriors of every component of a mixture (sidekit/mixture.py:52-64, 461-487) and products in
+ * float64; it has neither a choice of the best few components per row nor 8-bit products.  These entry points have NO
+ * COUNTERPART there: a mixture of linear transforms y_t = sum_j w_tj W_e(t,j) x_t, with the best k of E experts
+ * (components) per row, its gradients, and its products on the 8-bit matrix cores. */
+
+/* element types of logits, activations, weights and results */
+#define SKM_DT_F32  0
+#define SKM_DT_BF16 1
+#define SKM_DT_F16  2
+#define SKM_DT_F64  3   /* logits only */
+
+/* Choice of k of E experts per row of the logits x[T][ldx] (dev), with weights.
+ *   p = softmax of the row (SKM_ROUTE_SOFTMAX) or 1 / (1 + exp(-x)) (SKM_ROUTE_SIGMOID)
+ *   The order goes by x itself, with a bias (E float32, dev, or NULL) by c = p + bias, ties to the lowest index; it is
+ *   decided in float64 whatever the type of x.  groups > 1: E / groups neighbouring experts are a group, its score is
+ *   the sum of its group_top (1 or 2) largest c (p without a bias); only experts of the best group_k groups are taken.
+ *   weights = p of the chosen (divided by their sum with renorm) * scale.  The bias has no part in the weights.
+ *   A logit (or bias) of -inf is an expert that is not to be chosen.  Where fewer than k are left, ids = -1 and weight 0
+ *   fill the row.  A row with a NaN (softmax: or +inf) has ids -1 and weights NaN.
+ * ids_dev[T*k] int32 in the order of choice, weights_dev[T*k] float32.  E <= 4096, k <= 64, groups <= 64. */
+#define SKM_ROUTE_SOFTMAX 0
+#define SKM_ROUTE_SIGMOID 1
+int skm_route(void *ctx, const void *x_dev, int dtype, long T, int E, long ldx, int k, int scores, const float *bias_dev,
+              int groups, int group_k, int group_top, int renorm, float scale, int32_t *ids_dev, float *weights_dev,
+              void *stream);
+
+/* dx_dev[T*E] (type of x) = gradient of the logits for dweights_dev[T*k], the gradient of the weights; the choice itself
+ * has none.  Places with an id outside 0 .. E - 1 or a logit of -inf count as empty; an id that stands twice in a row
+ * gets the sum of both. */
+int skm_route_backward(void *ctx, const void *x_dev, int dtype, long T, int E, long ldx, int k, int scores, int renorm,
+                       float scale, const int32_t *ids_dev, const float *dweights_dev, void *dx_dev, void *stream);
+
+/* The rows of the experts' products: the n = T * k (token, slot) pairs with an id in 0 .. E - 1, by expert and within an
+ * expert in the order of the pairs.
+ *   offsets[E+1]  first row of an expert; [E] = rows in all         pair[n]  row -> t * k + j (behind the rows: untouched)
+ *   pos[n]        t * k + j -> row, -1 for a pair without an expert
+ *   first[E+1]    first tile of an expert, tiles of at most 128 of its rows; [E] = tiles in all
+ *   tiles[4 * skm_route_plan_tiles(n, E, 128)]       expert, first row, rows, 0 of every tile (behind them: untouched)
+ *   small_tiles[4 * skm_route_plan_tiles(n, E, 16)]  the same with 16 rows a tile, or NULL; small_count[1] their number
+ * all int32, dev.  Sizes stay on the device: nothing waits for it. */
+size_t skm_route_plan_workspace_bytes(long n, int E);
+long   skm_route_plan_tiles(long n, int E, int rows);
+int skm_route_plan(void *ctx, const int32_t *ids_dev, long n, int E, int32_t *offsets_dev, int32_t *pair_dev,
+                   int32_t *pos_dev, int32_t *first_dev, int32_t *tiles_dev, int32_t *small_tiles_dev,
+                   int32_t *small_count_dev, void *ws_dev, size_t ws_bytes, void *stream);
+
+/* out[t] = sum_j weights[t*k + j] rows[pos[t*k + j]], summed in the order of j in float32; a pos of -1 is a row of zeros.
+ * rows [.][N] and out [T][N] float32, bf16 or f16 (bf16 and f16 do not mix).  The gradient of the weights is
+ * dweights[t*k + j] = <dout[t], rows[pos]> (0 without a row); that of x is the same chain with the transposed weights. */
+int skm_route_combine(void *ctx, const void *rows_dev, int rows_dtype, const int32_t *pos_dev, const float *weights_dev,
+                      long T, int k, int N, void *out_dev, int out_dtype, void *stream);
+int skm_route_combine_backward(void *ctx, const void *rows_dev, int rows_dtype, const int32_t *pos_dev,
+                               const void *dout_dev, int dout_dtype, long T, int k, int N, float *dweights_dev,
+                               void *stream);
+
+/* Matrices of 8-bit floats with a power-of-two scale for each block of 128: a block is q * 2^e, e the smallest integer
+ * (>= -110; 0 for a block of zeros) with max |x| <= top * 2^e, top = 448 (e4m3) or 57344 (e5m2), q the nearest 8-bit
+ * floats to x * 2^-e, ties to even.  NaN and infinities have no part in e; they become NaN (an infinity stays one in
+ * e5m2).
+ *   q[rows][skm_fp8_row_bytes(K)]      K rounded up to 128, zeros behind K
+ *   s[rows][skm_fp8_scale_bytes(K)]    e + 127 of the row's blocks
+ * skm_fp8_rows     x[M][ldx]: blocks of 1 x 128 along the rows (activations, their gradients)
+ * skm_fp8_tiles    batch matrices w[N][ldw], sw elements apart: blocks of 128 x 128 (weights), every row of a block with
+ *                  the block's e; qt, st (or NULL, NULL): the transposed matrices [K][..N..] as well, the same numbers
+ * skm_fp8_columns  blocks of 128 rows x 1 column of x[R][ldx] (C columns), stored transposed: [C][..R..], for products
+ *                  over the rows (weight gradients).  With a plan (tiles, tile_count = first + E, max_tiles =
+ *                  skm_route_plan_tiles(n, E, 128), pair, slots = k) the rows are those of the pairs, x[pair / slots]
+ *                  times weights[pair] (float32 product; or NULL), and each expert's rows begin a new block: K is
+ *                  max_tiles * 128. */
+#define SKM_FP8_E4M3 0
+#define SKM_FP8_E5M2 1
+long skm_fp8_row_bytes(long K);
+long skm_fp8_scale_bytes(long K);
+int skm_fp8_rows(void *ctx, const void *x_dev, int dtype, long M, int K, long ldx, int fmt, void *q_dev, void *s_dev,
+                 void *stream);
+int skm_fp8_tiles(void *ctx, const void *w_dev, int dtype, int batch, int N, int K, long ldw, long sw, int fmt, void *q_dev,
+                  void *s_dev, void *qt_dev, void *st_dev, void *stream);
+int skm_fp8_columns(void *ctx, const void *x_dev, int dtype, long R, int C, long ldx, int fmt, const int32_t *tiles_dev,
+                    const int32_t *tile_count_dev, long max_tiles, const int32_t *pair_dev, int slots,
+                    const float *weights_dev, void *qt_dev, void *st_dev, void *stream);
+
+/* C[M][ldc] (+)= A B' of two such matrices [M][K], [N][K] (any of the three block shapes, either format), float32 sums.
+ * C float32, bf16 or f16; accumulate adds to what is there, before the rounding to C's type. */
+size_t skm_gemm_fp8_workspace_bytes(void *ctx, int M, int N, int K);
+int skm_gemm_fp8(void *ctx, const void *A_dev, const void *sA_dev, int fmt_a, const void *B_dev, const void *sB_dev,
+                 int fmt_b, int M, int N, int K, void *C_dev, int c_dtype, long ldc, int accumulate, void *ws_dev,
+                 size_t ws_bytes, void *stream);
+
+/* The experts' products: C[row] = W_e A[row of A], W [E][N][K] (tiles), for the rows of a plan of n pairs.  slots = k:
+ * the row of A is the pair's token (A is [T][K]); slots = 0: A is in the plan's order already ([n][K]).  Rows of C behind
+ * the plan's last are left as they are.
+ * skm_gemm_fp8_experts_wgrad: C[e] (+)= A_e B_e' (float32 [E][M][N]) over the rows of each expert, A [M], B [N] from
+ * skm_fp8_columns with the same plan; an expert without rows has zeros. */
+int skm_gemm_fp8_experts(void *ctx, const void *A_dev, const void *sA_dev, int fmt_a, const void *W_dev, const void *sW_dev,
+                         int fmt_w, int E, int N, int K, const int32_t *pair_dev, int slots, long n,
+                         const int32_t *first_dev, const int32_t *tiles_dev, const int32_t *small_tiles_dev,
+                         const int32_t *small_count_dev, void *C_dev, int c_dtype, void *stream);
+int skm_gemm_fp8_experts_wgrad(void *ctx, const void *A_dev, const void *sA_dev, int fmt_a, const void *B_dev,
+                               const void *sB_dev, int fmt_b, int E, int M, int N, const int32_t *first_dev, long max_tiles,
+                               float *C_dev, int accumulate, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

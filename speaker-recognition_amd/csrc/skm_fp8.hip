@@ -1,0 +1,680 @@
+// skm_fp8.hip -- matrix products of 8-bit floats with a scale for each block of 128 (gfx950 only).
+//
+// A block of 128 numbers is stored as 8-bit floats (e4m3 or e5m2) times 2^e, e the smallest integer with
+// max |x| <= top * 2^e (top 448 / 57344, the format's largest number).  A power of two costs nothing against any other
+// scale -- the 8-bit number has the same significand either way -- and buys two things: x * 2^-e is exact, so the
+// rounding to 8 bits is the only one, and the matrix cores apply 2^e themselves (v_mfma_scale_f32_*_f8f6f4 takes one
+// E8M0 byte per row and 32 k), so the product of blocks needs no vector-ALU work on the accumulators.
+//
+// Storage: q [rows][Kp] bytes, Kp = K rounded up to 128, zeros behind K; one scale byte (e + 127) per row and block of
+// 128 k, [rows][S] with S = Kp / 128 rounded up to 4 -- also where 128 rows share their scale (tiles of weights): the
+// kernels then have one operand layout, at 0.8 % more bytes.
+#include "skm_ops.h"
+
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+#define FP8_BLOCK 128
+// least e: the smallest number of either format (2^-16 in e5m2) times 2^e is still a normal float32 and bf16 number; only a
+// block whose largest number is below 57344 * 2^-110 (4e-29) loses digits to this
+#define FP8_MIN_EXP (-110)
+
+static inline long fp8_kpad(long K) { return (K + FP8_BLOCK - 1) / FP8_BLOCK * FP8_BLOCK; }
+static inline long fp8_sstride(long K) { return (fp8_kpad(K) / FP8_BLOCK + 3) / 4 * 4; }
+
+extern "C" long skm_fp8_row_bytes(long K) { return K < 1 ? 0 : fp8_kpad(K); }
+extern "C" long skm_fp8_scale_bytes(long K) { return K < 1 ? 0 : fp8_sstride(K); }
+
+// ------------------------------------------------------------------ quantization ------
+
+// e of a block whose largest finite magnitude is `top` (>= 0): 448 = 1.75 * 2^8, 57344 = 1.75 * 2^15
+__device__ __forceinline__ int fp8_exponent(float top, int fmt)
+{
+    const unsigned u = __float_as_uint(top);
+    if (u == 0) return 0;
+    const int e = (int)(u >> 23) - 127 - (fmt == SKM_FP8_E4M3 ? 8 : 15) + ((u & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    return e < FP8_MIN_EXP ? FP8_MIN_EXP : e;
+}
+
+__device__ __forceinline__ float fp8_pow2(int e) { return __uint_as_float((unsigned)(e + 127) << 23); }
+
+__device__ __forceinline__ float fp8_finite_abs(float x)
+{
+    const float a = fabsf(x);
+    return a < __builtin_inff() ? a : 0.f;      // NaN and infinities do not set the scale
+}
+
+// four scaled numbers -> four bytes, to nearest even.  e4m3 has no infinity: an infinite number becomes NaN
+template <int FMT>
+__device__ __forceinline__ unsigned fp8_pack4(float a, float b, float c, float d)
+{
+    if (FMT == SKM_FP8_E4M3) {
+        const float inf = __builtin_inff(), nan = __builtin_nanf("");
+        a = fabsf(a) == inf ? nan : a;
+        b = fabsf(b) == inf ? nan : b;
+        c = fabsf(c) == inf ? nan : c;
+        d = fabsf(d) == inf ? nan : d;
+        const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+        return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
+    }
+    const int lo = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, 0, false);
+    return (unsigned)__builtin_amdgcn_cvt_pk_bf8_f32(c, d, lo, true);
+}
+
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, bool vec, int n, float (&v)[8])
+{
+    typedef T v8 __attribute__((ext_vector_type(8)));
+    if (vec && n >= 8) {
+        const v8 x = *reinterpret_cast<const v8 *>(p);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = (float)x[q];
+    } else {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) v[q] = q < n ? (float)p[q] : 0.f;
+    }
+}
+
+struct RowsArgs {
+    const void *x;
+    long M, ldx;
+    int K, KB, S;           // blocks of a row, scale bytes of a row
+    int vec;                // 16-byte loads are allowed
+    uint8_t *q, *s;
+};
+
+// blocks of 1 x 128: 16 lanes per block, 8 numbers a lane
+template <typename T, int FMT>
+__global__ __launch_bounds__(256) void k_fp8_rows(RowsArgs a)
+{
+    const long b = ((long)blockIdx.x * 256 + threadIdx.x) >> 4;
+    const int l = threadIdx.x & 15;
+    const long row = b / a.KB;
+    const int kb = (int)(b - row * a.KB);
+    if (row >= a.M) return;                 // whole blocks of 16 lanes
+    const int k = kb * FP8_BLOCK + l * 8;
+    float v[8];
+    load8(static_cast<const T *>(a.x) + row * a.ldx + k, a.vec, a.K - k, v);
+    float top = 0.f;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) top = fmaxf(top, fp8_finite_abs(v[q]));
+#pragma unroll
+    for (int m = 8; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
+    const int e = fp8_exponent(top, FMT);
+    const float f = fp8_pow2(-e);
+    uint2 o;
+    o.x = fp8_pack4<FMT>(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+    o.y = fp8_pack4<FMT>(v[4] * f, v[5] * f, v[6] * f, v[7] * f);
+    *reinterpret_cast<uint2 *>(a.q + row * (long)a.KB * FP8_BLOCK + k) = o;
+    if (l == 0) a.s[row * a.S + kb] = (uint8_t)(e + 127);
+    if (kb == a.KB - 1 && l < a.S - a.KB) a.s[row * a.S + a.KB + l] = 127;
+}
+
+struct TileArgs {
+    const void *x;
+    long R, ldx, sx;        // rows, their stride, distance between matrices
+    int C;                  // columns
+    int vec;
+    uint8_t *q, *s;         // [z][R][Cp], [z][R][Sc]              (tiles only)
+    uint8_t *qt, *st;       // [z][C][Rp], [z][C][Sr]              NULL: not wanted
+    long Cp, Rp;
+    int Sc, Sr;
+    // columns by plan: rows in the plan's order, every expert from a new tile
+    const int32_t *tiles, *count, *pair;    // count[0] tiles of (expert, row, rows, 0)
+    int slots;
+    const float *w;         // weight of a pair or NULL
+};
+
+// blocks of 128 x 128 (COLS = 0) or 128 x 1 (COLS = 1): one workgroup per 128 x 128; a thread holds 8 columns of 8
+// consecutive rows, so that a transposed block goes through LDS in 8-byte pieces
+template <typename T, int FMT, int COLS>
+__global__ __launch_bounds__(256) void k_fp8_tiles(TileArgs a)
+{
+    __shared__ float red[16][FP8_BLOCK];
+    __shared__ __align__(16) uint8_t lt[FP8_BLOCK][FP8_BLOCK + 16];
+    const int tid = threadIdx.x, cg = tid & 15, rg = tid >> 4;
+    const int c0 = blockIdx.x * FP8_BLOCK, c = c0 + cg * 8;
+    const long rb = blockIdx.y, z = blockIdx.z;
+    long r0 = rb * FP8_BLOCK;
+    int rows = (int)(a.R - r0 < FP8_BLOCK ? a.R - r0 : FP8_BLOCK);
+    if (COLS && a.tiles) {
+        if (rb >= a.count[0]) return;
+        r0 = a.tiles[rb * 4 + 1];
+        rows = a.tiles[rb * 4 + 2];
+    }
+    const T *x = static_cast<const T *>(a.x) + z * a.sx;
+    float v[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = rg * 8 + i;
+        if (r < rows && c < a.C) {
+            long src = r0 + r;
+            float w = 1.f;
+            if (COLS && a.pair) {
+                const int pr = a.pair[src];
+                src = pr / a.slots;
+                if (a.w) w = a.w[pr];
+            }
+            load8(x + src * a.ldx + c, a.vec, a.C - c, v[i]);
+            if (COLS && a.w)
+#pragma unroll
+                for (int q = 0; q < 8; ++q) v[i][q] *= w;
+        } else {
+#pragma unroll
+            for (int q = 0; q < 8; ++q) v[i][q] = 0.f;
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = fmaxf(m, fp8_finite_abs(v[i][q]));
+        red[rg][cg * 8 + q] = m;
+    }
+    __syncthreads();
+    if (tid < FP8_BLOCK) {
+        float m = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) m = fmaxf(m, red[i][tid]);
+        red[0][tid] = m;
+    }
+    __syncthreads();
+    int e[8];
+    if (COLS) {
+#pragma unroll
+        for (int q = 0; q < 8; ++q) e[q] = fp8_exponent(red[0][cg * 8 + q], FMT);
+    } else {
+        float m = fmaxf(red[0][tid & 63], red[0][64 + (tid & 63)]);
+        m = wave_max(m);
+#pragma unroll
+        for (int q = 0; q < 8; ++q) e[q] = fp8_exponent(m, FMT);
+    }
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        const float f = fp8_pow2(-e[q]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i][q] *= f;
+    }
+    if (!COLS && a.q) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int r = rg * 8 + i;
+            if (r < rows) {
+                uint2 o;
+                o.x = fp8_pack4<FMT>(v[i][0], v[i][1], v[i][2], v[i][3]);
+                o.y = fp8_pack4<FMT>(v[i][4], v[i][5], v[i][6], v[i][7]);
+                *reinterpret_cast<uint2 *>(a.q + (z * a.R + r0 + r) * a.Cp + c) = o;
+            }
+        }
+        if (tid < rows) {
+            uint8_t *s = a.s + (z * a.R + r0 + tid) * a.Sc;
+            s[blockIdx.x] = (uint8_t)(e[0] + 127);
+            if (blockIdx.x == gridDim.x - 1)
+                for (int b = gridDim.x; b < a.Sc; ++b) s[b] = 127;
+        }
+    }
+    if (!a.qt) return;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        uint2 o;
+        o.x = fp8_pack4<FMT>(v[0][q], v[1][q], v[2][q], v[3][q]);
+        o.y = fp8_pack4<FMT>(v[4][q], v[5][q], v[6][q], v[7][q]);
+        *reinterpret_cast<uint2 *>(&lt[cg * 8 + q][rg * 8]) = o;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int col = i * 32 + (tid >> 3), piece = tid & 7;
+        if (c0 + col < a.C)
+            *reinterpret_cast<i32x4 *>(a.qt + (z * a.C + c0 + col) * a.Rp + rb * FP8_BLOCK + piece * 16) =
+                *reinterpret_cast<const i32x4 *>(&lt[col][piece * 16]);
+    }
+    if (tid < FP8_BLOCK && c0 + tid < a.C) {
+        const float m = red[0][tid];
+        uint8_t *s = a.st + (z * a.C + c0 + tid) * a.Sr;
+        s[rb] = (uint8_t)((COLS ? fp8_exponent(m, FMT) : e[0]) + 127);
+        if (rb == gridDim.y - 1)
+            for (int b = gridDim.y; b < a.Sr; ++b) s[b] = 127;
+    }
+}
+
+static bool aligned16(const void *p, long ld_bytes) { return ((uintptr_t)p & 15) == 0 && ld_bytes % 16 == 0; }
+
+#define FP8_IN_TYPES(F, ...)                                                             \
+    switch (dtype * 2 + fmt) {                                                           \
+    case SKM_DT_F32 * 2 + SKM_FP8_E4M3: F(float, SKM_FP8_E4M3, ##__VA_ARGS__); break;    \
+    case SKM_DT_F32 * 2 + SKM_FP8_E5M2: F(float, SKM_FP8_E5M2, ##__VA_ARGS__); break;    \
+    case SKM_DT_BF16 * 2 + SKM_FP8_E4M3: F(bf16_t, SKM_FP8_E4M3, ##__VA_ARGS__); break;  \
+    case SKM_DT_BF16 * 2 + SKM_FP8_E5M2: F(bf16_t, SKM_FP8_E5M2, ##__VA_ARGS__); break;  \
+    case SKM_DT_F16 * 2 + SKM_FP8_E4M3: F(f16_t, SKM_FP8_E4M3, ##__VA_ARGS__); break;    \
+    default: F(f16_t, SKM_FP8_E5M2, ##__VA_ARGS__); break;                               \
+    }
+
+static int fp8_check_types(const char *who, int dtype, int fmt)
+{
+    SKM_REQUIRE(dtype == SKM_DT_F32 || dtype == SKM_DT_BF16 || dtype == SKM_DT_F16, "%s: element type %d", who, dtype);
+    SKM_REQUIRE(fmt == SKM_FP8_E4M3 || fmt == SKM_FP8_E5M2, "%s: 8-bit format %d", who, fmt);
+    return SKM_OK;
+}
+
+extern "C" int skm_fp8_rows(void *ctx_, const void *x, int dtype, long M, int K, long ldx, int fmt, void *q, void *s,
+                            void *stream)
+{
+    SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
+    SKM_REQUIRE(ctx && M >= 0 && K >= 1 && ldx >= K && (M == 0 || (x && q && s)), "skm_fp8_rows: bad argument");
+    if (int rc = fp8_check_types("skm_fp8_rows", dtype, fmt)) return rc;
+    if (M == 0) return SKM_OK;
+    RowsArgs a{x, M, ldx, K, (int)(fp8_kpad(K) / FP8_BLOCK), (int)fp8_sstride(K),
+               aligned16(x, ldx * skm_dt_size(dtype)), static_cast<uint8_t *>(q), static_cast<uint8_t *>(s)};
+    const long grid = (M * a.KB + 15) / 16;
+    SKM_REQUIRE(grid <= 0x7FFFFFFF, "skm_fp8_rows: too many blocks");
+    SkmDeviceGuard guard(ctx);
+    hipStream_t st = (hipStream_t)stream;
+    SkmProfScope ps(ctx, "k_fp8_rows", st);
+#define ROWS_LAUNCH(T, FMT) hipLaunchKernelGGL((k_fp8_rows<T, FMT>), dim3((unsigned)grid), dim3(256), 0, st, a)
+    FP8_IN_TYPES(ROWS_LAUNCH)
+    SKM_HIP(hipGetLastError());
+    return SKM_OK;
+}
+
+extern "C" int skm_fp8_tiles(void *ctx_, const void *w, int dtype, int batch, int N, int K, long ldw, long sw, int fmt,
+                             void *q, void *s, void *qt, void *st_, void *stream)
+{
+    SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
+    SKM_REQUIRE(ctx && batch >= 0 && N >= 1 && K >= 1 && ldw >= K && (batch == 0 || (w && q && s)) && !qt == !st_,
+                "skm_fp8_tiles: bad argument");
+    if (int rc = fp8_check_types("skm_fp8_tiles", dtype, fmt)) return rc;
+    if (batch == 0) return SKM_OK;
+    SKM_REQUIRE(batch <= 65535 && fp8_kpad(N) / FP8_BLOCK <= 65535, "skm_fp8_tiles: too large");
+    TileArgs a{};
+    a.x = w; a.R = N; a.ldx = ldw; a.sx = sw; a.C = K;
+    a.vec = aligned16(w, ldw * skm_dt_size(dtype)) && (sw * skm_dt_size(dtype)) % 16 == 0;
+    a.q = static_cast<uint8_t *>(q); a.s = static_cast<uint8_t *>(s);
+    a.qt = static_cast<uint8_t *>(qt); a.st = static_cast<uint8_t *>(st_);
+    a.Cp = fp8_kpad(K); a.Rp = fp8_kpad(N); a.Sc = (int)fp8_sstride(K); a.Sr = (int)fp8_sstride(N);
+    SkmDeviceGuard guard(ctx);
+    hipStream_t st = (hipStream_t)stream;
+    SkmProfScope ps(ctx, "k_fp8_tiles", st);
+    const dim3 grid((unsigned)(a.Cp / FP8_BLOCK), (unsigned)(a.Rp / FP8_BLOCK), (unsigned)batch);
+#define TILES_LAUNCH(T, FMT, COLS) hipLaunchKernelGGL((k_fp8_tiles<T, FMT, COLS>), grid, dim3(256), 0, st, a)
+    FP8_IN_TYPES(TILES_LAUNCH, 0)
+    SKM_HIP(hipGetLastError());
+    return SKM_OK;
+}
+
+extern "C" int skm_fp8_columns(void *ctx_, const void *x, int dtype, long R, int C, long ldx, int fmt,
+                               const int32_t *tiles, const int32_t *tile_count, long max_tiles, const int32_t *pair,
+                               int slots, const float *weights, void *qt, void *st_, void *stream)
+{
+    SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
+    SKM_REQUIRE(ctx && R >= 0 && C >= 1 && ldx >= C, "skm_fp8_columns: bad argument");
+    SKM_REQUIRE(!tiles || (tile_count && pair && slots >= 1 && max_tiles >= 0), "skm_fp8_columns: incomplete plan");
+    SKM_REQUIRE(tiles || !weights, "skm_fp8_columns: weights go with a plan");
+    if (int rc = fp8_check_types("skm_fp8_columns", dtype, fmt)) return rc;
+    const long blocks = tiles ? max_tiles : fp8_kpad(R) / FP8_BLOCK;
+    if (blocks == 0) return SKM_OK;
+    SKM_REQUIRE(x && qt && st_, "skm_fp8_columns: bad argument");
+    SKM_REQUIRE(blocks <= 65535, "skm_fp8_columns: more than 65535 blocks of rows");
+    TileArgs a{};
+    a.x = x; a.R = R; a.ldx = ldx; a.C = C;
+    a.vec = aligned16(x, ldx * skm_dt_size(dtype));
+    a.qt = static_cast<uint8_t *>(qt); a.st = static_cast<uint8_t *>(st_);
+    a.Rp = blocks * FP8_BLOCK; a.Sr = (int)fp8_sstride(a.Rp);
+    a.tiles = tiles; a.count = tile_count; a.pair = tiles ? pair : nullptr; a.slots = slots; a.w = weights;
+    SkmDeviceGuard guard(ctx);
+    hipStream_t st = (hipStream_t)stream;
+    SkmProfScope ps(ctx, "k_fp8_columns", st);
+    const dim3 grid((unsigned)(fp8_kpad(C) / FP8_BLOCK), (unsigned)blocks, 1);
+    FP8_IN_TYPES(TILES_LAUNCH, 1)
+    SKM_HIP(hipGetLastError());
+    return SKM_OK;
+}
+
+// ------------------------------------------------------------------ product ------
+struct Fp8Args {
+    const uint8_t *A, *B;   // [M][lda], [N][ldb] bytes
+    const uint8_t *sA, *sB; // [M][SA], [N][SB]
+    long lda, ldb;
+    int SA, SB;
+    int M, N;
+    int kb0, kb1;           // blocks of 128 k
+    void *C;
+    long ldc;
+    int accumulate;
+    int tiles_m, tiles_n;
+    long zC;                // split over k: slab z holds the partial sums of its blocks, zC elements apart
+    int slabs;
+    // experts: row tiles from a table, the B operand by expert
+    const int32_t *tiles, *tile_count, *pair;
+    int slots;              // A row of a pair: pair / slots; 0: the plan's own order
+    long eB, esB;           // B, sB of the next expert
+    // weight gradient: blockIdx.y = expert, its blocks first[e] .. first[e + 1]
+    const int32_t *first;
+    long eC;
+};
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+
+// eight 8-bit floats times a power of two as bf16: exact (4 significant bits, normal numbers: FP8_MIN_EXP)
+template <int FMT>
+__device__ __forceinline__ bf16x8 fp8_to_bf16(int lo, int hi, float scale)
+{
+    bf16x2 v[4];
+    if (FMT == SKM_FP8_E4M3) {
+        v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, scale, false);
+        v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)lo, scale, true);
+        v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, scale, false);
+        v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8((unsigned)hi, scale, true);
+    } else {
+        v[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8((unsigned)lo, scale, false);
+        v[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8((unsigned)lo, scale, true);
+        v[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8((unsigned)hi, scale, false);
+        v[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_bf8((unsigned)hi, scale, true);
+    }
+    bf16x8 o;
+#pragma unroll
+    for (int q = 0; q < 8; ++q) o[q] = v[q >> 1][q & 1];
+    return o;
+}
+
+typedef __attribute__((address_space(3))) void *lds_ptr;
+typedef __attribute__((address_space(1))) const void *glb_ptr;
+
+// C = A B'.  Workgroup: 4 waves as 2 x 2, a wave MT x NT tiles of 32 x 32 (v_mfma_scale_f32_32x32x64_f8f6f4), one block
+// of 128 k a stage, two stages in LDS filled by global loads that go there directly.
+//   LDS: a row's 128 bytes of a stage are one line; its 16-byte pieces are stored at piece ^ (row & 7), so that the 8
+//   lanes of a read phase (8 rows, the same piece) meet 8 different bank groups.  The loads put consecutive lanes'
+//   pieces at consecutive addresses, so the exchange is made on the global side, within the line.
+//   The 8-bit matrix instructions add 8 products at a time in a window of 13 bits below the largest of the 8 (a product
+//   2^-14 of it is lost, measured): 1.4e-5 of a result of random operands.  Under a result that is rounded to bf16 or f16
+//   (2^-9, 2^-12) that is nothing; a float32 result is wanted as such (weight gradients that are added up, rows that a
+//   gradient is formed with), so there the operands become bf16 -- exactly, scale included -- and the products are exact
+//   and the sums float32, at half the rate.
+//   Which of the 64 k of a product lies where in the operand registers does not matter as long as A and B agree and a
+//   scale covers all of them: a lane's 32 bytes are 32 consecutive k of its row here.
+template <int MT, int NT, int FA, int FB, typename TO>
+__global__ __launch_bounds__(256, (MT * NT > 8) ? 1 : 2) void k_gemm_fp8(Fp8Args g)
+{
+    constexpr int BM = MT * 64, BN = NT * 64;
+    __shared__ __align__(16) uint8_t sh[2][(BM + BN) * FP8_BLOCK];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave >> 1, wn = wave & 1, r = lane & 31, h = lane >> 5;
+
+    int tm, tn;
+    {   // workgroups w, w + 8, ... share an XCD: an XCD takes a run of consecutive tiles, columns of 8 row tiles at a time
+        const int total = g.tiles_m * g.tiles_n;
+        const int q = total / 8, rem = total % 8, x = blockIdx.x % 8, i = blockIdx.x / 8;
+        int t = x * q + (x < rem ? x : rem) + i;
+        const int group = 8 * g.tiles_n, gi = t / group, m0 = gi * 8;
+        const int gm = g.tiles_m - m0 < 8 ? g.tiles_m - m0 : 8;
+        t -= gi * group;
+        tm = m0 + t % gm;
+        tn = t / gm;
+    }
+    int kb0 = g.kb0, kb1 = g.kb1;
+    int rows = g.M - tm * BM;               // rows of this tile
+    long row0 = (long)tm * BM;
+    const uint8_t *B = g.B, *sB = g.sB;
+    TO *C = static_cast<TO *>(g.C);
+    if (g.tiles) {
+        if (tm >= g.tile_count[0]) return;
+        const int32_t *t = g.tiles + (long)tm * 4;
+        B += t[0] * g.eB;
+        sB += t[0] * g.esB;
+        row0 = t[1];
+        rows = t[2];
+    } else if (g.first) {
+        const int e = blockIdx.y;
+        kb0 = g.first[e];
+        kb1 = g.first[e + 1];
+        C += e * g.eC;
+    } else if (g.slabs > 1) {
+        const int z = blockIdx.y, n = kb1 - kb0;
+        kb1 = kb0 + (int)((long)n * (z + 1) / g.slabs);
+        kb0 += (int)((long)n * z / g.slabs);
+        C += z * g.zC;
+    }
+    const int col0 = tn * BN, cols = g.N - col0;
+
+    // one row of A (B) per lane and load: rows behind the last repeat it
+    const int lr = lane >> 3, lp = ((lane & 7) ^ lr) * 16;
+    const uint8_t *pa[MT * 2], *pb[NT * 2];
+#pragma unroll
+    for (int i = 0; i < MT * 2; ++i) {
+        int rr = (wave * MT * 2 + i) * 8 + lr;
+        rr = rr < rows ? rr : rows - 1;
+        long src = row0 + rr;
+        if (g.tiles && g.slots) src = g.pair[src] / g.slots;
+        pa[i] = g.A + src * g.lda + (long)kb0 * FP8_BLOCK + lp;
+    }
+#pragma unroll
+    for (int i = 0; i < NT * 2; ++i) {
+        int cc = (wave * NT * 2 + i) * 8 + lr;
+        cc = cc < cols ? cc : cols - 1;
+        pb[i] = B + (col0 + cc) * g.ldb + (long)kb0 * FP8_BLOCK + lp;
+    }
+    const uint8_t *qa[MT], *qb[NT];         // scales of the rows (columns) of this lane
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        int rr = wm * MT * 32 + i * 32 + r;
+        rr = rr < rows ? rr : rows - 1;
+        long src = row0 + rr;
+        if (g.tiles && g.slots) src = g.pair[src] / g.slots;
+        qa[i] = g.sA + src * g.SA;
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        int cc = wn * NT * 32 + i * 32 + r;
+        cc = cc < cols ? cc : cols - 1;
+        qb[i] = sB + (long)(col0 + cc) * g.SB;
+    }
+    f32x16 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
+
+#define FP8_ISSUE(ST)                                                                                                  \
+    _Pragma("unroll") for (int i = 0; i < MT * 2; ++i) {                                                               \
+        __builtin_amdgcn_global_load_lds((glb_ptr)pa[i], (lds_ptr)&sh[ST][(wave * MT * 2 + i) * 8 * FP8_BLOCK], 16, 0, 0); \
+        pa[i] += FP8_BLOCK;                                                                                            \
+    }                                                                                                                  \
+    _Pragma("unroll") for (int i = 0; i < NT * 2; ++i) {                                                               \
+        __builtin_amdgcn_global_load_lds((glb_ptr)pb[i],                                                               \
+                                         (lds_ptr)&sh[ST][(BM + (wave * NT * 2 + i) * 8) * FP8_BLOCK], 16, 0, 0);      \
+        pb[i] += FP8_BLOCK;                                                                                            \
+    }
+
+    const int n = kb1 - kb0;
+    if (n > 0) { FP8_ISSUE(0) }
+    // bytes of this lane's pieces: half H of the block, pieces 4 H + 2 h and the next, exchanged by row & 7 = r & 7
+    const int x7 = r & 7;
+    for (int s = 0; s < n; ++s) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();                    // stage s is there, and everybody has left the other buffer
+        if (s + 1 < n) { FP8_ISSUE((s + 1) & 1) }
+        const int kb = kb0 + s;
+        int sa[MT], sb[NT];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) sa[i] = qa[i][kb];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) sb[i] = qb[i][kb];
+        const uint8_t *base = sh[s & 1];
+#pragma unroll
+        for (int H = 0; H < 2; ++H) {
+            i32x8 fa[MT], fb[NT];
+            const int p0 = ((H * 4 + h * 2) ^ x7) * 16, p1 = ((H * 4 + h * 2 + 1) ^ x7) * 16;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) {
+                const uint8_t *l = base + (wm * MT * 32 + i * 32 + r) * FP8_BLOCK;
+                const i32x4 lo = *reinterpret_cast<const i32x4 *>(l + p0), hi = *reinterpret_cast<const i32x4 *>(l + p1);
+                fa[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const uint8_t *l = base + (BM + wn * NT * 32 + i * 32 + r) * FP8_BLOCK;
+                const i32x4 lo = *reinterpret_cast<const i32x4 *>(l + p0), hi = *reinterpret_cast<const i32x4 *>(l + p1);
+                fb[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+            if (sizeof(TO) == 4) {
+                bf16x8 xb[NT][4];
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t)
+                        xb[j][t] = fp8_to_bf16<FB>(fb[j][2 * t], fb[j][2 * t + 1], fp8_pow2(sb[j] - 127));
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int t = 0; t < 4; ++t) {
+                        const bf16x8 xa = fp8_to_bf16<FA>(fa[i][2 * t], fa[i][2 * t + 1], fp8_pow2(sa[i] - 127));
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa, xb[j][t], acc[i][j], 0, 0, 0);
+                    }
+            } else {
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[i], fb[j], acc[i][j], FA, FB, 0,
+                                                                                    sa[i], 0, sb[j]);
+            }
+        }
+    }
+#undef FP8_ISSUE
+    // result of a 32 x 32 tile: lane: column lane & 31; register q: row (q & 3) + 8 (q >> 2) + 4 (lane >> 5)
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const int cc = wn * NT * 32 + j * 32 + r;
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+                const int rr = wm * MT * 32 + i * 32 + (q & 3) + 8 * (q >> 2) + 4 * h;
+                if (rr < rows && cc < cols) {
+                    TO *d = C + (row0 + rr) * g.ldc + col0 + cc;
+                    *d = (TO)(g.accumulate ? (float)*d + acc[i][j][q] : acc[i][j][q]);
+                }
+            }
+        }
+}
+
+template <int MT, int NT, typename TO>
+static void fp8_launch(const Fp8Args &g, int fa, int fb, unsigned gx, unsigned gy, hipStream_t st)
+{
+    const dim3 grid(gx, gy), block(256);
+    switch (fa * 2 + fb) {
+    case 0: hipLaunchKernelGGL((k_gemm_fp8<MT, NT, 0, 0, TO>), grid, block, 0, st, g); break;
+    case 1: hipLaunchKernelGGL((k_gemm_fp8<MT, NT, 0, 1, TO>), grid, block, 0, st, g); break;
+    case 2: hipLaunchKernelGGL((k_gemm_fp8<MT, NT, 1, 0, TO>), grid, block, 0, st, g); break;
+    default: hipLaunchKernelGGL((k_gemm_fp8<MT, NT, 1, 1, TO>), grid, block, 0, st, g); break;
+    }
+}
+
+static int fp8_run(SkmCtx *ctx, Fp8Args g, int fa, int fb, int dtype, unsigned gy, hipStream_t st, const char *tag)
+{
+    g.tiles_n = (g.N + 127) / 128;
+    const long total = (long)g.tiles_m * g.tiles_n;
+    SKM_REQUIRE(total <= 0x7FFFFFFF && gy <= 65535, "%s: too many tiles", tag);
+    if (total == 0 || gy == 0) return SKM_OK;
+    SkmProfScope ps(ctx, tag, st);
+    switch (dtype) {
+    case SKM_DT_F32: fp8_launch<2, 2, float>(g, fa, fb, (unsigned)total, gy, st); break;
+    case SKM_DT_BF16: fp8_launch<2, 2, bf16_t>(g, fa, fb, (unsigned)total, gy, st); break;
+    default: fp8_launch<2, 2, f16_t>(g, fa, fb, (unsigned)total, gy, st); break;
+    }
+    SKM_HIP(hipGetLastError());
+    return SKM_OK;
+}
+
+static int fp8_check_product(const char *who, int fa, int fb, int dtype, int M, int N, int K)
+{
+    SKM_REQUIRE((fa == 0 || fa == 1) && (fb == 0 || fb == 1), "%s: 8-bit formats %d, %d", who, fa, fb);
+    SKM_REQUIRE(dtype == SKM_DT_F32 || dtype == SKM_DT_BF16 || dtype == SKM_DT_F16, "%s: result type %d", who, dtype);
+    SKM_REQUIRE(M >= 0 && N >= 0 && K >= 0 && M < 0x7FFFFF00 && N < 0x7FFFFF00 && K < 0x7FFFFF00, "%s: bad shape", who);
+    return SKM_OK;
+}
+
+extern "C" size_t skm_gemm_fp8_workspace_bytes(void *ctx, int M, int N, int K)
+{
+    (void)ctx; (void)M; (void)N; (void)K;
+    return 0;
+}
+
+extern "C" int skm_gemm_fp8(void *ctx_, const void *A, const void *sA, int fmt_a, const void *B, const void *sB, int fmt_b,
+                            int M, int N, int K, void *C, int c_dtype, long ldc, int accumulate, void *ws,
+                            size_t ws_bytes, void *stream)
+{
+    SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
+    SKM_REQUIRE(ctx, "skm_gemm_fp8: bad argument");
+    if (int rc = fp8_check_product("skm_gemm_fp8", fmt_a, fmt_b, c_dtype, M, N, K)) return rc;
+    if (M == 0 || N == 0) return SKM_OK;
+    SKM_REQUIRE(K >= 1 && A && sA && B && sB && C && ldc >= N, "skm_gemm_fp8: bad argument");
+    if (ws_bytes < skm_gemm_fp8_workspace_bytes(ctx, M, N, K)) {
+        skm_set_error("skm_gemm_fp8: workspace too small");
+        return SKM_ERR_WORKSPACE;
+    }
+    (void)ws;
+    SkmDeviceGuard guard(ctx);
+    Fp8Args g{};
+    g.A = static_cast<const uint8_t *>(A); g.B = static_cast<const uint8_t *>(B);
+    g.sA = static_cast<const uint8_t *>(sA); g.sB = static_cast<const uint8_t *>(sB);
+    g.lda = g.ldb = fp8_kpad(K);
+    g.SA = g.SB = (int)fp8_sstride(K);
+    g.M = M; g.N = N; g.kb1 = (int)(fp8_kpad(K) / FP8_BLOCK);
+    g.C = C; g.ldc = ldc; g.accumulate = accumulate != 0; g.slabs = 1;
+    g.tiles_m = (M + 127) / 128;
+    return fp8_run(ctx, g, fmt_a, fmt_b, c_dtype, 1, (hipStream_t)stream, "k_gemm_fp8");
+}
+
+extern "C" int skm_gemm_fp8_experts(void *ctx_, const void *A, const void *sA, int fmt_a, const void *W, const void *sW,
+                                    int fmt_w, int E, int N, int K, const int32_t *pair, int slots, long n,
+                                    const int32_t *first, const int32_t *tiles, const int32_t *small_tiles,
+                                    const int32_t *small_count, void *C, int c_dtype, void *stream)
+{
+    SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
+    SKM_REQUIRE(ctx && E >= 1 && n >= 0 && n <= 0x3FFFFFFF && slots >= 0, "skm_gemm_fp8_experts: bad argument");
+    if (int rc = fp8_check_product("skm_gemm_fp8_experts", fmt_a, fmt_w, c_dtype, (int)n, N, K)) return rc;
+    if (n == 0 || N == 0) return SKM_OK;
+    SKM_REQUIRE(K >= 1 && A && sA && W && sW && C && pair && first && tiles, "skm_gemm_fp8_experts: bad argument");
+    (void)small_tiles; (void)small_count;
+    SkmDeviceGuard guard(ctx);
+    Fp8Args g{};
+    g.A = static_cast<const uint8_t *>(A); g.B = static_cast<const uint8_t *>(W);
+    g.sA = static_cast<const uint8_t *>(sA); g.sB = static_cast<const uint8_t *>(sW);
+    g.lda = g.ldb = fp8_kpad(K);
+    g.SA = g.SB = (int)fp8_sstride(K);
+    g.M = (int)n; g.N = N; g.kb1 = (int)(fp8_kpad(K) / FP8_BLOCK);
+    g.C = C; g.ldc = N; g.slabs = 1;
+    g.tiles = tiles; g.tile_count = first + E; g.pair = pair; g.slots = slots;
+    g.eB = (long)N * g.ldb; g.esB = (long)N * g.SB;
+    g.tiles_m = (int)skm_route_plan_tiles(n, E, 128);
+    return fp8_run(ctx, g, fmt_a, fmt_w, c_dtype, 1, (hipStream_t)stream, "k_gemm_fp8_experts");
+}
+
+extern "C" int skm_gemm_fp8_experts_wgrad(void *ctx_, const void *A, const void *sA, int fmt_a, const void *B,
+                                          const void *sB, int fmt_b, int E, int M, int N, const int32_t *first,
+                                          long max_tiles, float *C, int accumulate, void *stream)
+{
+    SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
+    SKM_REQUIRE(ctx && E >= 1 && E <= 65535 && max_tiles >= 0 && max_tiles < 0x7FFFFFFF / FP8_BLOCK,
+                "skm_gemm_fp8_experts_wgrad: bad argument");
+    if (int rc = fp8_check_product("skm_gemm_fp8_experts_wgrad", fmt_a, fmt_b, SKM_DT_F32, M, N, 1)) return rc;
+    if (M == 0 || N == 0) return SKM_OK;
+    SKM_REQUIRE(C && first && (max_tiles == 0 || (A && sA && B && sB)), "skm_gemm_fp8_experts_wgrad: bad argument");
+    SkmDeviceGuard guard(ctx);
+    Fp8Args g{};
+    g.A = static_cast<const uint8_t *>(A); g.B = static_cast<const uint8_t *>(B);
+    g.sA = static_cast<const uint8_t *>(sA); g.sB = static_cast<const uint8_t *>(sB);
+    g.lda = g.ldb = max_tiles * FP8_BLOCK;
+    g.SA = g.SB = (int)fp8_sstride(g.lda);
+    g.M = M; g.N = N;
+    g.C = C; g.ldc = N; g.accumulate = accumulate != 0; g.slabs = 1;
+    g.first = first; g.eC = (long)M * N;
+    g.tiles_m = (M + 127) / 128;
+    return fp8_run(ctx, g, fmt_a, fmt_b, SKM_DT_F32, (unsigned)E, (hipStream_t)stream, "k_gemm_fp8_wgrad");
+}

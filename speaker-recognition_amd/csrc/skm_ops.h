@@ -1,0 +1,45 @@
+// skm_ops.h -- what skm_route.hip and skm_fp8.hip share: element types, device guard, wave reductions (gfx950 only).
+#pragma once
+#include "skm_common.h"
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+// element size of an SKM_DT_* code, 0 for an unknown one
+static inline int skm_dt_size(int dt)
+{
+    return dt == SKM_DT_F32 ? 4 : dt == SKM_DT_BF16 || dt == SKM_DT_F16 ? 2 : dt == SKM_DT_F64 ? 8 : 0;
+}
+
+// The launches go to the ctx's GPU whatever device the calling thread has current.
+struct SkmDeviceGuard {
+    int prev;
+    bool changed;
+    explicit SkmDeviceGuard(const SkmCtx *ctx) : prev(-1), changed(false)
+    {
+        if (hipGetDevice(&prev) == hipSuccess && prev != ctx->device) changed = hipSetDevice(ctx->device) == hipSuccess;
+    }
+    ~SkmDeviceGuard()
+    {
+        if (changed) (void)hipSetDevice(prev);
+    }
+};
+
+template <typename T>
+__device__ __forceinline__ T wave_max(T v)
+{
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) {
+        const T o = __shfl_xor(v, m);
+        v = o > v ? o : v;
+    }
+    return v;
+}
+
+template <typename T>
+__device__ __forceinline__ T wave_sum(T v)
+{
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m);
+    return v;
+}

@@ -1,0 +1,677 @@
+// skm_route.hip -- routing of rows to the best few of E experts (components of a mixture, linear transforms): choice
+// and weights, their gradient, the order in which the experts' products take the rows, and the weighted sum of what
+// they return.  gfx950 only.
+#include "skm_ops.h"
+
+#define ROUTE_MAX_E 4096
+#define ROUTE_MAX_K 64
+#define ROUTE_MAX_G 64
+
+struct RouteArgs {
+    const void *x;          // logits [T][ldx]
+    long T, ldx;
+    int E, k;
+    const float *bias;      // [E] or NULL
+    int groups, group_k, group_top;
+    int sigmoid, renorm;
+    float scale;
+    int32_t *ids;           // [T][k]
+    float *w;               // [T][k]
+};
+
+// weights' numerators of the chosen places: t_j proportional to p_j, the same factor for the whole row, without
+// overflow or underflow of the largest one.  M: softmax the largest chosen logit, sigmoid min(0, that).
+//   softmax: exp(x - M)      sigmoid: exp(x - M) / (1 + exp(x)) for x <= 0 (= sigmoid(x) exp(-M)), sigmoid(x) above
+template <typename A>
+__device__ __forceinline__ A route_share(A x, A M, int sigmoid)
+{
+    if (!sigmoid) return exp(x - M);
+    if (x <= (A)0) return exp(x - M) / ((A)1 + exp(x));
+    return (A)1 / ((A)1 + exp(-x));
+}
+
+// One wave, one row, everything in float64: lane l holds the experts l, l + 64, ...
+// The order of the experts is what must not depend on rounding: two choices that differ by less than a float32
+// rounding are told apart here.  -inf as a key = not to be chosen.
+template <typename T, int NV>
+__device__ void route_row(const RouteArgs &a, long row, int lane)
+{
+    const T *x = static_cast<const T *>(a.x) + row * a.ldx;
+    const double inf = __builtin_inf();
+    double key[NV];
+    double top = -inf;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int e = lane + 64 * i;
+        key[i] = e < a.E ? (double)x[e] : -inf;
+        bad |= key[i] != key[i];
+        top = key[i] > top ? key[i] : top;
+    }
+    top = wave_max(top);
+    bad |= !a.sigmoid && top == inf;
+    double total = 1.0;
+    if (!a.sigmoid && (a.bias || a.groups > 1 || !a.renorm)) {
+        total = 0.0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) total += key[i] == -inf ? 0.0 : exp(key[i] - top);
+        total = wave_sum(total);
+    }
+    if (a.bias || a.groups > 1) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (key[i] == -inf) continue;
+            const int e = lane + 64 * i;
+            double p = a.sigmoid ? 1.0 / (1.0 + exp(-key[i])) : exp(key[i] - top) / total;
+            if (a.bias) p += (double)a.bias[e];
+            bad |= p != p;
+            key[i] = p;
+        }
+    }
+    if (__any(bad)) {                       // NaN: no choice, and the weights say so
+        if (lane < a.k) {
+            a.ids[row * a.k + lane] = -1;
+            a.w[row * a.k + lane] = __builtin_nanf("");
+        }
+        return;
+    }
+    if (a.groups > 1) {
+        const int per = a.E / a.groups;
+        double mine = -inf;
+        for (int g = 0; g < a.groups; ++g) {
+            double f1 = -inf, f2 = -inf;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int e = lane + 64 * i;
+                if (e >= g * per && e < (g + 1) * per) {
+                    if (key[i] > f1) { f2 = f1; f1 = key[i]; }
+                    else if (key[i] > f2) f2 = key[i];
+                }
+            }
+#pragma unroll
+            for (int m = 32; m > 0; m >>= 1) {
+                const double o1 = __shfl_xor(f1, m), o2 = __shfl_xor(f2, m);
+                const double lo = f1 < o1 ? f1 : o1, two = f2 > o2 ? f2 : o2;
+                f1 = f1 > o1 ? f1 : o1;
+                f2 = lo > two ? lo : two;
+            }
+            const double s = (a.group_top == 1 || f2 == -inf) ? f1 : f1 + f2;
+            if (lane == g) mine = s;
+        }
+        int ahead = 0;
+        for (int g = 0; g < a.groups; ++g) {
+            const double s = __shfl(mine, g);
+            ahead += (s > mine || (s == mine && g < lane)) ? 1 : 0;
+        }
+        const unsigned long long stay = __ballot(lane < a.groups && ahead < a.group_k);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = lane + 64 * i;
+            if (e >= a.E) continue;
+            if (!((stay >> (e / per)) & 1)) key[i] = -inf;
+            else if (!a.bias) key[i] = (double)x[e];        // within what stays the logits themselves give the order
+        }
+    }
+    int my_id = -1;
+    for (int j = 0; j < a.k; ++j) {
+        double best = -inf;
+        int at = 0x7FFFFFFF;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (key[i] > best) {
+                best = key[i];
+                at = lane + 64 * i;
+            }
+#pragma unroll
+        for (int m = 32; m > 0; m >>= 1) {
+            const double ob = __shfl_xor(best, m);
+            const int oa = __shfl_xor(at, m);
+            if (ob > best || (ob == best && oa < at)) {
+                best = ob;
+                at = oa;
+            }
+        }
+        if (best == -inf) break;            // uniform: nothing is left for any further place
+        if (lane == j) my_id = at;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (lane + 64 * i == at) key[i] = -inf;
+    }
+    const double xs = my_id >= 0 ? (double)x[my_id] : -inf;
+    double t = 0.0;
+    if (a.renorm) {
+        double M = wave_max(xs);
+        if (a.sigmoid && M > 0.0) M = 0.0;
+        if (my_id >= 0) t = route_share(xs, M, a.sigmoid);
+        const double s = wave_sum(t);
+        if (s > 0.0) t /= s;
+    } else if (my_id >= 0) {
+        t = a.sigmoid ? 1.0 / (1.0 + exp(-xs)) : exp(xs - top) / total;
+    }
+    if (lane < a.k) {
+        a.ids[row * a.k + lane] = my_id;
+        a.w[row * a.k + lane] = (float)(t * (double)a.scale);
+    }
+}
+
+template <typename T, int NV>
+__global__ __launch_bounds__(256) void k_route(RouteArgs a)
+{
+    const int lane = threadIdx.x & 63;
+    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row < a.T) route_row<T, NV>(a, row, lane);
+}
+
+struct RouteBackArgs {
+    const void *x;
+    long T, ldx;
+    int E, k;
+    const int32_t *ids;
+    const float *g;         // dL/dweights [T][k]
+    int sigmoid, renorm;
+    float scale;
+    void *dx;               // [T][E] in the type of x
+};
+
+// One wave per row.  Lane j < k holds place j: its logit, its share and d_j, what it adds to the gradient of its
+// logit.  Only softmax without renormalisation has a gradient beside the chosen places (- p_i sum_j p_j u_j):
+//   renorm   with s_j = t_j / sum t (t of route_share), G = sum_j s_j g_j:
+//            softmax d_j = scale s_j (g_j - G)          sigmoid d_j = scale s_j (1 - p_j) (g_j - G)
+//   else     sigmoid d_j = scale g_j p_j (1 - p_j)      softmax d_j = scale g_j p_j, dx_i = sum d_j - p_i sum_j d_j
+// so all the other variants read k logits of a row and not E.
+template <typename T, typename A>
+__global__ __launch_bounds__(256) void k_route_backward(RouteBackArgs a)
+{
+    const int lane = threadIdx.x & 63;
+    const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (row >= a.T) return;
+    const T *x = static_cast<const T *>(a.x) + row * a.ldx;
+    T *dx = static_cast<T *>(a.dx) + row * a.E;
+    const A inf = (A)__builtin_inf();
+    int id = -1;
+    A xs = -inf, g = 0;
+    if (lane < a.k) {
+        id = a.ids[row * a.k + lane];
+        if (id < 0 || id >= a.E) id = -1;
+        else {
+            xs = (A)x[id];
+            g = (A)a.g[row * a.k + lane];
+            if (xs == -inf) id = -1;
+        }
+    }
+    const bool there = id >= 0;
+    A d = 0, D = 0, top = 0, total = 1;
+    if (a.renorm) {
+        A M = wave_max(there ? xs : -inf);
+        if (a.sigmoid && M > (A)0) M = 0;
+        A t = there ? route_share(xs, M, a.sigmoid) : (A)0;
+        const A s = wave_sum(t);
+        t = s > (A)0 ? t / s : t;
+        const A G = wave_sum(there ? t * g : (A)0);
+        d = there ? (A)a.scale * t * (g - G) : (A)0;
+        if (a.sigmoid && there) d *= (A)1 / ((A)1 + exp(xs));
+    } else if (a.sigmoid) {
+        if (there) d = (A)a.scale * g / ((A)1 + exp(-xs)) / ((A)1 + exp(xs));
+    } else {
+        top = -inf;
+        for (int e = lane; e < a.E; e += 64) top = (A)x[e] > top ? (A)x[e] : top;
+        top = wave_max(top);
+        if (top == -inf) top = 0;
+        total = 0;
+        for (int e = lane; e < a.E; e += 64) total += exp((A)x[e] - top);
+        total = wave_sum(total);
+        if (there) d = (A)a.scale * g * exp(xs - top) / total;
+        D = wave_sum(d);
+    }
+    for (int e0 = 0; e0 < a.E; e0 += 64) {
+        const int e = e0 + lane;
+        A v = 0;
+        if (D != (A)0 && e < a.E) v = -D * exp((A)x[e] - top) / total;
+        for (int j = 0; j < a.k; ++j) {                 // in the order of the places: the same bits every time
+            const int at = __shfl(id, j);
+            const A dj = __shfl(d, j);
+            if (at == e) v += dj;
+        }
+        if (e < a.E) dx[e] = (T)v;
+    }
+}
+
+static int route_nv(int E)
+{
+    int nv = 1;
+    while (nv * 64 < E) nv *= 2;
+    return nv;
+}
+
+template <typename T>
+static void route_launch(const RouteArgs &a, hipStream_t st)
+{
+    const dim3 grid((unsigned)((a.T + 3) / 4)), block(256);
+    switch (route_nv(a.E)) {
+    case 1: hipLaunchKernelGGL((k_route<T, 1>), grid, block, 0, st, a); break;
+    case 2: hipLaunchKernelGGL((k_route<T, 2>), grid, block, 0, st, a); break;
+    case 4: hipLaunchKernelGGL((k_route<T, 4>), grid, block, 0, st, a); break;
+    case 8: hipLaunchKernelGGL((k_route<T, 8>), grid, block, 0, st, a); break;
+    case 16: hipLaunchKernelGGL((k_route<T, 16>), grid, block, 0, st, a); break;
+    case 32: hipLaunchKernelGGL((k_route<T, 32>), grid, block, 0, st, a); break;
+    default: hipLaunchKernelGGL((k_route<T, 64>), grid, block, 0, st, a); break;
+    }
+}
+
+extern "C" int skm_route(void *ctx_, const void *x, int dtype, long T, int E, long ldx, int k, int scores,
+                         const float *bias, int groups, int group_k, int group_top, int renorm, float scale,
+                         int32_t *ids, float *weights, void *stream)
+{
+    SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
+    SKM_REQUIRE(ctx && skm_dt_size(dtype) && T >= 0 && E >= 1 && ldx >= E && (T == 0 || (x && ids && weights)),
+                "skm_route: bad argument");
+    SKM_REQUIRE(scores == SKM_ROUTE_SOFTMAX || scores == SKM_ROUTE_SIGMOID, "skm_route: unknown scores %d", scores);
+    SKM_REQUIRE(k >= 1 && k <= E, "skm_route: k = %d of %d experts", k, E);
+    SKM_REQUIRE(groups >= 1 && E % groups == 0 && group_k >= 1 && group_k <= groups,
+                "skm_route: %d of %d groups over %d experts", group_k, groups, E);
+    SKM_REQUIRE(k <= E / groups * group_k, "skm_route: k = %d of the %d experts that %d groups hold", k,
+                E / groups * group_k, group_k);
+    SKM_REQUIRE(group_top == 1 || group_top == 2, "skm_route: group_top is 1 or 2");
+    if (E > ROUTE_MAX_E || k > ROUTE_MAX_K || groups > ROUTE_MAX_G || T > 4L * 0x7FFFFFFF) {
+        skm_set_error("skm_route: built for %d experts, k = %d, %d groups", ROUTE_MAX_E, ROUTE_MAX_K, ROUTE_MAX_G);
+        return SKM_ERR_UNSUPPORTED;
+    }
+    if (T == 0) return SKM_OK;
+    SkmDeviceGuard guard(ctx);
+    hipStream_t st = (hipStream_t)stream;
+    SkmProfScope ps(ctx, "k_route", st);
+    const RouteArgs a{x, T, ldx, E, k, bias, groups, group_k, group_top, scores == SKM_ROUTE_SIGMOID, renorm != 0, scale,
+                      ids, weights};
+    switch (dtype) {
+    case SKM_DT_F32: route_launch<float>(a, st); break;
+    case SKM_DT_BF16: route_launch<bf16_t>(a, st); break;
+    case SKM_DT_F16: route_launch<f16_t>(a, st); break;
+    default: route_launch<double>(a, st); break;
+    }
+    SKM_HIP(hipGetLastError());
+    return SKM_OK;
+}
+
+extern "C" int skm_route_backward(void *ctx_, const void *x, int dtype, long T, int E, long ldx, int k, int scores,
+                                  int renorm, float scale, const int32_t *ids, const float *dweights, void *dx,
+                                  void *stream)
+{
+    SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
+    SKM_REQUIRE(ctx && skm_dt_size(dtype) && T >= 0 && E >= 1 && ldx >= E && (T == 0 || (x && ids && dweights && dx)),
+                "skm_route_backward: bad argument");
+    SKM_REQUIRE(scores == SKM_ROUTE_SOFTMAX || scores == SKM_ROUTE_SIGMOID, "skm_route_backward: unknown scores %d", scores);
+    SKM_REQUIRE(k >= 1 && k <= E, "skm_route_backward: k = %d of %d experts", k, E);
+    if (E > ROUTE_MAX_E || k > ROUTE_MAX_K || T > 4L * 0x7FFFFFFF) {
+        skm_set_error("skm_route_backward: built for %d experts, k = %d", ROUTE_MAX_E, ROUTE_MAX_K);
+        return SKM_ERR_UNSUPPORTED;
+    }
+    if (T == 0) return SKM_OK;
+    SkmDeviceGuard guard(ctx);
+    hipStream_t st = (hipStream_t)stream;
+    SkmProfScope ps(ctx, "k_route_backward", st);
+    const RouteBackArgs a{x, T, ldx, E, k, ids, dweights, scores == SKM_ROUTE_SIGMOID, renorm != 0, scale, dx};
+    const dim3 grid((unsigned)((T + 3) / 4)), block(256);
+    switch (dtype) {
+    case SKM_DT_F32: hipLaunchKernelGGL((k_route_backward<float, float>), grid, block, 0, st, a); break;
+    case SKM_DT_BF16: hipLaunchKernelGGL((k_route_backward<bf16_t, float>), grid, block, 0, st, a); break;
+    case SKM_DT_F16: hipLaunchKernelGGL((k_route_backward<f16_t, float>), grid, block, 0, st, a); break;
+    default: hipLaunchKernelGGL((k_route_backward<double, double>), grid, block, 0, st, a); break;
+    }
+    SKM_HIP(hipGetLastError());
+    return SKM_OK;
+}
+
+// ------------------------------------------------------------------ plan: rows by expert, stable ------
+// The (token, slot) pairs n = t * k + j with 0 <= id < E, by expert and within an expert by n: a counting sort.
+// Every wave owns a run of `chunk` consecutive pairs; 1: its histogram; 2: where each (expert, wave) run starts;
+// 3: the waves walk their runs again, 64 pairs at a time; the rank of a pair among its equals of the 64 comes from
+// ballots over the bits of the id, so the order never depends on who is first.
+//   offsets[E + 1]  first row of an expert, [E] = number of rows
+//   pair[n]         row -> t * k + j               pos[n]  t * k + j -> row, -1 without an expert
+//   first[E + 1]    first 128-row tile of an expert (its rows from a tile's start), [E] = number of tiles
+//   tiles[.][4]     per tile: expert, first row, rows (<= 128), 0
+//   small[.][4]     the same with 16 rows a tile (NULL: none), small_count[1]
+#define PLAN_WAVES 4
+
+struct PlanArgs {
+    const int32_t *ids;
+    long n;
+    int E;
+    int chunk;              // pairs per wave, a multiple of 64
+    int nw;                 // waves (= runs)
+    int32_t *hist;          // [nw][E]: counts, then first rows
+    int32_t *offsets, *pair, *pos, *first, *tiles, *small, *small_count;
+};
+
+__device__ __forceinline__ void plan_clear(int32_t *h, int E, int lane)
+{
+    for (int e = lane; e < E; e += 64) h[e] = 0;
+}
+
+__device__ void plan_count(const PlanArgs &a, int run, int lane, int32_t *h)
+{
+    const long lo = (long)run * a.chunk, hi = lo + a.chunk < a.n ? lo + a.chunk : a.n;
+    for (long i = lo + lane; i < hi; i += 64) {
+        const int e = a.ids[i];
+        if (e >= 0 && e < a.E) atomicAdd(&h[e], 1);         // LDS, integers: the order does not matter
+    }
+}
+
+// h[e]: the row of this run's next pair of expert e
+__device__ void plan_place(const PlanArgs &a, int run, int lane, int32_t *h)
+{
+    const long lo = (long)run * a.chunk, hi = lo + a.chunk < a.n ? lo + a.chunk : a.n;
+    int bits = 1;
+    while ((1 << bits) < a.E) ++bits;
+    for (long i0 = lo; i0 < hi; i0 += 64) {
+        const long i = i0 + lane;
+        int e = i < hi ? a.ids[i] : -1;
+        const bool ok = e >= 0 && e < a.E;
+        unsigned long long same = __ballot(ok);
+        for (int b = 0; b < bits; ++b) {
+            const unsigned long long one = __ballot(ok && ((e >> b) & 1));
+            same &= ((e >> b) & 1) ? one : ~one;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        int row = -1;
+        if (ok) row = h[e] + rank;
+        __builtin_amdgcn_wave_barrier();                    // all lanes have read before the last of each kind writes
+        if (ok && rank == __popcll(same) - 1) h[e] = row + 1;
+        __builtin_amdgcn_wave_barrier();
+        if (i < hi) a.pos[i] = row;
+        if (ok) a.pair[row] = (int32_t)i;
+    }
+}
+
+// exclusive prefix over the experts of v (one value per thread and round of blockDim), all threads call it
+__device__ int plan_scan_block(int v, int *sh, int &total)
+{
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+    int s = v;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) {
+        const int o = __shfl_up(s, m);
+        if (lane >= m) s += o;
+    }
+    if (lane == 63) sh[wave] = s;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+    for (int w = 0; w < waves; ++w) {
+        if (w < wave) before += sh[w];
+        total += sh[w];
+    }
+    __syncthreads();
+    return before + s - v;
+}
+
+// From the histograms of all runs to the first row of every (run, expert), and the tile tables.  One workgroup.
+__device__ void plan_scan(const PlanArgs &a, int32_t *hist, int *sh)
+{
+    int rows0 = 0, tiles0 = 0, small0 = 0;
+    for (int e0 = 0; e0 < a.E; e0 += blockDim.x) {
+        const int e = e0 + threadIdx.x;
+        int count = 0;
+        if (e < a.E)
+            for (int r = 0; r < a.nw; ++r) count += hist[(long)r * a.E + e];
+        int nrows, ntiles, nsmall;
+        const int off = rows0 + plan_scan_block(count, sh, nrows);
+        const int t0 = tiles0 + plan_scan_block((count + 127) / 128, sh, ntiles);
+        const int s0 = small0 + plan_scan_block((count + 15) / 16, sh, nsmall);
+        rows0 += nrows;
+        tiles0 += ntiles;
+        small0 += nsmall;
+        if (e < a.E) {
+            a.offsets[e] = off;
+            a.first[e] = t0;
+            int at = off;
+            for (int r = 0; r < a.nw; ++r) {
+                const int c = hist[(long)r * a.E + e];
+                hist[(long)r * a.E + e] = at;
+                at += c;
+            }
+            for (int t = 0; t * 128 < count; ++t) {
+                int32_t *d = a.tiles + (long)(t0 + t) * 4;
+                d[0] = e; d[1] = off + t * 128; d[2] = count - t * 128 < 128 ? count - t * 128 : 128; d[3] = 0;
+            }
+            if (a.small)
+                for (int t = 0; t * 16 < count; ++t) {
+                    int32_t *d = a.small + (long)(s0 + t) * 4;
+                    d[0] = e; d[1] = off + t * 16; d[2] = count - t * 16 < 16 ? count - t * 16 : 16; d[3] = 0;
+                }
+        }
+    }
+    if (threadIdx.x == 0) {
+        a.offsets[a.E] = rows0;
+        a.first[a.E] = tiles0;
+        if (a.small) a.small_count[0] = small0;
+    }
+}
+
+// few pairs: everything in one workgroup, the histograms in LDS (nw = PLAN_WAVES)
+__global__ __launch_bounds__(64 * PLAN_WAVES) void k_plan_one(PlanArgs a)
+{
+    extern __shared__ int32_t lds[];
+    __shared__ int sh[PLAN_WAVES];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int32_t *h = lds + (long)wave * a.E;
+    plan_clear(h, a.E, lane);
+    __syncthreads();
+    plan_count(a, wave, lane, h);
+    __syncthreads();
+    plan_scan(a, lds, sh);
+    __syncthreads();
+    plan_place(a, wave, lane, h);
+}
+
+__global__ __launch_bounds__(64) void k_plan_count(PlanArgs a)
+{
+    extern __shared__ int32_t lds[];
+    plan_clear(lds, a.E, threadIdx.x);
+    __syncthreads();
+    plan_count(a, blockIdx.x, threadIdx.x, lds);
+    __syncthreads();
+    for (int e = threadIdx.x; e < a.E; e += 64) a.hist[(long)blockIdx.x * a.E + e] = lds[e];
+}
+
+__global__ __launch_bounds__(1024) void k_plan_scan(PlanArgs a)
+{
+    __shared__ int sh[16];
+    plan_scan(a, a.hist, sh);
+}
+
+__global__ __launch_bounds__(64) void k_plan_place(PlanArgs a)
+{
+    extern __shared__ int32_t lds[];
+    for (int e = threadIdx.x; e < a.E; e += 64) lds[e] = a.hist[(long)blockIdx.x * a.E + e];
+    __syncthreads();
+    plan_place(a, blockIdx.x, threadIdx.x, lds);
+}
+
+// few enough for one workgroup: 4 runs of up to 1024 pairs, 32 KB of histograms
+static bool plan_is_one(long n, int E) { return n <= 4096 && E <= 2048; }
+
+static int plan_runs(long n, int E, int *chunk)
+{
+    if (plan_is_one(n, E)) {
+        *chunk = (int)((n + PLAN_WAVES - 1) / PLAN_WAVES + 63) / 64 * 64;
+        return PLAN_WAVES;
+    }
+    long c = (n + 511) / 512;               // at most 512 runs
+    if (c < 512) c = 512;
+    c = (c + 63) / 64 * 64;
+    *chunk = (int)c;
+    return (int)((n + c - 1) / c);
+}
+
+extern "C" size_t skm_route_plan_workspace_bytes(long n, int E)
+{
+    if (n <= 0 || E <= 0 || plan_is_one(n, E)) return 0;
+    int chunk;
+    return (size_t)plan_runs(n, E, &chunk) * (size_t)E * 4;
+}
+
+extern "C" long skm_route_plan_tiles(long n, int E, int rows)
+{
+    if (n < 0 || E < 1 || rows < 1) return 0;
+    return n / rows + (n < E ? n : E);      // every expert adds less than one tile to its full ones
+}
+
+extern "C" int skm_route_plan(void *ctx_, const int32_t *ids, long n, int E, int32_t *offsets, int32_t *pair,
+                              int32_t *pos, int32_t *first, int32_t *tiles, int32_t *small_tiles, int32_t *small_count,
+                              void *ws, size_t ws_bytes, void *stream)
+{
+    SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
+    SKM_REQUIRE(ctx && n >= 0 && E >= 1 && offsets && first && (n == 0 || (ids && pair && pos && tiles)) &&
+                    (!small_tiles || small_count),
+                "skm_route_plan: bad argument");
+    if (E > ROUTE_MAX_E || n > 0x3FFFFFFF) {
+        skm_set_error("skm_route_plan: built for %d experts and 2^30 - 1 pairs", ROUTE_MAX_E);
+        return SKM_ERR_UNSUPPORTED;
+    }
+    if (ws_bytes < skm_route_plan_workspace_bytes(n, E) || (skm_route_plan_workspace_bytes(n, E) && !ws)) {
+        skm_set_error("skm_route_plan: workspace too small");
+        return SKM_ERR_WORKSPACE;
+    }
+    SkmDeviceGuard guard(ctx);
+    hipStream_t st = (hipStream_t)stream;
+    PlanArgs a{ids, n, E, 0, 0, static_cast<int32_t *>(ws), offsets, pair, pos, first, tiles, small_tiles, small_count};
+    a.nw = plan_runs(n, E, &a.chunk);
+    SkmProfScope ps(ctx, "k_plan", st);
+    if (plan_is_one(n, E)) {
+        hipLaunchKernelGGL(k_plan_one, dim3(1), dim3(64 * PLAN_WAVES), (size_t)PLAN_WAVES * E * 4, st, a);
+    } else {
+        hipLaunchKernelGGL(k_plan_count, dim3((unsigned)a.nw), dim3(64), (size_t)E * 4, st, a);
+        hipLaunchKernelGGL(k_plan_scan, dim3(1), dim3(1024), 0, st, a);
+        hipLaunchKernelGGL(k_plan_place, dim3((unsigned)a.nw), dim3(64), (size_t)E * 4, st, a);
+    }
+    SKM_HIP(hipGetLastError());
+    return SKM_OK;
+}
+
+// ------------------------------------------------------------------ weighted sum of the experts' rows ------
+struct CombineArgs {
+    const void *rows;       // [.][N]
+    const int32_t *pos;     // [T][k]
+    const float *w;         // [T][k]
+    long T;
+    int k, N;
+    void *out;              // [T][N]
+    const void *dout;
+    float *dw;
+};
+
+// out[t] = sum_j w[t][j] rows[pos[t][j]], in the order of j, float32.  An empty place adds w * 0: nothing, or the NaN
+// that a row without a choice carries in its weights.
+template <typename TR, typename TO, int VEC>
+__global__ __launch_bounds__(256) void k_route_combine(CombineArgs a)
+{
+    const long per = (a.N + VEC - 1) / VEC;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= a.T * per) return;
+    const long t = i / per;
+    const int c = (int)(i - t * per) * VEC;
+    typedef TR vr __attribute__((ext_vector_type(VEC)));
+    typedef TO vo __attribute__((ext_vector_type(VEC)));
+    float s[VEC];
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) s[q] = 0.f;
+    for (int j = 0; j < a.k; ++j) {
+        const int p = a.pos[t * a.k + j];
+        const float w = a.w[t * a.k + j];
+        if (p < 0) {
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) s[q] += w * 0.f;
+            continue;
+        }
+        const vr v = *reinterpret_cast<const vr *>(static_cast<const TR *>(a.rows) + (long)p * a.N + c);
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) s[q] += w * (float)v[q];
+    }
+    vo o;
+#pragma unroll
+    for (int q = 0; q < VEC; ++q) o[q] = (TO)s[q];
+    *reinterpret_cast<vo *>(static_cast<TO *>(a.out) + t * a.N + c) = o;
+}
+
+// dw[t][j] = <dout[t], rows[pos[t][j]]>: one wave per pair
+template <typename TR, typename TO>
+__global__ __launch_bounds__(256) void k_route_combine_backward(CombineArgs a)
+{
+    const int lane = threadIdx.x & 63;
+    const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i >= a.T * a.k) return;
+    const int p = a.pos[i];
+    float s = 0.f;
+    if (p >= 0) {
+        const TR *r = static_cast<const TR *>(a.rows) + (long)p * a.N;
+        const TO *d = static_cast<const TO *>(a.dout) + (i / a.k) * a.N;
+        for (int c = lane; c < a.N; c += 64) s += (float)r[c] * (float)d[c];
+        s = wave_sum(s);
+    }
+    if (lane == 0) a.dw[i] = s;
+}
+
+template <typename TR, typename TO>
+static void combine_launch(const CombineArgs &a, hipStream_t st)
+{
+    const bool vec = a.N % 4 == 0 && (((uintptr_t)a.rows | (uintptr_t)a.out) & 15) == 0;
+    const long n = a.T * (vec ? a.N / 4 : a.N);
+    const dim3 grid((unsigned)((n + 255) / 256));
+    if (vec) hipLaunchKernelGGL((k_route_combine<TR, TO, 4>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_route_combine<TR, TO, 1>), grid, dim3(256), 0, st, a);
+}
+
+template <typename TR, typename TO>
+static void combine_back_launch(const CombineArgs &a, hipStream_t st)
+{
+    hipLaunchKernelGGL((k_route_combine_backward<TR, TO>), dim3((unsigned)((a.T * a.k + 3) / 4)), dim3(256), 0, st, a);
+}
+
+#define COMBINE_TYPES(F, TR_CODE, TO_CODE)                                                                       \
+    switch ((TR_CODE) * 4 + (TO_CODE)) {                                                                         \
+    case SKM_DT_F32 * 4 + SKM_DT_F32: F<float, float>(a, st); break;                                             \
+    case SKM_DT_F32 * 4 + SKM_DT_BF16: F<float, bf16_t>(a, st); break;                                           \
+    case SKM_DT_F32 * 4 + SKM_DT_F16: F<float, f16_t>(a, st); break;                                             \
+    case SKM_DT_BF16 * 4 + SKM_DT_F32: F<bf16_t, float>(a, st); break;                                           \
+    case SKM_DT_BF16 * 4 + SKM_DT_BF16: F<bf16_t, bf16_t>(a, st); break;                                         \
+    case SKM_DT_F16 * 4 + SKM_DT_F32: F<f16_t, float>(a, st); break;                                             \
+    case SKM_DT_F16 * 4 + SKM_DT_F16: F<f16_t, f16_t>(a, st); break;                                             \
+    default: skm_set_error("rows of type %d and result of type %d do not go together", (int)(TR_CODE), (int)(TO_CODE)); \
+             return SKM_ERR_UNSUPPORTED;                                                                         \
+    }
+
+extern "C" int skm_route_combine(void *ctx_, const void *rows, int rows_dtype, const int32_t *pos, const float *weights,
+                                 long T, int k, int N, void *out, int out_dtype, void *stream)
+{
+    SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
+    SKM_REQUIRE(ctx && T >= 0 && k >= 1 && N >= 1 && (T == 0 || (rows && pos && weights && out)),
+                "skm_route_combine: bad argument");
+    SKM_REQUIRE(T * N < 0x7FFFFFFFL * 256, "skm_route_combine: too many elements");
+    if (T == 0) return SKM_OK;
+    SkmDeviceGuard guard(ctx);
+    hipStream_t st = (hipStream_t)stream;
+    SkmProfScope ps(ctx, "k_route_combine", st);
+    const CombineArgs a{rows, pos, weights, T, k, N, out, nullptr, nullptr};
+    COMBINE_TYPES(combine_launch, rows_dtype, out_dtype)
+    SKM_HIP(hipGetLastError());
+    return SKM_OK;
+}
+
+extern "C" int skm_route_combine_backward(void *ctx_, const void *rows, int rows_dtype, const int32_t *pos,
+                                          const void *dout, int dout_dtype, long T, int k, int N, float *dweights,
+                                          void *stream)
+{
+    SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
+    SKM_REQUIRE(ctx && T >= 0 && k >= 1 && N >= 1 && (T == 0 || (rows && pos && dout && dweights)),
+                "skm_route_combine_backward: bad argument");
+    SKM_REQUIRE(T * k < 0x7FFFFFFFL * 4, "skm_route_combine_backward: too many pairs");
+    if (T == 0) return SKM_OK;
+    SkmDeviceGuard guard(ctx);
+    hipStream_t st = (hipStream_t)stream;
+    SkmProfScope ps(ctx, "k_route_combine_backward", st);
+    const CombineArgs a{rows, pos, nullptr, T, k, N, nullptr, dout, dweights};
+    COMBINE_TYPES(combine_back_launch, rows_dtype, dout_dtype)
+    SKM_HIP(hipGetLastError());
+    return SKM_OK;
+}

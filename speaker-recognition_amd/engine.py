@@ -100,6 +100,34 @@ SIGNATURES = {
     "skm_feat_postproc": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_long, _c_void_p, _c_int, _c_void_p, _c_void_p,
                                    _c_int, _c_long, _c_int, _c_int, _dp, _c_int, _c_void_p, _c_void_p, _c_int, _c_void_p,
                                    _c_int, _c_void_p, _c_void_p, _c_void_p, _c_size_t, _c_void_p]),
+    # routing and 8-bit products
+    "skm_route": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_long, _c_int, _c_long, _c_int, _c_int, _c_void_p, _c_int,
+                           _c_int, _c_int, _c_int, ctypes.c_float, _c_void_p, _c_void_p, _c_void_p]),
+    "skm_route_backward": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_long, _c_int, _c_long, _c_int, _c_int, _c_int,
+                                    ctypes.c_float, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "skm_route_plan_workspace_bytes": (_c_size_t, [_c_long, _c_int]),
+    "skm_route_plan_tiles": (_c_long, [_c_long, _c_int, _c_int]),
+    "skm_route_plan": (_c_int, [_c_void_p, _c_void_p, _c_long, _c_int] + [_c_void_p] * 8 + [_c_size_t, _c_void_p]),
+    "skm_route_combine": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_long, _c_int, _c_int,
+                                   _c_void_p, _c_int, _c_void_p]),
+    "skm_route_combine_backward": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_long,
+                                            _c_int, _c_int, _c_void_p, _c_void_p]),
+    "skm_fp8_row_bytes": (_c_long, [_c_long]),
+    "skm_fp8_scale_bytes": (_c_long, [_c_long]),
+    "skm_fp8_rows": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_long, _c_int, _c_long, _c_int, _c_void_p, _c_void_p,
+                              _c_void_p]),
+    "skm_fp8_tiles": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_long, _c_long, _c_int,
+                               _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "skm_fp8_columns": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_long, _c_int, _c_long, _c_int, _c_void_p, _c_void_p,
+                                 _c_long, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
+    "skm_gemm_fp8_workspace_bytes": (_c_size_t, [_c_void_p, _c_int, _c_int, _c_int]),
+    "skm_gemm_fp8": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_int,
+                              _c_int, _c_void_p, _c_int, _c_long, _c_int, _c_void_p, _c_size_t, _c_void_p]),
+    "skm_gemm_fp8_experts": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_int,
+                                      _c_int, _c_int, _c_void_p, _c_int, _c_long, _c_void_p, _c_void_p, _c_void_p,
+                                      _c_void_p, _c_void_p, _c_int, _c_void_p]),
+    "skm_gemm_fp8_experts_wgrad": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int,
+                                            _c_int, _c_int, _c_int, _c_void_p, _c_long, _c_void_p, _c_int, _c_void_p]),
     # one process, several GPUs (team.py)
     "skm_comm_init_all": (_c_int, [_c_int, ctypes.POINTER(_c_int), ctypes.POINTER(_c_void_p)]),
     "skm_comm_size": (_c_int, [_c_void_p]),
@@ -170,6 +198,7 @@ class HipEngine(object):
         self.ctx = ctx
         self._ws = None
         self._ws_bytes = 0
+        self._dt_codes = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2, torch.float64: 3}   # SKM_DT_*
 
         _live_engines.add(self)
 
@@ -905,6 +934,266 @@ class HipEngine(object):
         return F
 
     # ------------------------------------------------------------------ per-kernel timing (HIP events)
+    # ------------------------------------------------------------------ routing and 8-bit products
+    def _dt(self, dtype, allowed, what):
+        """the SKM_DT_* code of a torch type, among the `allowed` codes"""
+        code = self._dt_codes.get(dtype)
+        if code is None or code not in allowed:
+            raise SkmError("%s: type %s" % (what, dtype))
+        return code
+
+    def _matrix(self, t, what, rows=None, cols=None, dtypes=None):
+        """a device matrix with unit stride along its rows; returns the distance between them"""
+        if not isinstance(t, self.torch.Tensor) or t.device != self.device or t.dim() != 2:
+            raise SkmError("%s: a 2-D tensor on %s is wanted" % (what, self.device))
+        if (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
+            raise SkmError("%s: shape %s, wanted %s x %s" % (what, tuple(t.shape), rows, cols))
+        if dtypes is not None and t.dtype not in dtypes:
+            raise SkmError("%s: type %s" % (what, t.dtype))
+        n, m = t.shape
+        if n == 0 or m == 0:
+            return m
+        ld = t.stride(0) if n > 1 else m
+        if (m > 1 and t.stride(1) != 1) or ld < m:
+            raise SkmError("%s: rows have to be contiguous (strides %s)" % (what, tuple(t.stride())))
+        return ld
+
+    def _dense(self, t, what, rows, cols, dtypes):
+        if self._matrix(t, what, rows, cols, dtypes) != cols:
+            raise SkmError("%s: a contiguous tensor is wanted" % what)
+        return t
+
+    def _vector(self, t, what, n, dtype):
+        if not isinstance(t, self.torch.Tensor) or t.device != self.device or t.dtype != dtype or tuple(t.shape) != (n,) \
+                or not t.is_contiguous():
+            raise SkmError("%s: a contiguous %s tensor of %d on %s is wanted" % (what, dtype, n, self.device))
+        return t
+
+    @staticmethod
+    def _scores(scores):
+        if scores not in ("softmax", "sigmoid"):
+            raise SkmError("scores: 'softmax' or 'sigmoid', not %r" % (scores,))
+        return 1 if scores == "sigmoid" else 0
+
+    def route(self, logits, k, scores="softmax", bias=None, groups=1, group_k=None, group_top=2, renorm=True, scale=1.0):
+        """The k best of E experts (components) for each row of the T x E logits (float32, bfloat16, float16 or, as
+        `logprob` returns them, float64) and their weights (skm_route).  `bias` (E float32) takes part in the choice, not
+        in the weights; with `groups` only experts of the `group_k` best groups are chosen.  -inf masks an expert.
+        Returns (ids int32 T x k, -1 where none was left; weights float32 T x k)."""
+        torch = self.torch
+        ldx = self._matrix(logits, "route: logits")
+        T, E = logits.shape
+        if bias is not None:
+            self._vector(bias, "route: bias", E, torch.float32)
+        k = int(k)
+        ids = torch.empty((T, max(k, 0)), dtype=torch.int32, device=self.device)
+        weights = torch.empty((T, max(k, 0)), dtype=torch.float32, device=self.device)
+        self._check(self.lib.skm_route(
+            self.ctx, logits.data_ptr(), self._dt(logits.dtype, (0, 1, 2, 3), "route: logits"), T, E, ldx, k,
+            self._scores(scores), bias.data_ptr() if bias is not None else None, int(groups),
+            int(groups if group_k is None else group_k), int(group_top), 1 if renorm else 0, float(scale),
+            ids.data_ptr(), weights.data_ptr(), self._stream()))
+        return ids, weights
+
+    def route_backward(self, logits, ids, dweights, scores="softmax", renorm=True, scale=1.0):
+        """Gradient of the logits (their type) from that of route's weights (skm_route_backward)."""
+        torch = self.torch
+        ldx = self._matrix(logits, "route_backward: logits")
+        T, E = logits.shape
+        k = ids.shape[-1]
+        self._dense(ids, "route_backward: ids", T, k, (torch.int32,))
+        self._dense(dweights, "route_backward: dweights", T, k, (torch.float32,))
+        dx = torch.empty((T, E), dtype=logits.dtype, device=self.device)
+        self._check(self.lib.skm_route_backward(
+            self.ctx, logits.data_ptr(), self._dt(logits.dtype, (0, 1, 2, 3), "route_backward: logits"), T, E, ldx, k,
+            self._scores(scores), 1 if renorm else 0, float(scale), ids.data_ptr(), dweights.data_ptr(), dx.data_ptr(),
+            self._stream()))
+        return dx
+
+    def route_plan(self, ids, E):
+        """The order in which the products of E experts take the rows that `ids` (int32 T x k, anything outside
+        0 .. E - 1 = no expert) chose: a RoutePlan (skm_route_plan)."""
+        torch = self.torch
+        E = int(E)
+        if not isinstance(ids, torch.Tensor) or ids.dim() != 2:
+            raise SkmError("route_plan: ids T x k are wanted")
+        T, k = ids.shape
+        self._dense(ids, "route_plan: ids", T, k, (torch.int32,))
+        if E < 1 or k < 1:
+            raise SkmError("route_plan: %d experts, %d places" % (E, k))
+        plan = RoutePlan(self, T, k, E)
+        need = self.lib.skm_route_plan_workspace_bytes(plan.n, E)
+        ws = torch.empty(int(need), dtype=torch.uint8, device=self.device) if need else None
+        p = plan._ptr
+        self._check(self.lib.skm_route_plan(
+            self.ctx, ids.data_ptr(), plan.n, E, p("offsets"), p("pair"), p("pos"), p("first"), p("tiles"),
+            p("small_tiles") if plan.few else None, p("small_count") if plan.few else None,
+            ws.data_ptr() if need else None, need, self._stream()))
+        return plan
+
+    def route_combine(self, rows, weights, plan, dtype=None):
+        """out[t] = sum_j weights[t, j] rows[the plan's row of (t, j)] in `dtype` (default: that of rows)."""
+        torch = self.torch
+        N = rows.shape[-1]
+        self._dense(rows, "route_combine: rows", plan.n, N, None)
+        self._dense(weights, "route_combine: weights", plan.T, plan.k, (torch.float32,))
+        dtype = dtype or rows.dtype
+        out = torch.empty((plan.T, N), dtype=dtype, device=self.device)
+        self._check(self.lib.skm_route_combine(
+            self.ctx, rows.data_ptr(), self._dt(rows.dtype, (0, 1, 2), "route_combine: rows"), plan._ptr("pos"),
+            weights.data_ptr(), plan.T, plan.k, N, out.data_ptr(), self._dt(dtype, (0, 1, 2), "route_combine"),
+            self._stream()))
+        return out
+
+    def route_combine_backward(self, rows, dout, plan):
+        """Gradient of route_combine's weights (float32 T x k)."""
+        torch = self.torch
+        N = rows.shape[-1]
+        self._dense(rows, "route_combine_backward: rows", plan.n, N, None)
+        self._dense(dout, "route_combine_backward: dout", plan.T, N, None)
+        dw = torch.empty((plan.T, plan.k), dtype=torch.float32, device=self.device)
+        self._check(self.lib.skm_route_combine_backward(
+            self.ctx, rows.data_ptr(), self._dt(rows.dtype, (0, 1, 2), "route_combine_backward: rows"), plan._ptr("pos"),
+            dout.data_ptr(), self._dt(dout.dtype, (0, 1, 2), "route_combine_backward: dout"), plan.T, plan.k, N,
+            dw.data_ptr(), self._stream()))
+        return dw
+
+    @staticmethod
+    def _fmt(fmt):
+        if fmt not in ("e4m3", "e5m2"):
+            raise SkmError("8-bit format: 'e4m3' or 'e5m2', not %r" % (fmt,))
+        return 1 if fmt == "e5m2" else 0
+
+    def fp8_rows(self, x, fmt="e4m3"):
+        """x (M x K; float32, bfloat16, float16) in 8-bit floats, a scale for each 128 along a row: an Fp8Matrix."""
+        ldx = self._matrix(x, "fp8_rows: x")
+        M, K = x.shape
+        if K < 1:
+            raise SkmError("fp8_rows: rows of no elements")
+        out = Fp8Matrix(self, (M,), K, fmt)
+        self._check(self.lib.skm_fp8_rows(self.ctx, x.data_ptr(), self._dt(x.dtype, (0, 1, 2), "fp8_rows: x"), M, K, ldx,
+                                          self._fmt(fmt), out.q.data_ptr(), out.s.data_ptr(), self._stream()))
+        return out
+
+    def fp8_tiles(self, w, fmt="e4m3", transposed=False):
+        """w (N x K, or E x N x K) in 8-bit floats, a scale for each 128 x 128: an Fp8Matrix, with `transposed` the pair
+        (w, its transpose: the same numbers, K x N) that a training step needs."""
+        torch = self.torch
+        if not isinstance(w, torch.Tensor) or w.dim() not in (2, 3) or w.device != self.device or not w.is_contiguous():
+            raise SkmError("fp8_tiles: a contiguous tensor N x K or E x N x K on %s is wanted" % self.device)
+        N, K = w.shape[-2:]
+        batch = tuple(w.shape[:-2])
+        if N < 1 or K < 1:
+            raise SkmError("fp8_tiles: shape %s" % (tuple(w.shape),))
+        out = Fp8Matrix(self, batch + (N,), K, fmt)
+        outt = Fp8Matrix(self, batch + (K,), N, fmt) if transposed else None
+        self._check(self.lib.skm_fp8_tiles(
+            self.ctx, w.data_ptr(), self._dt(w.dtype, (0, 1, 2), "fp8_tiles: w"), batch[0] if batch else 1, N, K, K, N * K,
+            self._fmt(fmt), out.q.data_ptr(), out.s.data_ptr(), outt.q.data_ptr() if transposed else None,
+            outt.s.data_ptr() if transposed else None, self._stream()))
+        return (out, outt) if transposed else out
+
+    def fp8_columns(self, x, fmt="e4m3", plan=None, weights=None):
+        """The transpose of x (R x C) in 8-bit floats, a scale for each 128 rows of a column, for products over the rows.
+        With a plan: the rows of its pairs (x holds a row per token), times `weights` (float32 T x k) if given, every
+        expert's from a new block: for gemm_fp8_experts_wgrad."""
+        torch = self.torch
+        ldx = self._matrix(x, "fp8_columns: x", rows=plan.T if plan is not None else None)
+        R, C = x.shape
+        if C < 1 or (R < 1 and plan is None):
+            raise SkmError("fp8_columns: shape %s" % (tuple(x.shape),))
+        if weights is not None:
+            if plan is None:
+                raise SkmError("fp8_columns: weights go with a plan")
+            self._dense(weights, "fp8_columns: weights", plan.T, plan.k, (torch.float32,))
+        out = Fp8Matrix(self, (C,), plan.max_tiles * 128 if plan is not None else R, fmt)
+        out.plan = plan
+        self._check(self.lib.skm_fp8_columns(
+            self.ctx, x.data_ptr(), self._dt(x.dtype, (0, 1, 2), "fp8_columns: x"), R, C, ldx, self._fmt(fmt),
+            plan._ptr("tiles") if plan is not None else None, plan._ptr("tile_count") if plan is not None else None,
+            plan.max_tiles if plan is not None else 0, plan._ptr("pair") if plan is not None else None,
+            plan.k if plan is not None else 0, weights.data_ptr() if weights is not None else None, out.q.data_ptr(),
+            out.s.data_ptr(), self._stream()))
+        return out
+
+    def _fp8(self, m, what, dims=1):
+        if not isinstance(m, Fp8Matrix) or m.q.device != self.device or len(m.shape) != dims + 1:
+            raise SkmError("%s: an Fp8Matrix of %d dimensions on %s is wanted" % (what, dims + 1, self.device))
+        return m
+
+    def gemm_fp8(self, A, B, dtype=None, out=None, accumulate=False):
+        """A B' of two Fp8Matrix [M x K], [N x K] (skm_gemm_fp8); a float matrix A is taken through fp8_rows.  The result
+        (M x N) is of type `dtype` (default bfloat16), or goes to `out` (rows may be apart), added to it with
+        `accumulate`."""
+        torch = self.torch
+        if isinstance(A, torch.Tensor):
+            A = self.fp8_rows(A)
+        self._fp8(A, "gemm_fp8: A")
+        self._fp8(B, "gemm_fp8: B")
+        if A.plan is not None or B.plan is not None:
+            raise SkmError("gemm_fp8: columns in a plan's order go to gemm_fp8_experts_wgrad")
+        M, K = A.shape
+        N = B.shape[0]
+        if B.shape[1] != K:
+            raise SkmError("gemm_fp8: K = %d and %d" % (K, B.shape[1]))
+        if out is None:
+            if accumulate:
+                raise SkmError("gemm_fp8: accumulate without out")
+            out = torch.empty((M, N), dtype=dtype or torch.bfloat16, device=self.device)
+            ldc = N
+        else:
+            ldc = self._matrix(out, "gemm_fp8: out", M, N, (dtype,) if dtype is not None else None)
+        need = self.lib.skm_gemm_fp8_workspace_bytes(self.ctx, M, N, K)
+        ws = torch.empty(int(need), dtype=torch.uint8, device=self.device) if need else None
+        self._check(self.lib.skm_gemm_fp8(
+            self.ctx, A.q.data_ptr(), A.s.data_ptr(), A.code, B.q.data_ptr(), B.s.data_ptr(), B.code, M, N, K,
+            out.data_ptr(), self._dt(out.dtype, (0, 1, 2), "gemm_fp8"), ldc, 1 if accumulate else 0,
+            ws.data_ptr() if need else None, need, self._stream()))
+        return out
+
+    def gemm_fp8_experts(self, A, W, plan, dtype=None):
+        """The experts' products in the plan's order: row r of the result (plan.n x N, rows behind the plan's last are
+        not written) is W[expert of r] times the row of A: of the pair's token where A has plan.T rows (a float matrix is
+        taken through fp8_rows), of r itself where it has plan.n and the plan more than one place.  W: Fp8Matrix E x N x K."""
+        torch = self.torch
+        if isinstance(A, torch.Tensor):
+            A = self.fp8_rows(A)
+        self._fp8(A, "gemm_fp8_experts: A")
+        self._fp8(W, "gemm_fp8_experts: W", 2)
+        E, N, K = W.shape
+        if E != plan.E or A.shape[1] != K or A.plan is not None or A.shape[0] not in (plan.T, plan.n):
+            raise SkmError("gemm_fp8_experts: A %s, W %s, a plan of %d x %d pairs over %d experts"
+                           % (A.shape, W.shape, plan.T, plan.k, plan.E))
+        dtype = dtype or torch.bfloat16
+        out = torch.empty((plan.n, N), dtype=dtype, device=self.device)
+        self._check(self.lib.skm_gemm_fp8_experts(
+            self.ctx, A.q.data_ptr(), A.s.data_ptr(), A.code, W.q.data_ptr(), W.s.data_ptr(), W.code, E, N, K,
+            plan._ptr("pair"), plan.k if A.shape[0] == plan.T else 0, plan.n, plan._ptr("first"), plan._ptr("tiles"),
+            plan._ptr("small_tiles") if plan.few else None, plan._ptr("small_count") if plan.few else None,
+            out.data_ptr(), self._dt(dtype, (0, 1, 2), "gemm_fp8_experts"), self._stream()))
+        return out
+
+    def gemm_fp8_experts_wgrad(self, A, B, plan, out=None, accumulate=False):
+        """float32 E x M x N: for each expert A B' over its rows, A (M) and B (N) from fp8_columns with this plan."""
+        torch = self.torch
+        self._fp8(A, "gemm_fp8_experts_wgrad: A")
+        self._fp8(B, "gemm_fp8_experts_wgrad: B")
+        if A.plan is not plan or B.plan is not plan:
+            raise SkmError("gemm_fp8_experts_wgrad: A and B come from fp8_columns with this plan")
+        M, N = A.shape[0], B.shape[0]
+        if out is None:
+            if accumulate:
+                raise SkmError("gemm_fp8_experts_wgrad: accumulate without out")
+            out = torch.empty((plan.E, M, N), dtype=torch.float32, device=self.device)
+        elif tuple(out.shape) != (plan.E, M, N) or out.dtype != torch.float32 or out.device != self.device \
+                or not out.is_contiguous():
+            raise SkmError("gemm_fp8_experts_wgrad: out is a contiguous float32 tensor %s" % ((plan.E, M, N),))
+        self._check(self.lib.skm_gemm_fp8_experts_wgrad(
+            self.ctx, A.q.data_ptr(), A.s.data_ptr(), A.code, B.q.data_ptr(), B.s.data_ptr(), B.code, plan.E, M, N,
+            plan._ptr("first"), plan.max_tiles, out.data_ptr(), 1 if accumulate else 0, self._stream()))
+        return out
+
+    # ------------------------------------------------------------------ profiling, copies
     def profile(self, on):
         self._check(self.lib.skm_prof_enable(self.ctx, 1 if on else 0))
 
@@ -1084,6 +1373,67 @@ class HipEngine(object):
 
     def synchronize(self):
         self.torch.cuda.synchronize(self.device)
+
+
+class Fp8Matrix(object):
+    """A matrix of 8-bit floats with a power-of-two scale for each block of 128 along its rows (include/skm.h): `q` uint8
+    [.., rows, K rounded up to 128], `s` uint8 [.., rows, blocks rounded up to 4]."""
+
+    def __init__(self, engine, rows, K, fmt):
+        torch = engine.torch
+        self.code = engine._fmt(fmt)
+        self.fmt = fmt
+        self.shape = tuple(rows) + (K,)
+        self.plan = None            # the plan whose order the columns are in
+        kp = (K + 127) // 128 * 128
+        self.q = torch.empty(tuple(rows) + (kp,), dtype=torch.uint8, device=engine.device)
+        self.s = torch.empty(tuple(rows) + ((kp // 128 + 3) // 4 * 4,), dtype=torch.uint8, device=engine.device)
+
+    def values(self):
+        """the numbers it stands for, float32 [.., rows, K]"""
+        import torch
+        K = self.shape[-1]
+        f8 = torch.float8_e5m2 if self.code else torch.float8_e4m3fn
+        e = self.s[..., :self.q.shape[-1] // 128].to(torch.int32)
+        # 2^(byte - 127) from its bits (the byte is 17 at least)
+        scale = (e << 23).view(torch.float32)
+        v = self.q.view(f8).to(torch.float32).reshape(self.q.shape[:-1] + (-1, 128)) * scale[..., None]
+        return v.reshape(self.q.shape)[..., :K]
+
+
+class RoutePlan(object):
+    """Rows of the experts' products (include/skm.h: skm_route_plan): device int32 tensors in one allocation, `offsets`
+    [E + 1], `pair` [n], `pos` [T, k], `first` [E + 1], `tiles` [max_tiles, 4]."""
+
+    def __init__(self, engine, T, k, E):
+        self.engine, self.T, self.k, self.E, self.n = engine, T, k, E, T * k
+        if self.n > 0x3FFFFFFF:
+            raise SkmError("route_plan: %d pairs" % self.n)
+        self.max_tiles = engine.lib.skm_route_plan_tiles(self.n, E, 128)
+        # up to 16 rows an expert on average the products stream the weights past 16 rows at a time
+        self.few = self.n <= 16 * E
+        small = engine.lib.skm_route_plan_tiles(self.n, E, 16) if self.few else 0
+        self._at, at = {}, 0
+        for name, size in (("offsets", E + 1), ("pair", self.n), ("pos", self.n), ("first", E + 1),
+                           ("tiles", 4 * self.max_tiles), ("small_tiles", 4 * small), ("small_count", 1)):
+            self._at[name] = (at, size)
+            at += (size + 3) // 4 * 4
+        self._at["tile_count"] = (self._at["first"][0] + E, 1)
+        self._buf = engine.torch.empty(at, dtype=engine.torch.int32, device=engine.device)
+        self._base = self._buf.data_ptr()
+
+    def _ptr(self, name):
+        return self._base + 4 * self._at[name][0]
+
+    def _view(self, name):
+        at, size = self._at[name]
+        return self._buf[at:at + size]
+
+    offsets = property(lambda self: self._view("offsets"))
+    pair = property(lambda self: self._view("pair"))
+    pos = property(lambda self: self._view("pos").view(self.T, self.k))
+    first = property(lambda self: self._view("first"))
+    tiles = property(lambda self: self._view("tiles").view(-1, 4))
 
 
 class PackedGMM(object):
