@@ -496,22 +496,30 @@ int skm_fp8_columns(void *ctx, const void *x_dev, int dtype, long R, int C, long
                     const int32_t *tile_count_dev, long max_tiles, const int32_t *pair_dev, int slots,
                     const float *weights_dev, void *qt_dev, void *st_dev, void *stream);
 
-/* C[M][ldc] (+)= A B' of two such matrices [M][K], [N][K] (any of the three block shapes, either format), float32 sums.
- * C float32, bf16 or f16; accumulate adds to what is there, before the rounding to C's type. */
-size_t skm_gemm_fp8_workspace_bytes(void *ctx, int M, int N, int K);
-int skm_gemm_fp8(void *ctx, const void *A_dev, const void *sA_dev, int fmt_a, const void *B_dev, const void *sB_dev,
-                 int fmt_b, int M, int N, int K, void *C_dev, int c_dtype, long ldc, int accumulate, void *ws_dev,
-                 size_t ws_bytes, void *stream);
+/* C[M][ldc] (+)= A B' of two such matrices [M][K], [N][K] (any of the three block shapes, either format).
+ * C float32: exact products, float32 sums.  C bf16 or f16: the 8-bit matrix instructions, which add 8 products at a time in
+ * 13 bits below the largest of them (1.4e-5 of a result of random operands, under the rounding to C's type).
+ * accumulate adds to what is there, before the rounding to C's type.
+ * a_dtype = -1: A is q, s (lda is not looked at).  a_dtype = SKM_DT_*: A is a float matrix in rows of lda that goes through
+ * 8-bit floats of format fmt_a as skm_fp8_rows makes them (sA is not looked at); it needs the workspace (a_float = 1, 16-byte
+ * aligned).  q 16-byte, s 4-byte aligned. */
+size_t skm_gemm_fp8_workspace_bytes(void *ctx, int M, int N, int K, int a_float);
+int skm_gemm_fp8(void *ctx, const void *A_dev, const void *sA_dev, int fmt_a, int a_dtype, long lda, const void *B_dev,
+                 const void *sB_dev, int fmt_b, int M, int N, int K, void *C_dev, int c_dtype, long ldc, int accumulate,
+                 void *ws_dev, size_t ws_bytes, void *stream);
 
-/* The experts' products: C[row] = W_e A[row of A], W [E][N][K] (tiles), for the rows of a plan of n pairs.  slots = k:
- * the row of A is the pair's token (A is [T][K]); slots = 0: A is in the plan's order already ([n][K]).  Rows of C behind
- * the plan's last are left as they are.
+/* The experts' products: C[row] = W_e A[row of A], W [E][N][K] (tiles), for the rows of a plan of n pairs.  A has `rows`
+ * rows, as for skm_gemm_fp8.  slots = k: the row of A is the pair's token (rows * k = n); slots = 0: A is in the plan's order
+ * already (rows = n).  With small_tiles and small_count (few = 1) the weights are read once per 16 rows of an expert straight
+ * into registers, for up to about 16 rows an expert.  Rows of C behind the plan's last are left as they are.
  * skm_gemm_fp8_experts_wgrad: C[e] (+)= A_e B_e' (float32 [E][M][N]) over the rows of each expert, A [M], B [N] from
  * skm_fp8_columns with the same plan; an expert without rows has zeros. */
-int skm_gemm_fp8_experts(void *ctx, const void *A_dev, const void *sA_dev, int fmt_a, const void *W_dev, const void *sW_dev,
-                         int fmt_w, int E, int N, int K, const int32_t *pair_dev, int slots, long n,
-                         const int32_t *first_dev, const int32_t *tiles_dev, const int32_t *small_tiles_dev,
-                         const int32_t *small_count_dev, void *C_dev, int c_dtype, void *stream);
+size_t skm_gemm_fp8_experts_workspace_bytes(void *ctx, long rows, int K, int a_float, int few);
+int skm_gemm_fp8_experts(void *ctx, const void *A_dev, const void *sA_dev, int fmt_a, int a_dtype, long lda, long rows,
+                         const void *W_dev, const void *sW_dev, int fmt_w, int E, int N, int K, const int32_t *pair_dev,
+                         int slots, long n, const int32_t *first_dev, const int32_t *tiles_dev,
+                         const int32_t *small_tiles_dev, const int32_t *small_count_dev, void *C_dev, int c_dtype,
+                         void *ws_dev, size_t ws_bytes, void *stream);
 int skm_gemm_fp8_experts_wgrad(void *ctx, const void *A_dev, const void *sA_dev, int fmt_a, const void *B_dev,
                                const void *sB_dev, int fmt_b, int E, int M, int N, const int32_t *first_dev, long max_tiles,
                                float *C_dev, int accumulate, void *stream);

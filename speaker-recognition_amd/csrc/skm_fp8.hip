@@ -575,6 +575,214 @@ static void fp8_launch(const Fp8Args &g, int fa, int fb, unsigned gx, unsigned g
     }
 }
 
+// ------------------------------------------------------------------ few rows ------
+// What A may be where it is quantized on the way: a float matrix in rows of ldx.
+struct Fp8Float {
+    const void *x;
+    long ldx;
+    int K;
+    int vec;                // 16-byte loads are allowed
+};
+
+// 16 consecutive numbers of a row; k behind K counts as 0
+template <typename T>
+__device__ __forceinline__ void load16(const T *row, int k, int K, int vec, float *v)
+{
+    float a[8], b[8];
+    load8(row + k, vec, K - k, a);
+    load8(row + k + 8, vec, K - k - 8, b);
+#pragma unroll
+    for (int q = 0; q < 8; ++q) {
+        v[q] = a[q];
+        v[8 + q] = b[q];
+    }
+}
+
+// C = A B' for up to 16 MT rows of A (or tiles of up to 16 rows of an expert): the bytes of B are what counts, each is
+// read once, straight into registers.  A workgroup holds 16 NT columns, its waves share the k blocks in groups of four
+// (one scale dword per row and group) and add their parts through LDS in a fixed order.  v_mfma_scale_f32_16x16x128:
+// B's columns are the rows of the instruction, so a lane ends with 4 consecutive columns of one row of C.
+// A lane (row r of 16, quarter g) holds bytes 16 g .. and 64 + 16 g .. of a block's 128: a load covers 64 consecutive
+// bytes of 16 rows.
+// XT = uint8_t: A is quantized already.  Otherwise a float type: A is quantized in registers, as k_fp8_rows does it --
+// with one row tile the same work in every workgroup costs less than a launch before this one.
+template <int MT, int NT, int FA, int FB, typename TO, typename XT>
+__global__ __launch_bounds__(512, 2) void k_gemm_fp8_rows16(Fp8Args g, Fp8Float fx)
+{
+    __shared__ float part[8][MT * NT * 4][64];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+    const int r = lane & 15, q4 = lane >> 4;
+    int rows = g.M;
+    long row0 = 0;
+    const uint8_t *B = g.B, *sB = g.sB;
+    if (g.tiles) {
+        if ((int)blockIdx.y >= g.tile_count[0]) return;
+        const int32_t *t = g.tiles + (long)blockIdx.y * 4;
+        B += t[0] * g.eB;
+        sB += t[0] * g.esB;
+        row0 = t[1];
+        rows = t[2];
+    }
+    const int col0 = blockIdx.x * 16 * NT;
+    const uint8_t *pb[NT], *qb[NT], *pa[MT], *qa[MT];
+    const XT *px[MT];
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+        const int n = col0 + j * 16 + r < g.N ? col0 + j * 16 + r : g.N - 1;
+        pb[j] = B + n * g.ldb + q4 * 16;
+        qb[j] = sB + (long)n * g.SB;
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const int m = i * 16 + r < rows ? i * 16 + r : rows - 1;
+        long src = row0 + m;
+        if (g.tiles && g.slots) src = g.pair[src] / g.slots;
+        if (sizeof(XT) == 1) {
+            pa[i] = g.A + src * g.lda + q4 * 16;
+            qa[i] = g.sA + src * g.SA;
+        } else {
+            px[i] = static_cast<const XT *>(fx.x) + src * fx.ldx;
+        }
+    }
+    f32x4 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) acc[i][j][q] = 0.f;
+
+    const int groups = (g.kb1 + 3) / 4;
+    for (int gr = wave; gr < groups; gr += waves) {
+        const int nb = g.kb1 - gr * 4 < 4 ? g.kb1 - gr * 4 : 4;
+        i32x8 w[NT][4];
+        int sw[NT];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            sw[j] = *reinterpret_cast<const int *>(qb[j] + gr * 4);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const int kb = gr * 4 + (b < nb ? b : 0);        // a short group repeats its first block, unused
+                const i32x4 lo = *reinterpret_cast<const i32x4 *>(pb[j] + (long)kb * FP8_BLOCK);
+                const i32x4 hi = *reinterpret_cast<const i32x4 *>(pb[j] + (long)kb * FP8_BLOCK + 64);
+                w[j][b] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            int sx = 0;
+            if (sizeof(XT) == 1) sx = *reinterpret_cast<const int *>(qa[i] + gr * 4);
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                if (b >= nb) break;
+                const int kb = gr * 4 + b;
+                i32x8 a;
+                int sa;
+                if (sizeof(XT) == 1) {
+                    const i32x4 lo = *reinterpret_cast<const i32x4 *>(pa[i] + (long)kb * FP8_BLOCK);
+                    const i32x4 hi = *reinterpret_cast<const i32x4 *>(pa[i] + (long)kb * FP8_BLOCK + 64);
+                    a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+                    sa = (sx >> (8 * b)) & 255;
+                } else {
+                    float v[32];
+                    load16(px[i], kb * FP8_BLOCK + q4 * 16, fx.K, fx.vec, v);
+                    load16(px[i], kb * FP8_BLOCK + 64 + q4 * 16, fx.K, fx.vec, v + 16);
+                    float top = 0.f;
+#pragma unroll
+                    for (int q = 0; q < 32; ++q) top = fmaxf(top, fp8_finite_abs(v[q]));
+                    top = fmaxf(top, __shfl_xor(top, 16));
+                    top = fmaxf(top, __shfl_xor(top, 32));
+                    const int e = fp8_exponent(top, FA);
+                    const float f = fp8_pow2(-e);
+                    sa = e + 127;
+#pragma unroll
+                    for (int q = 0; q < 8; ++q)
+                        a[q] = (int)fp8_pack4<FA>(v[4 * q] * f, v[4 * q + 1] * f, v[4 * q + 2] * f, v[4 * q + 3] * f);
+                }
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const int sb = (sw[j] >> (8 * b)) & 255;
+                    if (sizeof(TO) == 4) {
+#pragma unroll
+                        for (int t = 0; t < 4; ++t) {
+                            const bf16x8 xa = fp8_to_bf16<FA>(a[2 * t], a[2 * t + 1], fp8_pow2(sa - 127));
+                            const bf16x8 xb = fp8_to_bf16<FB>(w[j][b][2 * t], w[j][b][2 * t + 1], fp8_pow2(sb - 127));
+                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb, xa, acc[i][j], 0, 0, 0);
+                        }
+                    } else {
+                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[j][b], a, acc[i][j], FB, FA, 0, sb, 0,
+                                                                                     sa);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) part[wave][(i * NT + j) * 4 + q][lane] = acc[i][j][q];
+    __syncthreads();
+    // one wave per 16 x 16 tile of the result, in turn
+    for (int t = wave; t < MT * NT; t += waves) {
+        float v[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[q] = part[0][t * 4 + q][lane];
+        for (int w = 1; w < waves; ++w)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] += part[w][t * 4 + q][lane];
+        const int m = t / NT * 16 + r, n = col0 + t % NT * 16 + 4 * q4;
+        if (m >= rows) continue;
+        TO *c = static_cast<TO *>(g.C) + (row0 + m) * g.ldc + n;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+            if (n + q < g.N) c[q] = (TO)(g.accumulate ? (float)c[q] + v[q] : v[q]);
+    }
+}
+
+template <int MT, int NT, typename TO, typename XT>
+static void rows16_launch(const Fp8Args &g, const Fp8Float &fx, int fa, int fb, unsigned gy, hipStream_t st)
+{
+    const int groups = (g.kb1 + 3) / 4;
+    const dim3 grid((unsigned)((g.N + 16 * NT - 1) / (16 * NT)), gy), block(64u * (groups < 8 ? groups : 8));
+    switch (fa * 2 + fb) {
+    case 0: hipLaunchKernelGGL((k_gemm_fp8_rows16<MT, NT, 0, 0, TO, XT>), grid, block, 0, st, g, fx); break;
+    case 1: hipLaunchKernelGGL((k_gemm_fp8_rows16<MT, NT, 0, 1, TO, XT>), grid, block, 0, st, g, fx); break;
+    case 2: hipLaunchKernelGGL((k_gemm_fp8_rows16<MT, NT, 1, 0, TO, XT>), grid, block, 0, st, g, fx); break;
+    default: hipLaunchKernelGGL((k_gemm_fp8_rows16<MT, NT, 1, 1, TO, XT>), grid, block, 0, st, g, fx); break;
+    }
+}
+
+template <int MT, int NT, typename XT>
+static int rows16_types(const Fp8Args &g, const Fp8Float &fx, int fa, int fb, int dtype, unsigned gy, hipStream_t st)
+{
+    switch (dtype) {
+    case SKM_DT_F32: rows16_launch<MT, NT, float, XT>(g, fx, fa, fb, gy, st); break;
+    case SKM_DT_BF16: rows16_launch<MT, NT, bf16_t, XT>(g, fx, fa, fb, gy, st); break;
+    default: rows16_launch<MT, NT, f16_t, XT>(g, fx, fa, fb, gy, st); break;
+    }
+    SKM_HIP(hipGetLastError());
+    return SKM_OK;
+}
+
+// rows of A: up to 16 (one row tile, quantized on the way if it is a float matrix)
+static int rows16_run(SkmCtx *ctx, const Fp8Args &g, const Fp8Float &fx, int x_dtype, int fa, int fb, int dtype, unsigned gy,
+                      hipStream_t st)
+{
+    SkmProfScope ps(ctx, "k_gemm_fp8_rows16", st);
+    if (g.A) {
+        if (g.M > 32 && !g.tiles) return rows16_types<4, 2, uint8_t>(g, fx, fa, fb, dtype, gy, st);
+        if (g.M > 16 && !g.tiles) return rows16_types<2, 2, uint8_t>(g, fx, fa, fb, dtype, gy, st);
+        return rows16_types<1, 1, uint8_t>(g, fx, fa, fb, dtype, gy, st);
+    }
+    switch (x_dtype) {
+    case SKM_DT_F32: return rows16_types<1, 1, float>(g, fx, fa, fb, dtype, gy, st);
+    case SKM_DT_BF16: return rows16_types<1, 1, bf16_t>(g, fx, fa, fb, dtype, gy, st);
+    default: return rows16_types<1, 1, f16_t>(g, fx, fa, fb, dtype, gy, st);
+    }
+}
+
 static int fp8_run(SkmCtx *ctx, Fp8Args g, int fa, int fb, int dtype, unsigned gy, hipStream_t st, const char *tag)
 {
     g.tiles_n = (g.N + 127) / 128;
@@ -599,26 +807,64 @@ static int fp8_check_product(const char *who, int fa, int fb, int dtype, int M, 
     return SKM_OK;
 }
 
-extern "C" size_t skm_gemm_fp8_workspace_bytes(void *ctx, int M, int N, int K)
+// Up to this many rows the weights are read straight into registers, a workgroup's waves splitting k.
+#define FP8_FEW_ROWS 64
+
+// a float A is quantized on the way (no memory for it) up to one row tile
+static bool fp8_on_the_way(long rows) { return rows <= 16; }
+
+static size_t fp8_operand_bytes(long rows, long K)
 {
-    (void)ctx; (void)M; (void)N; (void)K;
-    return 0;
+    return skm_align_up((size_t)rows * fp8_kpad(K), 256) + skm_align_up((size_t)rows * fp8_sstride(K), 256);
 }
 
-extern "C" int skm_gemm_fp8(void *ctx_, const void *A, const void *sA, int fmt_a, const void *B, const void *sB, int fmt_b,
-                            int M, int N, int K, void *C, int c_dtype, long ldc, int accumulate, void *ws,
-                            size_t ws_bytes, void *stream)
+extern "C" size_t skm_gemm_fp8_workspace_bytes(void *ctx, int M, int N, int K, int a_float)
+{
+    (void)ctx; (void)N;
+    if (M <= 0 || K <= 0) return 0;
+    return a_float && !fp8_on_the_way(M) ? fp8_operand_bytes(M, K) : 0;
+}
+
+// A: q, s in 8-bit floats (a_dtype < 0), or a float matrix in rows of lda that goes through 8-bit floats of format fmt_a;
+// in the second case with more than 16 rows it is quantized into ws, q and s set to that
+static int fp8_take_a(SkmCtx *ctx, const char *who, const void *&q, const void *&s, int a_dtype, long lda, int fmt_a, long rows,
+                      int K, bool on_the_way, void *ws, size_t ws_bytes, Fp8Float *fx, void *stream)
+{
+    if (a_dtype < 0) {
+        SKM_REQUIRE(q && s && ((uintptr_t)q & 15) == 0 && ((uintptr_t)s & 3) == 0, "%s: A is missing or not aligned", who);
+        return SKM_OK;
+    }
+    if (int rc = fp8_check_types(who, a_dtype, fmt_a)) return rc;
+    SKM_REQUIRE(q && lda >= K, "%s: A is missing or its rows overlap", who);
+    if (on_the_way) {
+        *fx = Fp8Float{q, lda, K, aligned16(q, lda * skm_dt_size(a_dtype))};
+        q = s = nullptr;
+        return SKM_OK;
+    }
+    if (!ws || ws_bytes < fp8_operand_bytes(rows, K) || ((uintptr_t)ws & 15)) {
+        skm_set_error("%s: workspace too small or not aligned", who);
+        return SKM_ERR_WORKSPACE;
+    }
+    uint8_t *wq = static_cast<uint8_t *>(ws), *wss = wq + skm_align_up((size_t)rows * fp8_kpad(K), 256);
+    if (int rc = skm_fp8_rows(ctx, q, a_dtype, rows, K, lda, fmt_a, wq, wss, stream)) return rc;
+    q = wq;
+    s = wss;
+    return SKM_OK;
+}
+
+extern "C" int skm_gemm_fp8(void *ctx_, const void *A, const void *sA, int fmt_a, int a_dtype, long lda, const void *B,
+                            const void *sB, int fmt_b, int M, int N, int K, void *C, int c_dtype, long ldc, int accumulate,
+                            void *ws, size_t ws_bytes, void *stream)
 {
     SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
     SKM_REQUIRE(ctx, "skm_gemm_fp8: bad argument");
     if (int rc = fp8_check_product("skm_gemm_fp8", fmt_a, fmt_b, c_dtype, M, N, K)) return rc;
     if (M == 0 || N == 0) return SKM_OK;
-    SKM_REQUIRE(K >= 1 && A && sA && B && sB && C && ldc >= N, "skm_gemm_fp8: bad argument");
-    if (ws_bytes < skm_gemm_fp8_workspace_bytes(ctx, M, N, K)) {
-        skm_set_error("skm_gemm_fp8: workspace too small");
-        return SKM_ERR_WORKSPACE;
-    }
-    (void)ws;
+    SKM_REQUIRE(K >= 1 && B && sB && C && ldc >= N && ((uintptr_t)B & 15) == 0 && ((uintptr_t)sB & 3) == 0,
+                "skm_gemm_fp8: bad argument");
+    Fp8Float fx{};
+    if (int rc = fp8_take_a(ctx, "skm_gemm_fp8", A, sA, a_dtype, lda, fmt_a, M, K, fp8_on_the_way(M), ws, ws_bytes, &fx, stream))
+        return rc;
     SkmDeviceGuard guard(ctx);
     Fp8Args g{};
     g.A = static_cast<const uint8_t *>(A); g.B = static_cast<const uint8_t *>(B);
@@ -627,21 +873,35 @@ extern "C" int skm_gemm_fp8(void *ctx_, const void *A, const void *sA, int fmt_a
     g.SA = g.SB = (int)fp8_sstride(K);
     g.M = M; g.N = N; g.kb1 = (int)(fp8_kpad(K) / FP8_BLOCK);
     g.C = C; g.ldc = ldc; g.accumulate = accumulate != 0; g.slabs = 1;
+    if (M <= FP8_FEW_ROWS) return rows16_run(ctx, g, fx, a_dtype, fmt_a, fmt_b, c_dtype, 1, (hipStream_t)stream);
     g.tiles_m = (M + 127) / 128;
     return fp8_run(ctx, g, fmt_a, fmt_b, c_dtype, 1, (hipStream_t)stream, "k_gemm_fp8");
 }
 
-extern "C" int skm_gemm_fp8_experts(void *ctx_, const void *A, const void *sA, int fmt_a, const void *W, const void *sW,
-                                    int fmt_w, int E, int N, int K, const int32_t *pair, int slots, long n,
-                                    const int32_t *first, const int32_t *tiles, const int32_t *small_tiles,
-                                    const int32_t *small_count, void *C, int c_dtype, void *stream)
+extern "C" size_t skm_gemm_fp8_experts_workspace_bytes(void *ctx, long rows, int K, int a_float, int few)
+{
+    (void)ctx;
+    return a_float && !few && rows > 0 && K > 0 ? fp8_operand_bytes(rows, K) : 0;
+}
+
+extern "C" int skm_gemm_fp8_experts(void *ctx_, const void *A, const void *sA, int fmt_a, int a_dtype, long lda, long rows,
+                                    const void *W, const void *sW, int fmt_w, int E, int N, int K, const int32_t *pair,
+                                    int slots, long n, const int32_t *first, const int32_t *tiles,
+                                    const int32_t *small_tiles, const int32_t *small_count, void *C, int c_dtype, void *ws,
+                                    size_t ws_bytes, void *stream)
 {
     SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
-    SKM_REQUIRE(ctx && E >= 1 && n >= 0 && n <= 0x3FFFFFFF && slots >= 0, "skm_gemm_fp8_experts: bad argument");
+    SKM_REQUIRE(ctx && E >= 1 && n >= 0 && n <= 0x3FFFFFFF && slots >= 0 && !small_tiles == !small_count,
+                "skm_gemm_fp8_experts: bad argument");
     if (int rc = fp8_check_product("skm_gemm_fp8_experts", fmt_a, fmt_w, c_dtype, (int)n, N, K)) return rc;
     if (n == 0 || N == 0) return SKM_OK;
-    SKM_REQUIRE(K >= 1 && A && sA && W && sW && C && pair && first && tiles, "skm_gemm_fp8_experts: bad argument");
-    (void)small_tiles; (void)small_count;
+    SKM_REQUIRE(K >= 1 && W && sW && C && pair && first && tiles && ((uintptr_t)W & 15) == 0 && ((uintptr_t)sW & 3) == 0,
+                "skm_gemm_fp8_experts: bad argument");
+    SKM_REQUIRE(slots ? rows * slots == n : rows == n, "skm_gemm_fp8_experts: %ld rows of A for %ld pairs", rows, n);
+    Fp8Float fx{};
+    if (int rc = fp8_take_a(ctx, "skm_gemm_fp8_experts", A, sA, a_dtype, lda, fmt_a, rows, K, small_tiles != nullptr, ws,
+                            ws_bytes, &fx, stream))
+        return rc;
     SkmDeviceGuard guard(ctx);
     Fp8Args g{};
     g.A = static_cast<const uint8_t *>(A); g.B = static_cast<const uint8_t *>(W);
@@ -652,6 +912,13 @@ extern "C" int skm_gemm_fp8_experts(void *ctx_, const void *A, const void *sA, i
     g.C = C; g.ldc = N; g.slabs = 1;
     g.tiles = tiles; g.tile_count = first + E; g.pair = pair; g.slots = slots;
     g.eB = (long)N * g.ldb; g.esB = (long)N * g.SB;
+    if (small_tiles) {
+        g.tiles = small_tiles;
+        g.tile_count = small_count;
+        const long t = skm_route_plan_tiles(n, E, 16);
+        SKM_REQUIRE(t <= 65535, "skm_gemm_fp8_experts: more than 65535 tiles of 16 rows");
+        return rows16_run(ctx, g, fx, a_dtype, fmt_a, fmt_w, c_dtype, (unsigned)t, (hipStream_t)stream);
+    }
     g.tiles_m = (int)skm_route_plan_tiles(n, E, 128);
     return fp8_run(ctx, g, fmt_a, fmt_w, c_dtype, 1, (hipStream_t)stream, "k_gemm_fp8_experts");
 }
@@ -665,7 +932,9 @@ extern "C" int skm_gemm_fp8_experts_wgrad(void *ctx_, const void *A, const void 
                 "skm_gemm_fp8_experts_wgrad: bad argument");
     if (int rc = fp8_check_product("skm_gemm_fp8_experts_wgrad", fmt_a, fmt_b, SKM_DT_F32, M, N, 1)) return rc;
     if (M == 0 || N == 0) return SKM_OK;
-    SKM_REQUIRE(C && first && (max_tiles == 0 || (A && sA && B && sB)), "skm_gemm_fp8_experts_wgrad: bad argument");
+    SKM_REQUIRE(C && first && (max_tiles == 0 || (A && sA && B && sB)) &&
+                    (((uintptr_t)A | (uintptr_t)B) & 15) == 0 && (((uintptr_t)sA | (uintptr_t)sB) & 3) == 0,
+                "skm_gemm_fp8_experts_wgrad: bad argument");
     SkmDeviceGuard guard(ctx);
     Fp8Args g{};
     g.A = static_cast<const uint8_t *>(A); g.B = static_cast<const uint8_t *>(B);

@@ -120,12 +120,15 @@ SIGNATURES = {
                                _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
     "skm_fp8_columns": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_long, _c_int, _c_long, _c_int, _c_void_p, _c_void_p,
                                  _c_long, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
-    "skm_gemm_fp8_workspace_bytes": (_c_size_t, [_c_void_p, _c_int, _c_int, _c_int]),
-    "skm_gemm_fp8": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_int, _c_int,
-                              _c_int, _c_void_p, _c_int, _c_long, _c_int, _c_void_p, _c_size_t, _c_void_p]),
-    "skm_gemm_fp8_experts": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_int,
-                                      _c_int, _c_int, _c_void_p, _c_int, _c_long, _c_void_p, _c_void_p, _c_void_p,
-                                      _c_void_p, _c_void_p, _c_int, _c_void_p]),
+    "skm_gemm_fp8_workspace_bytes": (_c_size_t, [_c_void_p, _c_int, _c_int, _c_int, _c_int]),
+    "skm_gemm_fp8": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_long, _c_void_p, _c_void_p, _c_int,
+                              _c_int, _c_int, _c_int, _c_void_p, _c_int, _c_long, _c_int, _c_void_p, _c_size_t,
+                              _c_void_p]),
+    "skm_gemm_fp8_experts_workspace_bytes": (_c_size_t, [_c_void_p, _c_long, _c_int, _c_int, _c_int]),
+    "skm_gemm_fp8_experts": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_long, _c_long, _c_void_p,
+                                      _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_int, _c_long, _c_void_p,
+                                      _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_size_t,
+                                      _c_void_p]),
     "skm_gemm_fp8_experts_wgrad": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int,
                                             _c_int, _c_int, _c_int, _c_void_p, _c_long, _c_void_p, _c_int, _c_void_p]),
     # one process, several GPUs (team.py)
@@ -1023,7 +1026,7 @@ class HipEngine(object):
             raise SkmError("route_plan: %d experts, %d places" % (E, k))
         plan = RoutePlan(self, T, k, E)
         need = self.lib.skm_route_plan_workspace_bytes(plan.n, E)
-        ws = torch.empty(int(need), dtype=torch.uint8, device=self.device) if need else None
+        ws = self._scratch(need)
         p = plan._ptr
         self._check(self.lib.skm_route_plan(
             self.ctx, ids.data_ptr(), plan.n, E, p("offsets"), p("pair"), p("pos"), p("first"), p("tiles"),
@@ -1121,56 +1124,65 @@ class HipEngine(object):
             raise SkmError("%s: an Fp8Matrix of %d dimensions on %s is wanted" % (what, dims + 1, self.device))
         return m
 
+    def _operand(self, A, what):
+        """(q or the matrix, s, format, type or -1, distance of rows, shape) of a product's first operand"""
+        if isinstance(A, self.torch.Tensor):
+            lda = self._matrix(A, what)
+            return A.data_ptr(), None, 0, self._dt(A.dtype, (0, 1, 2), what), lda, A.shape
+        self._fp8(A, what)
+        if A.plan is not None:
+            raise SkmError("%s: columns in a plan's order go to gemm_fp8_experts_wgrad" % what)
+        return A.q.data_ptr(), A.s.data_ptr(), A.code, -1, 0, A.shape
+
+    def _scratch(self, need):
+        """memory of one call's own (the allocator keeps it in the order of the stream and apart from other graphs)"""
+        return self.torch.empty(int(need), dtype=self.torch.uint8, device=self.device) if need else None
+
     def gemm_fp8(self, A, B, dtype=None, out=None, accumulate=False):
-        """A B' of two Fp8Matrix [M x K], [N x K] (skm_gemm_fp8); a float matrix A is taken through fp8_rows.  The result
-        (M x N) is of type `dtype` (default bfloat16), or goes to `out` (rows may be apart), added to it with
-        `accumulate`."""
-        torch = self.torch
-        if isinstance(A, torch.Tensor):
-            A = self.fp8_rows(A)
-        self._fp8(A, "gemm_fp8: A")
+        """A B' of two Fp8Matrix [M x K], [N x K] (skm_gemm_fp8); a float matrix A goes through 8-bit floats as fp8_rows
+        makes them.  The result (M x N) is of type `dtype` (default bfloat16; float32 has exact products and float32
+        sums), or goes to `out` (rows may be apart), added to it with `accumulate`."""
+        a, sa, fa, a_dtype, lda, (M, K) = self._operand(A, "gemm_fp8: A")
         self._fp8(B, "gemm_fp8: B")
-        if A.plan is not None or B.plan is not None:
-            raise SkmError("gemm_fp8: columns in a plan's order go to gemm_fp8_experts_wgrad")
-        M, K = A.shape
         N = B.shape[0]
-        if B.shape[1] != K:
-            raise SkmError("gemm_fp8: K = %d and %d" % (K, B.shape[1]))
+        if B.shape[1] != K or B.plan is not None:
+            raise SkmError("gemm_fp8: A %s and B %s do not go together" % ((M, K), B.shape))
         if out is None:
             if accumulate:
                 raise SkmError("gemm_fp8: accumulate without out")
-            out = torch.empty((M, N), dtype=dtype or torch.bfloat16, device=self.device)
+            out = self.torch.empty((M, N), dtype=dtype or self.torch.bfloat16, device=self.device)
             ldc = N
         else:
             ldc = self._matrix(out, "gemm_fp8: out", M, N, (dtype,) if dtype is not None else None)
-        need = self.lib.skm_gemm_fp8_workspace_bytes(self.ctx, M, N, K)
-        ws = torch.empty(int(need), dtype=torch.uint8, device=self.device) if need else None
+        need = self.lib.skm_gemm_fp8_workspace_bytes(self.ctx, M, N, K, 1) if a_dtype >= 0 else 0
+        ws = self._scratch(need)
         self._check(self.lib.skm_gemm_fp8(
-            self.ctx, A.q.data_ptr(), A.s.data_ptr(), A.code, B.q.data_ptr(), B.s.data_ptr(), B.code, M, N, K,
-            out.data_ptr(), self._dt(out.dtype, (0, 1, 2), "gemm_fp8"), ldc, 1 if accumulate else 0,
-            ws.data_ptr() if need else None, need, self._stream()))
+            self.ctx, a, sa, fa, a_dtype, lda, B.q.data_ptr(), B.s.data_ptr(), B.code, M, N, K, out.data_ptr(),
+            self._dt(out.dtype, (0, 1, 2), "gemm_fp8"), ldc, 1 if accumulate else 0, ws.data_ptr() if need else None, need,
+            self._stream()))
         return out
 
     def gemm_fp8_experts(self, A, W, plan, dtype=None):
         """The experts' products in the plan's order: row r of the result (plan.n x N, rows behind the plan's last are
-        not written) is W[expert of r] times the row of A: of the pair's token where A has plan.T rows (a float matrix is
-        taken through fp8_rows), of r itself where it has plan.n and the plan more than one place.  W: Fp8Matrix E x N x K."""
-        torch = self.torch
-        if isinstance(A, torch.Tensor):
-            A = self.fp8_rows(A)
-        self._fp8(A, "gemm_fp8_experts: A")
+        not written) is W[expert of r] times the row of A: of the pair's token where A has plan.T rows, of r itself
+        where it has plan.n and the plan more than one place.  A: Fp8Matrix, or a float matrix that goes through 8-bit
+        floats as fp8_rows makes them; W: Fp8Matrix E x N x K."""
+        a, sa, fa, a_dtype, lda, (M, K) = self._operand(A, "gemm_fp8_experts: A")
         self._fp8(W, "gemm_fp8_experts: W", 2)
-        E, N, K = W.shape
-        if E != plan.E or A.shape[1] != K or A.plan is not None or A.shape[0] not in (plan.T, plan.n):
+        E, N, Kw = W.shape
+        if E != plan.E or K != Kw or M not in (plan.T, plan.n):
             raise SkmError("gemm_fp8_experts: A %s, W %s, a plan of %d x %d pairs over %d experts"
-                           % (A.shape, W.shape, plan.T, plan.k, plan.E))
-        dtype = dtype or torch.bfloat16
-        out = torch.empty((plan.n, N), dtype=dtype, device=self.device)
+                           % ((M, K), W.shape, plan.T, plan.k, plan.E))
+        dtype = dtype or self.torch.bfloat16
+        out = self.torch.empty((plan.n, N), dtype=dtype, device=self.device)
+        need = self.lib.skm_gemm_fp8_experts_workspace_bytes(self.ctx, M, K, 1, plan.few) if a_dtype >= 0 else 0
+        ws = self._scratch(need)
         self._check(self.lib.skm_gemm_fp8_experts(
-            self.ctx, A.q.data_ptr(), A.s.data_ptr(), A.code, W.q.data_ptr(), W.s.data_ptr(), W.code, E, N, K,
-            plan._ptr("pair"), plan.k if A.shape[0] == plan.T else 0, plan.n, plan._ptr("first"), plan._ptr("tiles"),
+            self.ctx, a, sa, fa, a_dtype, lda, M, W.q.data_ptr(), W.s.data_ptr(), W.code, E, N, K,
+            plan._ptr("pair"), plan.k if M == plan.T else 0, plan.n, plan._ptr("first"), plan._ptr("tiles"),
             plan._ptr("small_tiles") if plan.few else None, plan._ptr("small_count") if plan.few else None,
-            out.data_ptr(), self._dt(dtype, (0, 1, 2), "gemm_fp8_experts"), self._stream()))
+            out.data_ptr(), self._dt(dtype, (0, 1, 2), "gemm_fp8_experts"), ws.data_ptr() if need else None, need,
+            self._stream()))
         return out
 
     def gemm_fp8_experts_wgrad(self, A, B, plan, out=None, accumulate=False):

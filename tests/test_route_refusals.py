@@ -128,14 +128,28 @@ def test_fp8_refusals(lib, ctx):
     assert lib.skm_fp8_tiles(ctx, P, 0, 1, 0, 8, 8, 64, 0, P, P, None, None, None) == ARG
     assert lib.skm_fp8_columns(ctx, P, 0, 8, 8, 8, 0, P, None, 4, P, 2, None, P, P, None) == ARG
     assert lib.skm_fp8_columns(ctx, P, 0, 8, 8, 8, 0, None, None, 0, None, 0, P, P, P, None) == ARG
-    assert lib.skm_gemm_fp8(ctx, P, P, 0, P, P, 0, 8, 8, 0, P, 0, 8, 0, None, 0, None) == ARG
-    assert lib.skm_gemm_fp8(ctx, P, P, 0, P, P, 0, 8, 8, 8, P, 3, 8, 0, None, 0, None) == ARG
-    assert lib.skm_gemm_fp8(ctx, P, P, 2, P, P, 0, 8, 8, 8, P, 0, 8, 0, None, 0, None) == ARG
-    assert lib.skm_gemm_fp8(ctx, P, P, 0, P, P, 0, 8, 8, 8, P, 0, 7, 0, None, 0, None) == ARG
-    assert lib.skm_gemm_fp8(ctx, P, None, 0, P, P, 0, 8, 8, 8, P, 0, 8, 0, None, 0, None) == ARG
-    assert lib.skm_gemm_fp8(ctx, P, P, 0, P, P, 0, 0, 8, 8, P, 0, 8, 0, None, 0, None) == 0
-    assert lib.skm_gemm_fp8_experts(ctx, P, P, 0, P, P, 0, 0, 8, 8, P, 2, 8, P, P, None, None, P, 0, None) == ARG
-    assert lib.skm_gemm_fp8_experts(ctx, P, P, 0, P, P, 0, 4, 8, 8, P, 2, 8, None, P, None, None, P, 0, None) == ARG
+    gemm = lib.skm_gemm_fp8
+    assert gemm(ctx, P, P, 0, -1, 0, P, P, 0, 8, 8, 0, P, 0, 8, 0, None, 0, None) == ARG          # no K
+    assert gemm(ctx, P, P, 0, -1, 0, P, P, 0, 8, 8, 8, P, 3, 8, 0, None, 0, None) == ARG          # float64 result
+    assert gemm(ctx, P, P, 2, -1, 0, P, P, 0, 8, 8, 8, P, 0, 8, 0, None, 0, None) == ARG          # format
+    assert gemm(ctx, P, P, 0, -1, 0, P, P, 0, 8, 8, 8, P, 0, 7, 0, None, 0, None) == ARG          # ldc < N
+    assert gemm(ctx, P, None, 0, -1, 0, P, P, 0, 8, 8, 8, P, 0, 8, 0, None, 0, None) == ARG       # no scales
+    assert gemm(ctx, P, P, 0, 3, 8, P, P, 0, 8, 8, 8, P, 0, 8, 0, None, 0, None) == ARG           # float64 A
+    assert gemm(ctx, P, P, 0, 0, 7, P, P, 0, 8, 8, 8, P, 0, 8, 0, None, 0, None) == ARG           # rows overlap
+    assert gemm(ctx, P, P, 0, 0, 8, P, P, 0, 99, 8, 8, P, 0, 8, 0, None, 0, None) == WORKSPACE
+    odd = ctypes.c_void_p(0x1004)
+    assert gemm(ctx, odd, P, 0, -1, 0, P, P, 0, 8, 8, 8, P, 0, 8, 0, None, 0, None) == ARG        # alignment
+    assert gemm(ctx, P, P, 0, -1, 0, odd, P, 0, 8, 8, 8, P, 0, 8, 0, None, 0, None) == ARG
+    assert gemm(ctx, P, P, 0, -1, 0, P, P, 0, 0, 8, 8, P, 0, 8, 0, None, 0, None) == 0
+    assert lib.skm_gemm_fp8_workspace_bytes(ctx, 99, 8, 8, 0) == 0
+    assert lib.skm_gemm_fp8_workspace_bytes(ctx, 99, 8, 8, 1) >= 99 * (128 + 4)
+    ex = lib.skm_gemm_fp8_experts
+    assert ex(ctx, P, P, 0, -1, 0, 4, P, P, 0, 0, 8, 8, P, 2, 8, P, P, None, None, P, 0, None, 0, None) == ARG     # E
+    assert ex(ctx, P, P, 0, -1, 0, 4, P, P, 0, 4, 8, 8, None, 2, 8, P, P, None, None, P, 0, None, 0, None) == ARG  # no pairs
+    assert ex(ctx, P, P, 0, -1, 0, 5, P, P, 0, 4, 8, 8, P, 2, 8, P, P, None, None, P, 0, None, 0, None) == ARG     # 5 x 2 != 8
+    assert ex(ctx, P, P, 0, -1, 0, 4, P, P, 0, 4, 8, 8, P, 0, 8, P, P, None, None, P, 0, None, 0, None) == ARG
+    assert ex(ctx, P, P, 0, -1, 0, 4, P, P, 0, 4, 8, 8, P, 2, 8, P, P, P, None, P, 0, None, 0, None) == ARG        # no count
+    assert ex(ctx, P, None, 0, 0, 8, 4, P, P, 0, 4, 8, 8, P, 2, 8, P, P, None, None, P, 0, None, 0, None) == WORKSPACE
     assert lib.skm_gemm_fp8_experts_wgrad(ctx, P, P, 0, P, P, 0, 4, 8, 8, P, 2, None, 0, None) == ARG
     assert lib.skm_gemm_fp8_experts_wgrad(ctx, P, P, 0, P, P, 0, 70000, 8, 8, P, 2, P, 0, None) == ARG
 
