@@ -337,10 +337,12 @@ struct Fp8Args {
     long lda, ldb;
     int SA, SB;
     int M, N;
+    long rowsA;             // rows that A has (by plan: tokens or pairs)
     int kb0, kb1;           // blocks of 128 k
     void *C;
     long ldc;
     int accumulate;
+    int c_vec;              // C takes 16-byte stores
     int tiles_m, tiles_n;
     long zC;                // split over k: slab z holds the partial sums of its blocks, zC elements apart
     int slabs;
@@ -386,6 +388,7 @@ typedef __attribute__((address_space(1))) const void *glb_ptr;
 //   LDS: a row's 128 bytes of a stage are one line; its 16-byte pieces are stored at piece ^ (row & 7), so that the 8
 //   lanes of a read phase (8 rows, the same piece) meet 8 different bank groups.  The loads put consecutive lanes'
 //   pieces at consecutive addresses, so the exchange is made on the global side, within the line.
+//   The scales come the same way, a dword (four blocks) of every row in every fourth stage.
 //   The 8-bit matrix instructions add 8 products at a time in a window of 13 bits below the largest of the 8 (a product
 //   2^-14 of it is lost, measured): 1.4e-5 of a result of random operands.  Under a result that is rounded to bf16 or f16
 //   (2^-9, 2^-12) that is nothing; a float32 result is wanted as such (weight gradients that are added up, rows that a
@@ -393,11 +396,22 @@ typedef __attribute__((address_space(1))) const void *glb_ptr;
 //   and the sums float32, at half the rate.
 //   Which of the 64 k of a product lies where in the operand registers does not matter as long as A and B agree and a
 //   scale covers all of them: a lane's 32 bytes are 32 consecutive k of its row here.
+// A stage is two halves of 64 k in two sets of fragments: while one set is multiplied, the other is read.  Stage s:
+//   read half 1 of s; multiply half 0 (all but the last row of tiles)
+//   wait for the own reads and for the own loads of stage s + 1; barrier: nobody reads buffer s & 1 any more, stage s + 1 is
+//   complete
+//   issue the loads of stage s + 2 into buffer s & 1; multiply the rest of half 0
+//   read half 0 of s + 1; multiply half 1
+// so a load has one and a half stages to arrive, an LDS read half a stage, and the barrier stands among multiplications
+// that are under way already.
 template <int MT, int NT, int FA, int FB, typename TO>
-__global__ __launch_bounds__(256, (MT * NT > 8) ? 1 : 2) void k_gemm_fp8(Fp8Args g)
+__global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args g)
 {
-    constexpr int BM = MT * 64, BN = NT * 64;
-    __shared__ __align__(16) uint8_t sh[2][(BM + BN) * FP8_BLOCK];
+    constexpr int BM = MT * 64, BN = NT * 64, LOADS = (MT + NT) * 2;
+    // One array: with two of them hipcc waits for the loads in flight in front of every read of LDS.
+    // [two stages of (BM + BN) rows of 128 bytes][two groups of four blocks of (BM + BN) scale dwords]
+    constexpr int STAGE = (BM + BN) * FP8_BLOCK, GROUP = (BM + BN) * 4;
+    __shared__ __align__(16) uint8_t sh[2 * STAGE + 2 * GROUP];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 1, wn = wave & 1, r = lane & 31, h = lane >> 5;
 
@@ -437,38 +451,60 @@ __global__ __launch_bounds__(256, (MT * NT > 8) ? 1 : 2) void k_gemm_fp8(Fp8Args
     }
     const int col0 = tn * BN, cols = g.N - col0;
 
-    // one row of A (B) per lane and load: rows behind the last repeat it
+    // From this tile's first row (A by plan: from A's first), so that a lane's offset is 32 bits wide.
+    const bool by_pair = g.tiles && g.slots;
+    const long a0 = by_pair ? 0 : row0;
+    const uint8_t *ba = g.A + a0 * g.lda + (long)kb0 * FP8_BLOCK, *bb = B + col0 * g.ldb + (long)kb0 * FP8_BLOCK;
+    const uint8_t *bsa = g.sA + a0 * g.SA, *bsb = sB + (long)col0 * g.SB;
+    // one row of A (B) per 8 lanes and load: rows behind the last repeat it
     const int lr = lane >> 3, lp = ((lane & 7) ^ lr) * 16;
-    const uint8_t *pa[MT * 2], *pb[NT * 2];
+    unsigned oa[MT * 2], ob[NT * 2];
 #pragma unroll
     for (int i = 0; i < MT * 2; ++i) {
         int rr = (wave * MT * 2 + i) * 8 + lr;
         rr = rr < rows ? rr : rows - 1;
-        long src = row0 + rr;
-        if (g.tiles && g.slots) src = g.pair[src] / g.slots;
-        pa[i] = g.A + src * g.lda + (long)kb0 * FP8_BLOCK + lp;
+        if (by_pair) rr = g.pair[row0 + rr] / g.slots;
+        oa[i] = (unsigned)rr * (unsigned)g.lda + lp;
     }
 #pragma unroll
     for (int i = 0; i < NT * 2; ++i) {
         int cc = (wave * NT * 2 + i) * 8 + lr;
         cc = cc < cols ? cc : cols - 1;
-        pb[i] = B + (col0 + cc) * g.ldb + (long)kb0 * FP8_BLOCK + lp;
+        ob[i] = (unsigned)cc * (unsigned)g.ldb + lp;
     }
-    const uint8_t *qa[MT], *qb[NT];         // scales of the rows (columns) of this lane
+    // scales: 64 rows a load, the rows of A, then the columns of B; waves take turns
+    constexpr int CHUNKS = (BM + BN) / 64, MINE = (CHUNKS + 3) / 4;
+    unsigned os[MINE];
 #pragma unroll
-    for (int i = 0; i < MT; ++i) {
-        int rr = wm * MT * 32 + i * 32 + r;
-        rr = rr < rows ? rr : rows - 1;
-        long src = row0 + rr;
-        if (g.tiles && g.slots) src = g.pair[src] / g.slots;
-        qa[i] = g.sA + src * g.SA;
+    for (int i = 0; i < MINE; ++i) {
+        int rr = (wave + 4 * i) * 64 + lane;
+        if (rr < BM) {
+            rr = rr < rows ? rr : rows - 1;
+            if (by_pair) rr = g.pair[row0 + rr] / g.slots;
+            os[i] = (unsigned)rr * (unsigned)g.SA;
+        } else {
+            rr = rr - BM < cols ? rr - BM : cols - 1;
+            os[i] = (unsigned)rr * (unsigned)g.SB;
+        }
     }
-#pragma unroll
-    for (int i = 0; i < NT; ++i) {
-        int cc = wn * NT * 32 + i * 32 + r;
-        cc = cc < cols ? cc : cols - 1;
-        qb[i] = sB + (long)(col0 + cc) * g.SB;
+
+    // loads of the stage S (blocks from kb0) into buffer ST; scales of the blocks 4 G .. 4 G + 3
+#define FP8_ISSUE(S, ST)                                                                                               \
+    {                                                                                                                  \
+        const uint8_t *la = ba + (long)(S) * FP8_BLOCK, *lb = bb + (long)(S) * FP8_BLOCK;                              \
+        _Pragma("unroll") for (int i = 0; i < MT * 2; ++i) __builtin_amdgcn_global_load_lds(                           \
+            (glb_ptr)(la + oa[i]), (lds_ptr)&sh[(ST) * STAGE + (wave * MT * 2 + i) * 8 * FP8_BLOCK], 16, 0, 0);        \
+        _Pragma("unroll") for (int i = 0; i < NT * 2; ++i) __builtin_amdgcn_global_load_lds(                           \
+            (glb_ptr)(lb + ob[i]), (lds_ptr)&sh[(ST) * STAGE + (BM + (wave * NT * 2 + i) * 8) * FP8_BLOCK], 16, 0, 0); \
     }
+#define FP8_SCALES(G)                                                                                                  \
+    _Pragma("unroll") for (int i = 0; i < MINE; ++i) {                                                                 \
+        const int c = wave + 4 * i;                                                                                    \
+        const uint8_t *l = (c * 64 < BM ? bsa : bsb) + (long)(G) * 4;                                                  \
+        if (CHUNKS % 4 == 0 || c < CHUNKS)                                                                             \
+            __builtin_amdgcn_global_load_lds((glb_ptr)(l + os[i]), (lds_ptr)&sh[2 * STAGE + ((G) & 1) * GROUP + c * 256], 4, 0, 0); \
+    }
+
     f32x16 acc[MT][NT];
 #pragma unroll
     for (int i = 0; i < MT; ++i)
@@ -477,90 +513,163 @@ __global__ __launch_bounds__(256, (MT * NT > 8) ? 1 : 2) void k_gemm_fp8(Fp8Args
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
 
-#define FP8_ISSUE(ST)                                                                                                  \
-    _Pragma("unroll") for (int i = 0; i < MT * 2; ++i) {                                                               \
-        __builtin_amdgcn_global_load_lds((glb_ptr)pa[i], (lds_ptr)&sh[ST][(wave * MT * 2 + i) * 8 * FP8_BLOCK], 16, 0, 0); \
-        pa[i] += FP8_BLOCK;                                                                                            \
-    }                                                                                                                  \
-    _Pragma("unroll") for (int i = 0; i < NT * 2; ++i) {                                                               \
-        __builtin_amdgcn_global_load_lds((glb_ptr)pb[i],                                                               \
-                                         (lds_ptr)&sh[ST][(BM + (wave * NT * 2 + i) * 8) * FP8_BLOCK], 16, 0, 0);      \
-        pb[i] += FP8_BLOCK;                                                                                            \
-    }
-
-    const int n = kb1 - kb0;
-    if (n > 0) { FP8_ISSUE(0) }
-    // bytes of this lane's pieces: half H of the block, pieces 4 H + 2 h and the next, exchanged by row & 7 = r & 7
+    // this lane's pieces of a half H: 4 H + 2 h and the next, exchanged by row & 7 = r & 7
     const int x7 = r & 7;
-    for (int s = 0; s < n; ++s) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();                    // stage s is there, and everybody has left the other buffer
-        if (s + 1 < n) { FP8_ISSUE((s + 1) & 1) }
-        const int kb = kb0 + s;
-        int sa[MT], sb[NT];
+    int at[2][2];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) sa[i] = qa[i][kb];
+    for (int H = 0; H < 2; ++H)
 #pragma unroll
-        for (int i = 0; i < NT; ++i) sb[i] = qb[i][kb];
-        const uint8_t *base = sh[s & 1];
-#pragma unroll
-        for (int H = 0; H < 2; ++H) {
-            i32x8 fa[MT], fb[NT];
-            const int p0 = ((H * 4 + h * 2) ^ x7) * 16, p1 = ((H * 4 + h * 2 + 1) ^ x7) * 16;
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const uint8_t *l = base + (wm * MT * 32 + i * 32 + r) * FP8_BLOCK;
-                const i32x4 lo = *reinterpret_cast<const i32x4 *>(l + p0), hi = *reinterpret_cast<const i32x4 *>(l + p1);
-                fa[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            }
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const uint8_t *l = base + (BM + wn * NT * 32 + i * 32 + r) * FP8_BLOCK;
-                const i32x4 lo = *reinterpret_cast<const i32x4 *>(l + p0), hi = *reinterpret_cast<const i32x4 *>(l + p1);
-                fb[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            }
-            if (sizeof(TO) == 4) {
-                bf16x8 xb[NT][4];
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int t = 0; t < 4; ++t)
-                        xb[j][t] = fp8_to_bf16<FB>(fb[j][2 * t], fb[j][2 * t + 1], fp8_pow2(sb[j] - 127));
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int t = 0; t < 4; ++t) {
-                        const bf16x8 xa = fp8_to_bf16<FA>(fa[i][2 * t], fa[i][2 * t + 1], fp8_pow2(sa[i] - 127));
-#pragma unroll
-                        for (int j = 0; j < NT; ++j)
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xa, xb[j][t], acc[i][j], 0, 0, 0);
-                    }
-            } else {
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fa[i], fb[j], acc[i][j], FA, FB, 0,
-                                                                                    sa[i], 0, sb[j]);
-            }
-        }
+        for (int u = 0; u < 2; ++u) at[H][u] = r * FP8_BLOCK + ((H * 4 + h * 2 + u) ^ x7) * 16;
+    i32x8 fa[2][MT], fb[2][NT];
+    int sa[MT], sb[NT], na[MT], nb[NT];
+#define FP8_READ(H, ST)                                                                                                \
+    _Pragma("unroll") for (int i = 0; i < MT; ++i) {                                                                   \
+        const uint8_t *l = &sh[(ST) * STAGE + (wm * MT + i) * 32 * FP8_BLOCK];                                         \
+        const i32x4 lo = *reinterpret_cast<const i32x4 *>(l + at[H][0]), hi = *reinterpret_cast<const i32x4 *>(l + at[H][1]); \
+        fa[H][i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);                                            \
+    }                                                                                                                  \
+    _Pragma("unroll") for (int j = 0; j < NT; ++j) {                                                                   \
+        const uint8_t *l = &sh[(ST) * STAGE + (BM + (wn * NT + j) * 32) * FP8_BLOCK];                                  \
+        const i32x4 lo = *reinterpret_cast<const i32x4 *>(l + at[H][0]), hi = *reinterpret_cast<const i32x4 *>(l + at[H][1]); \
+        fb[H][j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);                                            \
     }
+#define FP8_READ_SCALES(KB)                                                                                            \
+    {                                                                                                                  \
+        const uint8_t *l = &sh[2 * STAGE + (((KB) >> 2) & 1) * GROUP + r * 4 + ((KB) & 3)];                            \
+        _Pragma("unroll") for (int i = 0; i < MT; ++i) na[i] = l[(wm * MT + i) * 128];                                 \
+        _Pragma("unroll") for (int j = 0; j < NT; ++j) nb[j] = l[(BM + (wn * NT + j) * 32) * 4];                       \
+    }
+    // rows I0 .. I1 - 1 of the wave's tiles times half H
+    bf16x8 xb[NT][4];
+#define FP8_CONVERT_B(H)                                                                                               \
+    if (sizeof(TO) == 4) {                                                                                             \
+        _Pragma("unroll") for (int j = 0; j < NT; ++j) _Pragma("unroll") for (int t = 0; t < 4; ++t)                   \
+            xb[j][t] = fp8_to_bf16<FB>(fb[H][j][2 * t], fb[H][j][2 * t + 1], fp8_pow2(sb[j] - 127));                   \
+    }
+#define FP8_MULTIPLY(H, I0, I1)                                                                                        \
+    _Pragma("unroll") for (int i = I0; i < I1; ++i) {                                                                  \
+        if (sizeof(TO) == 4) {                                                                                         \
+            _Pragma("unroll") for (int t = 0; t < 4; ++t) {                                                            \
+                const bf16x8 xa = fp8_to_bf16<FA>(fa[H][i][2 * t], fa[H][i][2 * t + 1], fp8_pow2(sa[i] - 127));        \
+                _Pragma("unroll") for (int j = 0; j < NT; ++j)                                                         \
+                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xb[j][t], xa, acc[i][j], 0, 0, 0);             \
+            }                                                                                                          \
+        } else {                                                                                                       \
+            _Pragma("unroll") for (int j = 0; j < NT; ++j)                                                             \
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[H][j], fa[H][i], acc[i][j], FB, FA, 0,  \
+                                                                            sb[j], 0, sa[i]);                          \
+        }                                                                                                              \
+    }
+    const int n = kb1 - kb0;
+    if (n > 0) {
+        FP8_SCALES(kb0 >> 2)
+        if (n > 1 && ((kb0 + 1) >> 2) != (kb0 >> 2)) { FP8_SCALES((kb0 + 1) >> 2) }
+        FP8_ISSUE(0, 0)
+        if (n > 1) {
+            FP8_ISSUE(1, 1)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
+        } else {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        }
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        FP8_READ(0, 0)
+        FP8_READ_SCALES(kb0)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) sa[i] = na[i];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) sb[j] = nb[j];
+    }
+    // One straight block per stage, without a branch: behind the last stage the last one is loaded again into the free
+    // buffer, and what is read of it is not used; a group's scales are loaded again with each of its stages.
+    for (int s = 0; s < n; ++s) {
+        const int st = s & 1, kb = kb0 + s;
+        const int s2 = s + 2 < n ? s + 2 : n - 1;
+        FP8_READ(1, st)
+        FP8_CONVERT_B(0)
+        FP8_MULTIPLY(0, 0, MT - 1)
+        // the multiplications stand in front of the barrier (an empty statement that takes their results; it reads nothing)
+#pragma unroll
+        for (int i = 0; i < MT - 1; ++i)
+#pragma unroll
+            for (int j = 0; j < NT; ++j) asm volatile("" : "+a"(acc[i][j]));
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        FP8_SCALES((kb0 + s2) >> 2)
+        FP8_ISSUE(s2, st)
+        FP8_MULTIPLY(0, MT - 1, MT)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) asm volatile("" : "+a"(acc[MT - 1][j]));
+        __builtin_amdgcn_sched_barrier(0);
+        FP8_READ(0, st ^ 1)
+        FP8_READ_SCALES(kb + 1)
+        FP8_CONVERT_B(1)
+        FP8_MULTIPLY(1, 0, MT)
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < MT; ++i) sa[i] = na[i];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) sb[j] = nb[j];
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // nothing lands in LDS behind the loop
 #undef FP8_ISSUE
-    // result of a 32 x 32 tile: lane: column lane & 31; register q: row (q & 3) + 8 (q >> 2) + 4 (lane >> 5)
+#undef FP8_SCALES
+#undef FP8_READ
+#undef FP8_READ_SCALES
+#undef FP8_CONVERT_B
+#undef FP8_MULTIPLY
+    // Result of a 32 x 32 tile (B's columns are the rows of the instruction): lane: row lane & 31 of C; register q: column
+    // (q & 3) + 8 (q >> 2) + 4 (lane >> 5).  32 rows at a time go through the wave's own part of LDS, so that 16 bytes of a
+    // row are stored by one lane and a row's bytes by neighbouring ones.
+    constexpr int CW = NT * 32, PITCH = CW + 4, VE = 16 / sizeof(TO), PER = CW / VE, RSTEP = 64 / PER;
+    static_assert(sizeof(sh) >= 4 * 32 * PITCH * sizeof(float), "the result's rows fit where the stages were");
+    float *lw = reinterpret_cast<float *>(sh) + wave * 32 * PITCH;
+    typedef TO vo __attribute__((ext_vector_type(VE)));
+    const bool vec = g.c_vec;
+    __syncthreads();                        // the other waves have read their last stage
+    const int sr = lane / PER, scol = (lane % PER) * VE, gc = wn * CW + scol;
+    // cols - gc columns from here on: VE of them or fewer
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int i = 0; i < MT; ++i) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-            const int cc = wn * NT * 32 + j * 32 + r;
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int q = 0; q < 16; ++q) {
-                const int rr = wm * MT * 32 + i * 32 + (q & 3) + 8 * (q >> 2) + 4 * h;
-                if (rr < rows && cc < cols) {
-                    TO *d = C + (row0 + rr) * g.ldc + col0 + cc;
-                    *d = (TO)(g.accumulate ? (float)*d + acc[i][j][q] : acc[i][j][q]);
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+                *reinterpret_cast<f32x4 *>(lw + r * PITCH + j * 32 + 8 * q + 4 * h) = v;
+            }
+        __builtin_amdgcn_wave_barrier();    // a wave's LDS instructions are carried out in order
+#pragma unroll
+        for (int t = 0; t < 32 / RSTEP; ++t) {
+            const int lrow = t * RSTEP + sr, rr = (wm * MT + i) * 32 + lrow;
+            float v[VE];
+#pragma unroll
+            for (int q = 0; q < VE; q += 4) {
+                const f32x4 x = *reinterpret_cast<const f32x4 *>(lw + lrow * PITCH + scol + q);
+                v[q] = x[0]; v[q + 1] = x[1]; v[q + 2] = x[2]; v[q + 3] = x[3];
+            }
+            if (rr < rows && gc < cols) {
+                TO *d = C + (row0 + rr) * g.ldc + col0 + gc;
+                if (vec && gc + VE <= cols) {
+                    vo o;
+                    if (g.accumulate) {
+                        o = *reinterpret_cast<const vo *>(d);
+#pragma unroll
+                        for (int q = 0; q < VE; ++q) v[q] += (float)o[q];
+                    }
+#pragma unroll
+                    for (int q = 0; q < VE; ++q) o[q] = (TO)v[q];
+                    *reinterpret_cast<vo *>(d) = o;
+                } else {
+#pragma unroll
+                    for (int q = 0; q < VE; ++q)
+                        if (gc + q < cols) d[q] = (TO)(g.accumulate ? (float)d[q] + v[q] : v[q]);
                 }
             }
         }
+        __builtin_amdgcn_wave_barrier();
+    }
 }
 
 template <int MT, int NT, typename TO>
@@ -785,15 +894,31 @@ static int rows16_run(SkmCtx *ctx, const Fp8Args &g, const Fp8Float &fx, int x_d
 
 static int fp8_run(SkmCtx *ctx, Fp8Args g, int fa, int fb, int dtype, unsigned gy, hipStream_t st, const char *tag)
 {
-    g.tiles_n = (g.N + 127) / 128;
+    // 256 x 256 tiles (float32 results: 256 x 128, the converted operands need the registers) where they fill the GPU
+    const long wide = (long)((g.M + 255) / 256) * ((g.N + 255) / 256) * gy;
+    const bool big = !g.tiles && wide >= ctx->cu_count / 2;
+    const int bm = big ? 256 : 128, bn = big && dtype != SKM_DT_F32 ? 256 : 128;
+    if (!g.tiles) g.tiles_m = (g.M + bm - 1) / bm;
+    g.tiles_n = (g.N + bn - 1) / bn;
+    const int csize = skm_dt_size(dtype);
+    g.c_vec = aligned16(g.C, g.ldc * csize) && (g.eC * csize) % 16 == 0 && (g.zC * csize) % 16 == 0;
+    // a lane's offset inside a tile (by plan: inside A) is 32 bits wide
+    const long reach = g.tiles && g.slots ? g.rowsA : 256;
+    if (reach * g.lda > 0xFFFFFFFFL || reach * g.SA > 0x7FFFFFFFL || 256 * g.ldb > 0xFFFFFFFFL) {
+        skm_set_error("%s: %ld rows of %ld bytes are more than 4 GB", tag, reach, g.lda > g.ldb ? g.lda : g.ldb);
+        return SKM_ERR_UNSUPPORTED;
+    }
     const long total = (long)g.tiles_m * g.tiles_n;
     SKM_REQUIRE(total <= 0x7FFFFFFF && gy <= 65535, "%s: too many tiles", tag);
     if (total == 0 || gy == 0) return SKM_OK;
     SkmProfScope ps(ctx, tag, st);
-    switch (dtype) {
-    case SKM_DT_F32: fp8_launch<2, 2, float>(g, fa, fb, (unsigned)total, gy, st); break;
-    case SKM_DT_BF16: fp8_launch<2, 2, bf16_t>(g, fa, fb, (unsigned)total, gy, st); break;
-    default: fp8_launch<2, 2, f16_t>(g, fa, fb, (unsigned)total, gy, st); break;
+    switch (dtype * 2 + big) {
+    case SKM_DT_F32 * 2: fp8_launch<2, 2, float>(g, fa, fb, (unsigned)total, gy, st); break;
+    case SKM_DT_F32 * 2 + 1: fp8_launch<4, 2, float>(g, fa, fb, (unsigned)total, gy, st); break;
+    case SKM_DT_BF16 * 2: fp8_launch<2, 2, bf16_t>(g, fa, fb, (unsigned)total, gy, st); break;
+    case SKM_DT_BF16 * 2 + 1: fp8_launch<4, 4, bf16_t>(g, fa, fb, (unsigned)total, gy, st); break;
+    case SKM_DT_F16 * 2: fp8_launch<2, 2, f16_t>(g, fa, fb, (unsigned)total, gy, st); break;
+    default: fp8_launch<4, 4, f16_t>(g, fa, fb, (unsigned)total, gy, st); break;
     }
     SKM_HIP(hipGetLastError());
     return SKM_OK;
@@ -871,10 +996,9 @@ extern "C" int skm_gemm_fp8(void *ctx_, const void *A, const void *sA, int fmt_a
     g.sA = static_cast<const uint8_t *>(sA); g.sB = static_cast<const uint8_t *>(sB);
     g.lda = g.ldb = fp8_kpad(K);
     g.SA = g.SB = (int)fp8_sstride(K);
-    g.M = M; g.N = N; g.kb1 = (int)(fp8_kpad(K) / FP8_BLOCK);
+    g.M = M; g.N = N; g.rowsA = M; g.kb1 = (int)(fp8_kpad(K) / FP8_BLOCK);
     g.C = C; g.ldc = ldc; g.accumulate = accumulate != 0; g.slabs = 1;
     if (M <= FP8_FEW_ROWS) return rows16_run(ctx, g, fx, a_dtype, fmt_a, fmt_b, c_dtype, 1, (hipStream_t)stream);
-    g.tiles_m = (M + 127) / 128;
     return fp8_run(ctx, g, fmt_a, fmt_b, c_dtype, 1, (hipStream_t)stream, "k_gemm_fp8");
 }
 
@@ -908,7 +1032,7 @@ extern "C" int skm_gemm_fp8_experts(void *ctx_, const void *A, const void *sA, i
     g.sA = static_cast<const uint8_t *>(sA); g.sB = static_cast<const uint8_t *>(sW);
     g.lda = g.ldb = fp8_kpad(K);
     g.SA = g.SB = (int)fp8_sstride(K);
-    g.M = (int)n; g.N = N; g.kb1 = (int)(fp8_kpad(K) / FP8_BLOCK);
+    g.M = (int)n; g.N = N; g.rowsA = rows; g.kb1 = (int)(fp8_kpad(K) / FP8_BLOCK);
     g.C = C; g.ldc = N; g.slabs = 1;
     g.tiles = tiles; g.tile_count = first + E; g.pair = pair; g.slots = slots;
     g.eB = (long)N * g.ldb; g.esB = (long)N * g.SB;
@@ -941,9 +1065,8 @@ extern "C" int skm_gemm_fp8_experts_wgrad(void *ctx_, const void *A, const void 
     g.sA = static_cast<const uint8_t *>(sA); g.sB = static_cast<const uint8_t *>(sB);
     g.lda = g.ldb = max_tiles * FP8_BLOCK;
     g.SA = g.SB = (int)fp8_sstride(g.lda);
-    g.M = M; g.N = N;
+    g.M = M; g.N = N; g.rowsA = M;
     g.C = C; g.ldc = N; g.accumulate = accumulate != 0; g.slabs = 1;
     g.first = first; g.eC = (long)M * N;
-    g.tiles_m = (M + 127) / 128;
     return fp8_run(ctx, g, fmt_a, fmt_b, SKM_DT_F32, (unsigned)E, (hipStream_t)stream, "k_gemm_fp8_wgrad");
 }
