@@ -385,8 +385,9 @@ typedef __attribute__((address_space(1))) const void *glb_ptr;
 
 // C = A B'.  Workgroup: 4 waves as 2 x 2, a wave MT x NT tiles of 32 x 32 (v_mfma_scale_f32_32x32x64_f8f6f4), one block
 // of 128 k a stage, two stages in LDS filled by global loads that go there directly.
-//   LDS: a row's 128 bytes of a stage are one line; its 16-byte pieces are stored at piece ^ (row & 7), so that the 8
-//   lanes of a read phase (8 rows, the same piece) meet 8 different bank groups.  The loads put consecutive lanes'
+//   LDS: a row's 128 bytes of a stage are one line; its 16-byte pieces are stored at piece ^ ((row >> 1) & 7), so that the
+//   lanes of a read phase (16 rows, the same piece) meet different bank groups (row & 7 costs 4 cycles more per read,
+//   measured).  The loads put consecutive lanes'
 //   pieces at consecutive addresses, so the exchange is made on the global side, within the line.
 //   The scales come the same way, a dword (four blocks) of every row in every fourth stage.
 //   The 8-bit matrix instructions add 8 products at a time in a window of 13 bits below the largest of the 8 (a product
@@ -457,21 +458,23 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
     const uint8_t *ba = g.A + a0 * g.lda + (long)kb0 * FP8_BLOCK, *bb = B + col0 * g.ldb + (long)kb0 * FP8_BLOCK;
     const uint8_t *bsa = g.sA + a0 * g.SA, *bsb = sB + (long)col0 * g.SB;
     // one row of A (B) per 8 lanes and load: rows behind the last repeat it
-    const int lr = lane >> 3, lp = ((lane & 7) ^ lr) * 16;
+    const int lr = lane >> 3;
+#define FP8_PIECE(I) (((lane & 7) ^ ((((I) & 1) << 2) | (lr >> 1))) * 16)   // rows 8 I + lr: exchanged by (row >> 1) & 7
     unsigned oa[MT * 2], ob[NT * 2];
 #pragma unroll
     for (int i = 0; i < MT * 2; ++i) {
         int rr = (wave * MT * 2 + i) * 8 + lr;
         rr = rr < rows ? rr : rows - 1;
         if (by_pair) rr = g.pair[row0 + rr] / g.slots;
-        oa[i] = (unsigned)rr * (unsigned)g.lda + lp;
+        oa[i] = (unsigned)rr * (unsigned)g.lda + FP8_PIECE(i);
     }
 #pragma unroll
     for (int i = 0; i < NT * 2; ++i) {
         int cc = (wave * NT * 2 + i) * 8 + lr;
         cc = cc < cols ? cc : cols - 1;
-        ob[i] = (unsigned)cc * (unsigned)g.ldb + lp;
+        ob[i] = (unsigned)cc * (unsigned)g.ldb + FP8_PIECE(i);
     }
+#undef FP8_PIECE
     // scales: 64 rows a load, the rows of A, then the columns of B; waves take turns
     constexpr int CHUNKS = (BM + BN) / 64, MINE = (CHUNKS + 3) / 4;
     unsigned os[MINE];
@@ -513,8 +516,8 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
 
-    // this lane's pieces of a half H: 4 H + 2 h and the next, exchanged by row & 7 = r & 7
-    const int x7 = r & 7;
+    // this lane's pieces of a half H: 4 H + 2 h and the next, exchanged by (row >> 1) & 7 = (r >> 1) & 7
+    const int x7 = (r >> 1) & 7;
     int at[2][2];
 #pragma unroll
     for (int H = 0; H < 2; ++H)
