@@ -492,20 +492,21 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
     }
 
     // loads of the stage S (blocks from kb0) into buffer ST; scales of the blocks 4 G .. 4 G + 3
-#define FP8_ISSUE(S, ST)                                                                                               \
+#define FP8_ISSUE1(S, L, BUF)                                                                                          \
     {                                                                                                                  \
-        const uint8_t *la = ba + (long)(S) * FP8_BLOCK, *lb = bb + (long)(S) * FP8_BLOCK;                              \
-        _Pragma("unroll") for (int i = 0; i < MT * 2; ++i) __builtin_amdgcn_global_load_lds(                           \
-            (glb_ptr)(la + oa[i]), (lds_ptr)&sh[(ST) * STAGE + (wave * MT * 2 + i) * 8 * FP8_BLOCK], 16, 0, 0);        \
-        _Pragma("unroll") for (int i = 0; i < NT * 2; ++i) __builtin_amdgcn_global_load_lds(                           \
-            (glb_ptr)(lb + ob[i]), (lds_ptr)&sh[(ST) * STAGE + (BM + (wave * NT * 2 + i) * 8) * FP8_BLOCK], 16, 0, 0); \
+        const uint8_t *p_ = ((L) < MT * 2 ? ba : bb) + (long)(S) * FP8_BLOCK;                                          \
+        const unsigned o_ = (L) < MT * 2 ? oa[(L) < MT * 2 ? (L) : 0] : ob[(L) < MT * 2 ? 0 : (L) - MT * 2];            \
+        const int row8_ = (L) < MT * 2 ? wave * MT * 2 + (L) : BM / 8 + wave * NT * 2 + (L) - MT * 2;                   \
+        __builtin_amdgcn_global_load_lds((glb_ptr)(p_ + o_), (lds_ptr)((BUF) + row8_ * 8 * FP8_BLOCK), 16, 0, 0);      \
     }
-#define FP8_SCALES(G)                                                                                                  \
+#define FP8_ISSUE(S, BUF)                                                                                              \
+    _Pragma("unroll") for (int l_ = 0; l_ < LOADS; ++l_) FP8_ISSUE1(S, l_, BUF)
+#define FP8_SCALES(G, BUF)                                                                                                \
     _Pragma("unroll") for (int i = 0; i < MINE; ++i) {                                                                 \
         const int c = wave + 4 * i;                                                                                    \
         const uint8_t *l = (c * 64 < BM ? bsa : bsb) + (long)(G) * 4;                                                  \
         if (CHUNKS % 4 == 0 || c < CHUNKS)                                                                             \
-            __builtin_amdgcn_global_load_lds((glb_ptr)(l + os[i]), (lds_ptr)&sh[2 * STAGE + ((G) & 1) * GROUP + c * 256], 4, 0, 0); \
+            __builtin_amdgcn_global_load_lds((glb_ptr)(l + os[i]), (lds_ptr)((BUF) + c * 256), 4, 0, 0);                \
     }
 
     f32x16 acc[MT][NT];
@@ -525,23 +526,25 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
         for (int u = 0; u < 2; ++u) at[H][u] = r * FP8_BLOCK + ((H * 4 + h * 2 + u) ^ x7) * 16;
     i32x8 fa[2][MT], fb[2][NT];
     int sa[MT], sb[NT], na[MT], nb[NT];
-#define FP8_READ(H, ST)                                                                                                \
-    _Pragma("unroll") for (int i = 0; i < MT; ++i) {                                                                   \
-        const uint8_t *l = &sh[(ST) * STAGE + (wm * MT + i) * 32 * FP8_BLOCK];                                         \
-        const i32x4 lo = *reinterpret_cast<const i32x4 *>(l + at[H][0]), hi = *reinterpret_cast<const i32x4 *>(l + at[H][1]); \
-        fa[H][i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);                                            \
-    }                                                                                                                  \
-    _Pragma("unroll") for (int j = 0; j < NT; ++j) {                                                                   \
-        const uint8_t *l = &sh[(ST) * STAGE + (BM + (wn * NT + j) * 32) * FP8_BLOCK];                                  \
-        const i32x4 lo = *reinterpret_cast<const i32x4 *>(l + at[H][0]), hi = *reinterpret_cast<const i32x4 *>(l + at[H][1]); \
-        fb[H][j] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);                                            \
-    }
-#define FP8_READ_SCALES(KB)                                                                                            \
+    // fragment F of half H: rows of A, then columns of B
+#define FP8_READ1(H, F, BUF)                                                                                           \
     {                                                                                                                  \
-        const uint8_t *l = &sh[2 * STAGE + (((KB) >> 2) & 1) * GROUP + r * 4 + ((KB) & 3)];                            \
+        const uint8_t *p_ = (BUF) + ((F) < MT ? wm * MT + (F) : MT + wn * NT + (F)) * 32 * FP8_BLOCK;                  \
+        const i32x4 lo_ = *reinterpret_cast<const i32x4 *>(p_ + at[H][0]), hi_ = *reinterpret_cast<const i32x4 *>(p_ + at[H][1]); \
+        const i32x8 v_ = __builtin_shufflevector(lo_, hi_, 0, 1, 2, 3, 4, 5, 6, 7);                                    \
+        if ((F) < MT) fa[H][(F) < MT ? (F) : 0] = v_;                                                                  \
+        else fb[H][(F) < MT ? 0 : (F) - MT] = v_;                                                                      \
+    }
+#define FP8_READ(H, BUF)                                                                                               \
+    _Pragma("unroll") for (int f = 0; f < MT + NT; ++f) FP8_READ1(H, f, BUF)
+#define FP8_READ_SCALES(KB, BUF)                                                                                           \
+    {                                                                                                                  \
+        const uint8_t *l = (BUF) + r * 4 + ((KB) & 3);                                                                 \
         _Pragma("unroll") for (int i = 0; i < MT; ++i) na[i] = l[(wm * MT + i) * 128];                                 \
         _Pragma("unroll") for (int j = 0; j < NT; ++j) nb[j] = l[(BM + (wn * NT + j) * 32) * 4];                       \
     }
+#define FP8_TILE(H, I, J)                                                                                              \
+    acc[I][J] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[H][J], fa[H][I], acc[I][J], FB, FA, 0, sb[J], 0, sa[I]);
     // rows I0 .. I1 - 1 of the wave's tiles times half H
     bf16x8 xb[NT][4];
 #define FP8_CONVERT_B(H)                                                                                               \
@@ -558,39 +561,87 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
                     acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xb[j][t], xa, acc[i][j], 0, 0, 0);             \
             }                                                                                                          \
         } else {                                                                                                       \
-            _Pragma("unroll") for (int j = 0; j < NT; ++j)                                                             \
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[H][j], fa[H][i], acc[i][j], FB, FA, 0,  \
-                                                                            sb[j], 0, sa[i]);                          \
+            _Pragma("unroll") for (int j = 0; j < NT; ++j) FP8_TILE(H, i, j)                                           \
         }                                                                                                              \
     }
+#define FP8_STAGE(S) (sh + ((S) & 1) * STAGE)
+#define FP8_SCALE_GROUP(KB) (sh + 2 * STAGE + (((KB) >> 2) & 1) * GROUP)
     const int n = kb1 - kb0;
     if (n > 0) {
-        FP8_SCALES(kb0 >> 2)
-        if (n > 1 && ((kb0 + 1) >> 2) != (kb0 >> 2)) { FP8_SCALES((kb0 + 1) >> 2) }
-        FP8_ISSUE(0, 0)
+        FP8_SCALES(kb0 >> 2, FP8_SCALE_GROUP(kb0))
+        if (n > 1 && ((kb0 + 1) >> 2) != (kb0 >> 2)) { FP8_SCALES((kb0 + 1) >> 2, FP8_SCALE_GROUP(kb0 + 1)) }
+        FP8_ISSUE(0, sh)
         if (n > 1) {
-            FP8_ISSUE(1, 1)
+            FP8_ISSUE(1, sh + STAGE)
             asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
         } else {
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         }
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        FP8_READ(0, 0)
-        FP8_READ_SCALES(kb0)
+        FP8_READ(0, sh)
+        FP8_READ_SCALES(kb0, FP8_SCALE_GROUP(kb0))
 #pragma unroll
         for (int i = 0; i < MT; ++i) sa[i] = na[i];
 #pragma unroll
         for (int j = 0; j < NT; ++j) sb[j] = nb[j];
     }
+    // Behind the barrier of a stage: the loads of stage s2 fill the buffer that it frees while the next stage is read.  The
+    // two buffers (and the two groups of scales, or the same group with the same bytes) do not overlap: restrict lets the
+    // compiler mix the instructions.
+    auto late = [&](int s2, int kb, uint8_t *__restrict__ fill, const uint8_t *__restrict__ next,
+                    uint8_t *__restrict__ fill_scales, const uint8_t *__restrict__ next_scales) __attribute__((always_inline)) {
+        FP8_SCALES((kb0 + s2) >> 2, fill_scales)
+        if (sizeof(TO) == 4) {
+            FP8_ISSUE(s2, fill)
+            FP8_MULTIPLY(0, MT - 1, MT)
+            FP8_READ(0, next)
+            FP8_READ_SCALES(kb + 1, next_scales)
+            FP8_CONVERT_B(1)
+            FP8_MULTIPLY(1, 0, MT)
+        } else {
+            // In this order: the four waves' loads take 16 cycles each on the way to the cache, a wave that waits to issue
+            // one multiplies nothing, so there is one beside every multiplication (64 cycles).
+            constexpr int EACH = (LOADS + (MT + 1) * NT - 1) / ((MT + 1) * NT);
+#pragma unroll
+            for (int u = 0; u < (MT + 1) * NT; ++u) {
+                if (u < NT) {
+                    FP8_TILE(0, MT - 1, u)
+                } else {
+                    FP8_TILE(1, (u - NT) / NT, (u - NT) % NT)
+                }
+#pragma unroll
+                for (int l = u * EACH; l < (u + 1) * EACH; ++l)
+                    if (l < LOADS) FP8_ISSUE1(s2, l, fill)
+                if (u >= NT && u < NT + MT + NT) {
+                    FP8_READ1(0, u - NT, next)
+                }
+                if (u == (MT + 2 * NT < (MT + 1) * NT ? MT + 2 * NT : (MT + 1) * NT - 1)) {
+                    FP8_READ_SCALES(kb + 1, next_scales)
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    };
     // One straight block per stage, without a branch: behind the last stage the last one is loaded again into the free
     // buffer, and what is read of it is not used; a group's scales are loaded again with each of its stages.
     for (int s = 0; s < n; ++s) {
-        const int st = s & 1, kb = kb0 + s;
-        const int s2 = s + 2 < n ? s + 2 : n - 1;
-        FP8_READ(1, st)
-        FP8_CONVERT_B(0)
-        FP8_MULTIPLY(0, 0, MT - 1)
+        const int kb = kb0 + s, s2 = s + 2 < n ? s + 2 : n - 1;
+        if (sizeof(TO) == 4) {
+            FP8_READ(1, FP8_STAGE(s))
+            FP8_CONVERT_B(0)
+            FP8_MULTIPLY(0, 0, MT - 1)
+        } else {
+            constexpr int EACH = (MT + NT + (MT - 1) * NT - 1) / ((MT - 1) * NT);
+#pragma unroll
+            for (int u = 0; u < (MT - 1) * NT; ++u) {
+                FP8_TILE(0, u / NT, u % NT)
+#pragma unroll
+                for (int f = u * EACH; f < (u + 1) * EACH; ++f)
+                    if (f < MT + NT) FP8_READ1(1, f, FP8_STAGE(s))
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
         // the multiplications stand in front of the barrier (an empty statement that takes their results; it reads nothing)
 #pragma unroll
         for (int i = 0; i < MT - 1; ++i)
@@ -599,16 +650,7 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
         __builtin_amdgcn_sched_barrier(0);
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
-        FP8_SCALES((kb0 + s2) >> 2)
-        FP8_ISSUE(s2, st)
-        FP8_MULTIPLY(0, MT - 1, MT)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) asm volatile("" : "+a"(acc[MT - 1][j]));
-        __builtin_amdgcn_sched_barrier(0);
-        FP8_READ(0, st ^ 1)
-        FP8_READ_SCALES(kb + 1)
-        FP8_CONVERT_B(1)
-        FP8_MULTIPLY(1, 0, MT)
+        late(s2, kb, FP8_STAGE(s), FP8_STAGE(s + 1), FP8_SCALE_GROUP(kb0 + s2), FP8_SCALE_GROUP(kb + 1));
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < MT; ++i) sa[i] = na[i];
@@ -616,6 +658,11 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
         for (int j = 0; j < NT; ++j) sb[j] = nb[j];
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // nothing lands in LDS behind the loop
+#undef FP8_STAGE
+#undef FP8_SCALE_GROUP
+#undef FP8_READ1
+#undef FP8_ISSUE1
+#undef FP8_TILE
 #undef FP8_ISSUE
 #undef FP8_SCALES
 #undef FP8_READ
