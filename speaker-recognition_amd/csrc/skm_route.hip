@@ -154,12 +154,300 @@ __device__ void route_row(const RouteArgs &a, long row, int lane)
     }
 }
 
+// Every row in float64: what the fast kernel has no form for (float64 logits that need probabilities, many groups).
 template <typename T, int NV>
-__global__ __launch_bounds__(256) void k_route(RouteArgs a)
+__global__ __launch_bounds__(256) void k_route_wide(RouteArgs a)
 {
     const int lane = threadIdx.x & 63;
     const long row = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row < a.T) route_row<T, NV>(a, row, lane);
+}
+
+// reductions over the L = 16 or 64 lanes of a row; every lane gets the result
+template <int CTRL, typename V>
+__device__ __forceinline__ V dpp_ror(V v)
+{
+    const int i = __builtin_bit_cast(int, v);
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xF, 0xF, false));
+}
+template <int L, typename V, typename F>
+__device__ __forceinline__ V row_reduce(V v, F f)
+{
+    v = f(v, dpp_ror<0x128>(v));
+    v = f(v, dpp_ror<0x124>(v));
+    v = f(v, dpp_ror<0x122>(v));
+    v = f(v, dpp_ror<0x121>(v));
+    if (L == 64) {
+        const int i = __builtin_bit_cast(int, v);
+        const V a = __builtin_bit_cast(V, __builtin_amdgcn_readlane(i, 0)), b = __builtin_bit_cast(V, __builtin_amdgcn_readlane(i, 16));
+        const V c = __builtin_bit_cast(V, __builtin_amdgcn_readlane(i, 32)), d = __builtin_bit_cast(V, __builtin_amdgcn_readlane(i, 48));
+        v = f(f(a, b), f(c, d));
+    }
+    return v;
+}
+template <int L> __device__ __forceinline__ unsigned row_max(unsigned v)
+{
+    return row_reduce<L>(v, [](unsigned a, unsigned b) { return a > b ? a : b; });
+}
+template <int L> __device__ __forceinline__ float row_max(float v)
+{
+    return row_reduce<L>(v, [](float a, float b) { return fmaxf(a, b); });
+}
+template <int L> __device__ __forceinline__ float row_sum(float v)
+{
+    return row_reduce<L>(v, [](float a, float b) { return a + b; });
+}
+
+// order of float32 numbers as unsigned ones (0 is below all of them), and back
+__device__ __forceinline__ unsigned order_bits(float x)
+{
+    const unsigned u = __float_as_uint(x);
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float order_value(unsigned k)
+{
+    return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
+}
+
+// One row per L lanes (16: four rows a wave), lane l holds the experts l, l + L, ...: NV of them.
+//   A choice is a 32-bit key: the float32 number in an order-preserving form, its last log2(NV) bits replaced by the place
+//   in the lane (lower place = larger), so that one v_max keeps the expert with it.  The largest of the row comes from four
+//   DPP steps, the lowest lane that holds it from a ballot.
+//   The order itself is that of 64 bits.  Half-precision logits without a bias are exact in the key.  Otherwise the choice
+//   is only trusted where neighbours in it (the first not taken among them) are further apart than what float32
+//   arithmetic and the cut bits can have moved them; other rows -- a few in ten thousand for random logits, and those with
+//   NaN or infinities -- are done again by the whole wave in float64 (route_row).  Error of p: exp of a difference d <= 0 by
+//   exp2(d log2 e): (3 |d| + 2) 2^-24 of it, |d| exp(d) <= 0.37; the sum S of E terms: (NV + 6) additions and the terms'
+//   errors, in all (NV + 48) 2^-24 / S bounds it; 1 / (1 + exp(-x)): p (1 - p) |x| <= 0.23, 8 2^-24.  Error of c = p + bias:
+//   that and |c| 2^-24; of the key: |c| 2^-(23 - bits).
+template <typename T, int NV, int L>
+__global__ __launch_bounds__(256) void k_route(RouteArgs a)
+{
+    constexpr int R = 64 / L, BITS = NV == 1 ? 0 : NV == 2 ? 1 : NV == 4 ? 2 : NV == 8 ? 3 : NV == 16 ? 4 : NV == 32 ? 5 : 6;
+    constexpr bool HALF = sizeof(T) == 2;
+    constexpr int PL = (ROUTE_MAX_K + L - 1) / L;       // places of a lane
+    constexpr int NV64 = (NV * L + 63) / 64;
+    __shared__ int32_t chosen[4 * R][ROUTE_MAX_K];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane % L, sub = lane / L;
+    const long row0 = ((long)blockIdx.x * 4 + wave) * R;
+    if (row0 >= a.T) return;                            // whole waves
+    const long row = row0 + sub < a.T ? row0 + sub : a.T - 1;
+    const T *x = static_cast<const T *>(a.x) + row * a.ldx;
+    const float inf = __builtin_inff();
+    float c[NV];
+    bool bad = false;
+    float top = -inf;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int e = l + L * i;
+        c[i] = e < a.E ? (float)x[e] + 0.f : -inf;      // -0 and 0 are the same number
+    }
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        bad |= c[i] != c[i];
+        top = fmaxf(top, c[i]);
+    }
+    bool none[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) none[i] = c[i] == -inf;
+    bad |= !a.sigmoid && top == inf;
+    // float64 logits below float32's range are -inf as float32 numbers and no masked ones
+    if (sizeof(T) == 8) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) bad |= l + L * i < a.E && none[i] && x[l + L * i] != (T)-inf;
+    }
+    float total = 1.f, err = 0.f;
+    float p[NV];
+    const bool probabilities = a.bias || a.groups > 1 || (!a.renorm && !a.sigmoid);
+    if (probabilities) {
+        if (a.sigmoid) {
+            err = 8.f * 5.9604645e-8f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) p[i] = 1.f / (1.f + __expf(-c[i]));
+        } else {
+            top = row_max<L>(top);
+            total = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                p[i] = none[i] ? 0.f : __expf(c[i] - top);
+                total += p[i];
+            }
+            total = row_sum<L>(total);
+            const float inv = 1.f / total;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) p[i] *= inv;
+            err = (float)(NV + 48) * 5.9604645e-8f * inv;
+        }
+        if (a.bias) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int e = l + L * i;
+                const float b = e < a.E ? a.bias[e] : -inf;
+                p[i] += b;
+                none[i] |= b == -inf;
+                bad |= !none[i] && p[i] != p[i];
+            }
+        }
+    }
+    bool doubt = false;
+    if (a.groups > 1) {
+        // the two largest c of a group in every lane of the row; lane g keeps those of group g
+        const int per = a.E / a.groups;
+        const unsigned inv = per > 1 ? (unsigned)(((1ull << 32) + per - 1) / per) : 0;
+        float s1 = -inf, s2 = -inf;
+        for (int g = 0; g < a.groups; ++g) {
+            float f1 = -inf, f2 = -inf;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int e = l + L * i;
+                const int ge = per > 1 ? (int)__umulhi((unsigned)e, inv) : e;
+                const float v = ge == g && !none[i] ? p[i] : -inf;
+                f2 = fmaxf(f2, fminf(f1, v));
+                f1 = fmaxf(f1, v);
+            }
+#define ROUTE_TOP2(CTRL)                                            \
+    {                                                               \
+        const float o1 = dpp_ror<CTRL>(f1), o2 = dpp_ror<CTRL>(f2); \
+        f2 = fmaxf(fmaxf(f2, o2), fminf(f1, o1));                   \
+        f1 = fmaxf(f1, o1);                                         \
+    }
+            ROUTE_TOP2(0x128) ROUTE_TOP2(0x124) ROUTE_TOP2(0x122) ROUTE_TOP2(0x121)
+#undef ROUTE_TOP2
+            if (L == 64) {
+#pragma unroll
+                for (int m = 32; m > 8; m >>= 1) {
+                    const float o1 = __shfl_xor(f1, m), o2 = __shfl_xor(f2, m);
+                    f2 = fmaxf(fmaxf(f2, o2), fminf(f1, o1));
+                    f1 = fmaxf(f1, o1);
+                }
+            }
+            if (l == g) {
+                s1 = f1;
+                s2 = f2;
+            }
+        }
+        const bool pair = a.group_top == 2 && s2 != -inf;
+        const float score = pair ? s1 + s2 : s1;
+        // what two scores can have been moved against each other
+        float near = s1 == -inf ? 0.f : 4.f * err + 2.3841858e-7f * (fabsf(s1) + (pair ? fabsf(s2) : 0.f));
+        near = row_max<L>(near);
+        int ahead = 0;
+        for (int g = 0; g < a.groups; ++g) {
+            const float o = __shfl(score, sub * L + g);
+            ahead += (o > score || (o == score && g < l)) ? 1 : 0;
+        }
+        const bool kept = l < a.groups && ahead < a.group_k;
+        const unsigned long long all = __ballot(kept);
+        for (int g = 0; g < a.groups; ++g) {
+            const float o = __shfl(score, sub * L + g);
+            const bool ok = (all >> (sub * L + g)) & 1;
+            if (l < a.groups && ok != kept && (score != -inf || o != -inf)) doubt |= fabsf(score - o) <= near;
+        }
+        const unsigned long long stay = L == 64 ? all : (all >> (sub * L)) & 0xFFFFull;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int e = l + L * i;
+            const int ge = per > 1 ? (int)__umulhi((unsigned)e, inv) : e;
+            none[i] |= ge >= a.groups || !((stay >> (ge & 63)) & 1);
+        }
+    }
+    unsigned key[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        key[i] = none[i] ? 0u : (order_bits(a.bias ? p[i] + 0.f : c[i]) & ~(unsigned)(NV - 1)) | (unsigned)(NV - 1 - i);
+    const bool exact = HALF && !a.bias;
+    for (int j = l; j < a.k; j += L) chosen[wave * R + sub][j] = -1;
+    __builtin_amdgcn_wave_barrier();
+    unsigned before = 0;
+    const int rounds = exact ? a.k : a.k + 1;
+    for (int j = 0; j < rounds; ++j) {
+        unsigned mine = key[0];
+#pragma unroll
+        for (int i = 1; i < NV; ++i) mine = key[i] > mine ? key[i] : mine;
+        const unsigned best = row_max<L>(mine);
+        const unsigned long long who = __ballot(mine == best);
+        const int first = L == 64 ? __ffsll((long long)who) - 1 : __ffs((int)((who >> (sub * L)) & 0xFFFFu)) - 1;
+        if (!exact && j > 0 && best != 0) {
+            if (a.bias) {
+                const float f = order_value(before & ~(unsigned)(NV - 1)), g = order_value(best & ~(unsigned)(NV - 1));
+                doubt |= f - g <= 2.f * err + fmaxf(fabsf(f), fabsf(g)) * (1.1920929e-7f * (float)(1 + 2 * NV));
+            } else {
+                doubt |= ((before ^ best) & ~(unsigned)(NV - 1)) == 0;
+            }
+        }
+        before = best;
+        if (l == first && best != 0) {
+            const int i = NV - 1 - (int)(best & (unsigned)(NV - 1));
+            if (j < a.k) chosen[wave * R + sub][j] = l + L * i;
+        }
+        const unsigned gone = l == first ? best : 0u;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) key[i] = key[i] == gone ? 0u : key[i];
+    }
+    __builtin_amdgcn_wave_barrier();
+    // weights: lane l has the places l, l + L, ...
+    int id[PL];
+    float t[PL];
+    if (a.renorm) {
+        T xs[PL];
+        float M = -inf;
+#pragma unroll
+        for (int q = 0; q < PL; ++q) {
+            const int j = l + q * L;
+            id[q] = j < a.k ? chosen[wave * R + sub][j] : -1;
+            xs[q] = id[q] >= 0 ? x[id[q]] : (T)-inf;
+            if (sizeof(T) < 8) M = fmaxf(M, (float)xs[q]);
+        }
+        float sum = 0.f;
+        if (sizeof(T) == 8) {               // without a bias: the first choice is the largest
+            const int lead = chosen[wave * R + sub][0];
+            double Md = lead >= 0 ? (double)x[lead] : 0.0;
+            if (a.sigmoid && Md > 0.0) Md = 0.0;
+#pragma unroll
+            for (int q = 0; q < PL; ++q) {
+                const double v = (double)xs[q];
+                t[q] = id[q] < 0 ? 0.f : !a.sigmoid ? expf((float)(v - Md))
+                                       : v <= 0.0   ? expf((float)(v - Md)) / (1.f + expf((float)v))
+                                                    : 1.f / (1.f + expf((float)-v));
+                sum += t[q];
+            }
+        } else {
+            M = row_max<L>(M);
+            if (a.sigmoid && M > 0.f) M = 0.f;
+#pragma unroll
+            for (int q = 0; q < PL; ++q) {
+                t[q] = id[q] >= 0 ? route_share((float)xs[q], M, a.sigmoid) : 0.f;
+                sum += t[q];
+            }
+        }
+        sum = row_sum<L>(sum);
+        const float f = sum > 0.f ? a.scale / sum : 0.f;
+#pragma unroll
+        for (int q = 0; q < PL; ++q) t[q] *= f;
+    } else {
+#pragma unroll
+        for (int q = 0; q < PL; ++q) {
+            const int j = l + q * L;
+            id[q] = j < a.k ? chosen[wave * R + sub][j] : -1;
+            const float xs = id[q] >= 0 ? (float)x[id[q]] : -inf;
+            t[q] = id[q] < 0 ? 0.f : a.scale * (a.sigmoid ? 1.f / (1.f + expf(-xs)) : expf(xs - top) / total);
+        }
+    }
+    const unsigned long long again = __ballot(bad || doubt);
+    const unsigned long long rowmask = (L == 64 ? ~0ull : 0xFFFFull << (sub * L));
+    if (row0 + sub < a.T && !(again & rowmask)) {
+#pragma unroll
+        for (int q = 0; q < PL; ++q) {
+            const int j = l + q * L;
+            if (j < a.k) {
+                a.ids[row * a.k + j] = id[q];
+                a.w[row * a.k + j] = t[q];
+            }
+        }
+    }
+    if (!again) return;
+    for (int s = 0; s < R; ++s)             // the rows in doubt, one after the other
+        if (row0 + s < a.T && (again & (L == 64 ? ~0ull : 0xFFFFull << (s * L)))) route_row<T, NV64>(a, row0 + s, lane);
 }
 
 struct RouteBackArgs {
@@ -236,26 +524,41 @@ __global__ __launch_bounds__(256) void k_route_backward(RouteBackArgs a)
     }
 }
 
-static int route_nv(int E)
+template <typename T, int NV, int L>
+static void route_go(const RouteArgs &a, hipStream_t st)
 {
-    int nv = 1;
-    while (nv * 64 < E) nv *= 2;
-    return nv;
+    const long per = 4 * (64 / L);
+    hipLaunchKernelGGL((k_route<T, NV, L>), dim3((unsigned)((a.T + per - 1) / per)), dim3(256), 0, st, a);
+}
+
+template <typename T, int NV>
+static void route_go_wide(const RouteArgs &a, hipStream_t st)
+{
+    hipLaunchKernelGGL((k_route_wide<T, NV>), dim3((unsigned)((a.T + 3) / 4)), dim3(256), 0, st, a);
 }
 
 template <typename T>
 static void route_launch(const RouteArgs &a, hipStream_t st)
 {
-    const dim3 grid((unsigned)((a.T + 3) / 4)), block(256);
-    switch (route_nv(a.E)) {
-    case 1: hipLaunchKernelGGL((k_route<T, 1>), grid, block, 0, st, a); break;
-    case 2: hipLaunchKernelGGL((k_route<T, 2>), grid, block, 0, st, a); break;
-    case 4: hipLaunchKernelGGL((k_route<T, 4>), grid, block, 0, st, a); break;
-    case 8: hipLaunchKernelGGL((k_route<T, 8>), grid, block, 0, st, a); break;
-    case 16: hipLaunchKernelGGL((k_route<T, 16>), grid, block, 0, st, a); break;
-    case 32: hipLaunchKernelGGL((k_route<T, 32>), grid, block, 0, st, a); break;
-    default: hipLaunchKernelGGL((k_route<T, 64>), grid, block, 0, st, a); break;
+    // 16 lanes a row up to 256 experts (16 of them a lane), the whole wave above.
+    // In float64 throughout: probabilities of float64 logits; more groups than a row has lanes.
+    const bool wide = (sizeof(T) == 8 && (a.bias || a.groups > 1 || (!a.renorm && !a.sigmoid))) || a.groups > (a.E <= 256 ? 16 : 64);
+    if (wide) {
+        if (a.E <= 64) route_go_wide<T, 1>(a, st);
+        else if (a.E <= 256) route_go_wide<T, 4>(a, st);
+        else if (a.E <= 1024) route_go_wide<T, 16>(a, st);
+        else route_go_wide<T, 64>(a, st);
+        return;
     }
+    if (a.E <= 16) route_go<T, 1, 16>(a, st);
+    else if (a.E <= 32) route_go<T, 2, 16>(a, st);
+    else if (a.E <= 64) route_go<T, 4, 16>(a, st);
+    else if (a.E <= 128) route_go<T, 8, 16>(a, st);
+    else if (a.E <= 256) route_go<T, 16, 16>(a, st);
+    else if (a.E <= 512) route_go<T, 8, 64>(a, st);
+    else if (a.E <= 1024) route_go<T, 16, 64>(a, st);
+    else if (a.E <= 2048) route_go<T, 32, 64>(a, st);
+    else route_go<T, 64, 64>(a, st);
 }
 
 extern "C" int skm_route(void *ctx_, const void *x, int dtype, long T, int E, long ldx, int k, int scores,

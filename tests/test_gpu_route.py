@@ -85,12 +85,34 @@ def test_route_ties_and_near_ties(eng):
     x = 5.0 + r.permutation(T * E).reshape(T, E) * 1e-12
     ids, _ = eng.route(torch.from_numpy(x).cuda(), k)
     np.testing.assert_array_equal(ids.cpu().numpy(), rc.route(x, k)[0])
+    # zeros of either sign are one number; whole rows of equal logits
+    for dt in (torch.bfloat16, torch.float32, torch.float64):
+        z = torch.zeros(T, E, dtype=dt)
+        z[r.rand(T, E) < 0.5] = -0.0
+        z[3] = 1.5
+        ids, w = eng.route(z.cuda(), k)
+        assert ids.cpu().tolist() == [list(range(k))] * T
+        assert (torch.abs(w.cpu().double() - 1 / k) <= 4 * rc.U32 / k).all()
     # groups whose scores differ by 1e-9
     x = np.tile(r.randn(T, 12), (1, 8)) + r.randn(T, 96) * 1e-9
     b = (r.randn(96) * 0.1).astype(np.float32)
     b = np.tile(b[:12], 8)
     ids, _ = eng.route(torch.from_numpy(x).cuda(), k, bias=torch.from_numpy(b).cuda(), groups=8, group_k=3)
     np.testing.assert_array_equal(ids.cpu().numpy(), rc.route(x, k, "softmax", b, 8, 3)[0])
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+def test_route_many_rows(eng, scores):
+    """more rows than a launch has workgroups at once, the last workgroup partly filled; float32 and half-precision"""
+    for dtype, T, E, k, bias, groups, group_k in (("f32", 20011, 256, 8, True, 8, 4), ("bf16", 30001, 128, 8, True, 1, 1),
+                                                  ("f64", 5003, 512, 20, False, 1, 1), ("f16", 4099, 300, 3, True, 6, 2)):
+        x, x64 = _logits(T, E, dtype, T, False, 1.5)
+        b = (np.random.RandomState(8).randn(E) * 0.05).astype(np.float32) if bias else None
+        ids, w = eng.route(x.cuda(), k, scores=scores, bias=torch.from_numpy(b).cuda() if bias else None, groups=groups,
+                           group_k=group_k)
+        rids, rw, _ = rc.route(x64, k, scores, b, groups, group_k)
+        np.testing.assert_array_equal(ids.cpu().numpy(), rids)
+        _check_weights(w.cpu().numpy().astype(np.float64), rw, x64, rids, 1.0)
 
 
 @pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
