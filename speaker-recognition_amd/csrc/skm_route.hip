@@ -30,6 +30,69 @@ __device__ __forceinline__ A route_share(A x, A M, int sigmoid)
     return (A)1 / ((A)1 + exp(-x));
 }
 
+// a lane's value from another lane of its 16 (CTRL 0x120 + n: n lanes on)
+template <int CTRL, typename V>
+__device__ __forceinline__ V dpp_ror(V v)
+{
+    const int i = __builtin_bit_cast(int, v);
+    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xF, 0xF, false));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp_ror(double v)
+{
+    const long long i = __builtin_bit_cast(long long, v);
+    const int lo = dpp_ror<CTRL>((int)i), hi = dpp_ror<CTRL>((int)(i >> 32));
+    return __builtin_bit_cast(double, ((long long)hi << 32) | (unsigned)lo);
+}
+__device__ __forceinline__ double read_lane(double v, int lane)
+{
+    const long long i = __builtin_bit_cast(long long, v);
+    const int lo = __builtin_amdgcn_readlane((int)i, lane), hi = __builtin_amdgcn_readlane((int)(i >> 32), lane);
+    return __builtin_bit_cast(double, ((long long)hi << 32) | (unsigned)lo);
+}
+template <typename F>
+__device__ __forceinline__ double wave_reduce(double v, F f)
+{
+    v = f(v, dpp_ror<0x128>(v));
+    v = f(v, dpp_ror<0x124>(v));
+    v = f(v, dpp_ror<0x122>(v));
+    v = f(v, dpp_ror<0x121>(v));
+    return f(f(read_lane(v, 0), read_lane(v, 16)), f(read_lane(v, 32), read_lane(v, 48)));
+}
+__device__ __forceinline__ double wave_max(double v)
+{
+    return wave_reduce(v, [](double a, double b) { return b > a ? b : a; });
+}
+__device__ __forceinline__ double wave_sum(double v)
+{
+    return wave_reduce(v, [](double a, double b) { return a + b; });
+}
+// the larger value, at equal ones the lower place; every lane gets the result
+__device__ __forceinline__ void wave_best(double &v, int &at)
+{
+#define ROUTE_BEST(OV, OA)                              \
+    {                                                   \
+        const double ov = OV;                           \
+        const int oa = OA;                              \
+        if (ov > v || (ov == v && oa < at)) {           \
+            v = ov;                                     \
+            at = oa;                                    \
+        }                                               \
+    }
+    ROUTE_BEST(dpp_ror<0x128>(v), dpp_ror<0x128>(at))
+    ROUTE_BEST(dpp_ror<0x124>(v), dpp_ror<0x124>(at))
+    ROUTE_BEST(dpp_ror<0x122>(v), dpp_ror<0x122>(at))
+    ROUTE_BEST(dpp_ror<0x121>(v), dpp_ror<0x121>(at))
+    const double wv = v;
+    const int wa = at;
+    v = read_lane(wv, 0);
+    at = __builtin_amdgcn_readlane(wa, 0);
+    ROUTE_BEST(read_lane(wv, 16), __builtin_amdgcn_readlane(wa, 16))
+    ROUTE_BEST(read_lane(wv, 32), __builtin_amdgcn_readlane(wa, 32))
+    ROUTE_BEST(read_lane(wv, 48), __builtin_amdgcn_readlane(wa, 48))
+#undef ROUTE_BEST
+}
+
 // One wave, one row, everything in float64: lane l holds the experts l, l + 64, ...
 // The order of the experts is what must not depend on rounding: two choices that differ by less than a float32
 // rounding are told apart here.  -inf as a key = not to be chosen.
@@ -88,19 +151,27 @@ __device__ void route_row(const RouteArgs &a, long row, int lane)
                     else if (key[i] > f2) f2 = key[i];
                 }
             }
-#pragma unroll
-            for (int m = 32; m > 0; m >>= 1) {
-                const double o1 = __shfl_xor(f1, m), o2 = __shfl_xor(f2, m);
+            const auto merge = [&](double o1, double o2) {
                 const double lo = f1 < o1 ? f1 : o1, two = f2 > o2 ? f2 : o2;
                 f1 = f1 > o1 ? f1 : o1;
                 f2 = lo > two ? lo : two;
-            }
+            };
+            merge(dpp_ror<0x128>(f1), dpp_ror<0x128>(f2));
+            merge(dpp_ror<0x124>(f1), dpp_ror<0x124>(f2));
+            merge(dpp_ror<0x122>(f1), dpp_ror<0x122>(f2));
+            merge(dpp_ror<0x121>(f1), dpp_ror<0x121>(f2));
+            const double w1 = f1, w2 = f2;
+            f1 = read_lane(w1, 0);
+            f2 = read_lane(w2, 0);
+            merge(read_lane(w1, 16), read_lane(w2, 16));
+            merge(read_lane(w1, 32), read_lane(w2, 32));
+            merge(read_lane(w1, 48), read_lane(w2, 48));
             const double s = (a.group_top == 1 || f2 == -inf) ? f1 : f1 + f2;
             if (lane == g) mine = s;
         }
         int ahead = 0;
         for (int g = 0; g < a.groups; ++g) {
-            const double s = __shfl(mine, g);
+            const double s = read_lane(mine, g);
             ahead += (s > mine || (s == mine && g < lane)) ? 1 : 0;
         }
         const unsigned long long stay = __ballot(lane < a.groups && ahead < a.group_k);
@@ -122,15 +193,7 @@ __device__ void route_row(const RouteArgs &a, long row, int lane)
                 best = key[i];
                 at = lane + 64 * i;
             }
-#pragma unroll
-        for (int m = 32; m > 0; m >>= 1) {
-            const double ob = __shfl_xor(best, m);
-            const int oa = __shfl_xor(at, m);
-            if (ob > best || (ob == best && oa < at)) {
-                best = ob;
-                at = oa;
-            }
-        }
+        wave_best(best, at);
         if (best == -inf) break;            // uniform: nothing is left for any further place
         if (lane == j) my_id = at;
 #pragma unroll
@@ -164,12 +227,6 @@ __global__ __launch_bounds__(256) void k_route_wide(RouteArgs a)
 }
 
 // reductions over the L = 16 or 64 lanes of a row; every lane gets the result
-template <int CTRL, typename V>
-__device__ __forceinline__ V dpp_ror(V v)
-{
-    const int i = __builtin_bit_cast(int, v);
-    return __builtin_bit_cast(V, __builtin_amdgcn_update_dpp(i, i, CTRL, 0xF, 0xF, false));
-}
 template <int L, typename V, typename F>
 __device__ __forceinline__ V row_reduce(V v, F f)
 {
@@ -209,19 +266,55 @@ __device__ __forceinline__ float order_value(unsigned k)
     return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k);
 }
 
+// v[0 .. N) in descending order (Batcher's odd-even merge sort)
+template <int N>
+__device__ __forceinline__ void sort_down(unsigned *v)
+{
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j <= N - 1 - k; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i)
+                    if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+                        const unsigned a = v[i + j], b = v[i + j + k];
+                        v[i + j] = a > b ? a : b;
+                        v[i + j + k] = a > b ? b : a;
+                    }
+}
+// the 8 largest of two descending runs of 8, descending, in a
+__device__ __forceinline__ void merge_down8(unsigned *a, const unsigned *b)
+{
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = a[i] > b[7 - i] ? a[i] : b[7 - i];       // rises and falls once
+#pragma unroll
+    for (int k = 4; k >= 1; k /= 2)
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (!(i & k)) {
+                const unsigned x = a[i], y = a[i + k];
+                a[i] = x > y ? x : y;
+                a[i + k] = x > y ? y : x;
+            }
+}
+
 // One row per L lanes (16: four rows a wave), lane l holds the experts l, l + L, ...: NV of them.
 //   A choice is a 32-bit key: the float32 number in an order-preserving form, its last log2(NV) bits replaced by the place
-//   in the lane (lower place = larger), so that one v_max keeps the expert with it.  The largest of the row comes from four
-//   DPP steps, the lowest lane that holds it from a ballot.
-//   The order itself is that of 64 bits.  Half-precision logits without a bias are exact in the key.  Otherwise the choice
-//   is only trusted where neighbours in it (the first not taken among them) are further apart than what float32
-//   arithmetic and the cut bits can have moved them; other rows -- a few in ten thousand for random logits, and those with
-//   NaN or infinities -- are done again by the whole wave in float64 (route_row).  Error of p: exp of a difference d <= 0 by
-//   exp2(d log2 e): (3 |d| + 2) 2^-24 of it, |d| exp(d) <= 0.37; the sum S of E terms: (NV + 6) additions and the terms'
-//   errors, in all (NV + 48) 2^-24 / S bounds it; 1 / (1 + exp(-x)): p (1 - p) |x| <= 0.23, 8 2^-24.  Error of c = p + bias:
-//   that and |c| 2^-24; of the key: |c| 2^-(23 - bits).
+//   in the lane (lower place = larger), so that one v_max keeps the expert with it.  A lane sorts its keys and keeps the 8
+//   largest; in each round the largest head of the row comes from four DPP steps, the lowest lane that holds it from a
+//   ballot, and that lane moves up.  A lane that has given all 8 leaves the row in doubt.
+//   The order itself is that of 64 bits.  Half-precision logits without a bias are exact in the key.  Otherwise the chosen
+//   ones are compared with their neighbours once more (logits as they are, 1 / (1 + exp(-x)) + bias in float64, softmax
+//   + bias in float32), and the choice is only trusted where they, and the last one and the first not taken, are further
+//   apart than what float32 arithmetic and (the latter) the cut bits can have moved them; other rows -- about one in a
+//   thousand for random logits, and those with NaN or infinities -- are done again by the whole wave in float64 (route_row).
+//   Error of p: exp of a difference d <= 0 by exp2(d log2 e): (3 |d| + 2) 2^-24 of it, |d| exp(d) <= 0.37; the sum S of E
+//   terms: (NV + 6) additions and the terms' errors, in all (NV + 48) 2^-24 / S bounds it; 1 / (1 + exp(-x)):
+//   p (1 - p) |x| <= 0.23 and an approximate reciprocal, 8 2^-24.  Error of c = p + bias: that and |c| 2^-24; of the key: |c| 2^-(23 - bits).
 template <typename T, int NV, int L>
-__global__ __launch_bounds__(256) void k_route(RouteArgs a)
+__global__ __launch_bounds__(256, NV <= 16 ? 4 : NV == 32 ? (L == 16 ? 3 : 2) : 1) void k_route(RouteArgs a)
 {
     constexpr int R = 64 / L, BITS = NV == 1 ? 0 : NV == 2 ? 1 : NV == 4 ? 2 : NV == 8 ? 3 : NV == 16 ? 4 : NV == 32 ? 5 : 6;
     constexpr bool HALF = sizeof(T) == 2;
@@ -237,55 +330,42 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a)
     float c[NV];
     bool bad = false;
     float top = -inf;
+    // an expert that is not to be chosen has c = -inf, here and below
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int e = l + L * i;
-        c[i] = e < a.E ? (float)x[e] + 0.f : -inf;      // -0 and 0 are the same number
-    }
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
+        const T v = e < a.E ? x[e] : (T)-inf;
+        c[i] = (float)v + 0.f;              // -0 and 0 are the same number
+        if (sizeof(T) == 8) bad |= c[i] == -inf && v != (T)-inf;        // masked is what is -inf in float64
         bad |= c[i] != c[i];
         top = fmaxf(top, c[i]);
     }
-    bool none[NV];
-#pragma unroll
-    for (int i = 0; i < NV; ++i) none[i] = c[i] == -inf;
     bad |= !a.sigmoid && top == inf;
-    // float64 logits below float32's range are -inf as float32 numbers and no masked ones
-    if (sizeof(T) == 8) {
-#pragma unroll
-        for (int i = 0; i < NV; ++i) bad |= l + L * i < a.E && none[i] && x[l + L * i] != (T)-inf;
-    }
     float total = 1.f, err = 0.f;
-    float p[NV];
-    const bool probabilities = a.bias || a.groups > 1 || (!a.renorm && !a.sigmoid);
-    if (probabilities) {
-        if (a.sigmoid) {
-            err = 8.f * 5.9604645e-8f;
+    if (!a.sigmoid && (a.bias || a.groups > 1 || !a.renorm)) {
+        top = row_max<L>(top);
+        total = 0.f;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) p[i] = 1.f / (1.f + __expf(-c[i]));
-        } else {
-            top = row_max<L>(top);
-            total = 0.f;
+        for (int i = 0; i < NV; ++i) total += c[i] == -inf ? 0.f : __expf(c[i] - top);
+        total = row_sum<L>(total);
+        err = (float)(NV + 48) * 5.9604645e-8f / total;
+    } else if (a.sigmoid) {
+        err = 8.f * 5.9604645e-8f;
+    }
+    if (a.bias || a.groups > 1) {           // c becomes the probability, with the bias
+        const float inv = 1.f / total;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                p[i] = none[i] ? 0.f : __expf(c[i] - top);
-                total += p[i];
-            }
-            total = row_sum<L>(total);
-            const float inv = 1.f / total;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) p[i] *= inv;
-            err = (float)(NV + 48) * 5.9604645e-8f * inv;
+        for (int i = 0; i < NV; ++i) {
+            const float p = a.sigmoid ? __builtin_amdgcn_rcpf(1.f + __expf(-c[i])) : __expf(c[i] - top) * inv;
+            c[i] = c[i] == -inf ? -inf : p;
         }
         if (a.bias) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
                 const int e = l + L * i;
                 const float b = e < a.E ? a.bias[e] : -inf;
-                p[i] += b;
-                none[i] |= b == -inf;
-                bad |= !none[i] && p[i] != p[i];
+                c[i] = c[i] == -inf ? -inf : c[i] + b;
+                bad |= c[i] != c[i];
             }
         }
     }
@@ -294,17 +374,12 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a)
         // the two largest c of a group in every lane of the row; lane g keeps those of group g
         const int per = a.E / a.groups;
         const unsigned inv = per > 1 ? (unsigned)(((1ull << 32) + per - 1) / per) : 0;
-        float s1 = -inf, s2 = -inf;
-        for (int g = 0; g < a.groups; ++g) {
-            float f1 = -inf, f2 = -inf;
-#pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int e = l + L * i;
-                const int ge = per > 1 ? (int)__umulhi((unsigned)e, inv) : e;
-                const float v = ge == g && !none[i] ? p[i] : -inf;
-                f2 = fmaxf(f2, fminf(f1, v));
-                f1 = fmaxf(f1, v);
-            }
+        float s1 = -inf, s2 = -inf, f1 = -inf, f2 = -inf;
+        const auto take = [&](float v) {
+            f2 = fmaxf(f2, fminf(f1, v));
+            f1 = fmaxf(f1, v);
+        };
+        const auto give = [&](int g) {      // over the lanes of the row; lane g keeps the result
 #define ROUTE_TOP2(CTRL)                                            \
     {                                                               \
         const float o1 = dpp_ror<CTRL>(f1), o2 = dpp_ror<CTRL>(f2); \
@@ -324,6 +399,28 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a)
             if (l == g) {
                 s1 = f1;
                 s2 = f2;
+            }
+            f1 = f2 = -inf;
+        };
+        if (per % L == 0) {                 // a group is per / L places of every lane
+            int left = per / L, g = 0;
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                take(c[i]);
+                if (--left == 0 && g < a.groups) {
+                    give(g++);
+                    left = per / L;
+                }
+            }
+        } else {
+            for (int g = 0; g < a.groups; ++g) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) {
+                    const int e = l + L * i;
+                    const int ge = per > 1 ? (int)__umulhi((unsigned)e, inv) : e;
+                    take(ge == g ? c[i] : -inf);
+                }
+                give(g);
             }
         }
         const bool pair = a.group_top == 2 && s2 != -inf;
@@ -348,41 +445,52 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a)
         for (int i = 0; i < NV; ++i) {
             const int e = l + L * i;
             const int ge = per > 1 ? (int)__umulhi((unsigned)e, inv) : e;
-            none[i] |= ge >= a.groups || !((stay >> (ge & 63)) & 1);
+            if (!a.bias) c[i] = e < a.E ? (float)x[e] + 0.f : -inf;     // the order goes by the logits
+            if (ge >= a.groups || !((stay >> (ge & 63)) & 1)) c[i] = -inf;
         }
     }
-    unsigned key[NV];
+    constexpr int DEEP = NV < 8 ? NV : 8;
+    unsigned key[NV < 8 ? 8 : NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-        key[i] = none[i] ? 0u : (order_bits(a.bias ? p[i] + 0.f : c[i]) & ~(unsigned)(NV - 1)) | (unsigned)(NV - 1 - i);
-    const bool exact = HALF && !a.bias;
-    for (int j = l; j < a.k; j += L) chosen[wave * R + sub][j] = -1;
-    __builtin_amdgcn_wave_barrier();
-    unsigned before = 0;
-    const int rounds = exact ? a.k : a.k + 1;
-    for (int j = 0; j < rounds; ++j) {
-        unsigned mine = key[0];
+        key[i] = c[i] == -inf ? 0u : (order_bits(c[i] + 0.f) & ~(unsigned)(NV - 1)) | (unsigned)(NV - 1 - i);
+    sort_down<DEEP>(key);
 #pragma unroll
-        for (int i = 1; i < NV; ++i) mine = key[i] > mine ? key[i] : mine;
-        const unsigned best = row_max<L>(mine);
-        const unsigned long long who = __ballot(mine == best);
+    for (int i = 8; i < NV; i += 8) {
+        sort_down<8>(key + i);
+        merge_down8(key, key + i);
+    }
+    const bool exact = HALF && !a.bias;
+    int32_t *mine = chosen[wave * R + sub];
+    for (int j = l; j < a.k; j += L) mine[j] = -1;
+    __builtin_amdgcn_wave_barrier();
+    unsigned last = 0;
+    int given = 0;
+    for (int j = 0; j < a.k; ++j) {
+        const unsigned best = row_max<L>(key[0]);
+        const unsigned long long who = __ballot(key[0] == best);
         const int first = L == 64 ? __ffsll((long long)who) - 1 : __ffs((int)((who >> (sub * L)) & 0xFFFFu)) - 1;
-        if (!exact && j > 0 && best != 0) {
+        last = best;
+        if (l == first && best != 0) {
+            mine[j] = l + L * (NV - 1 - (int)(best & (unsigned)(NV - 1)));
+            ++given;
+#pragma unroll
+            for (int i = 0; i + 1 < DEEP; ++i) key[i] = key[i + 1];
+            key[DEEP - 1] = 0;
+        }
+    }
+    if (NV > DEEP) doubt |= given == DEEP;
+    if (!exact) {                           // the last one taken and the first one that was not
+        const unsigned next = row_max<L>(key[0]);
+        const unsigned m = ~(unsigned)(NV - 1);
+        if (next != 0) {
             if (a.bias) {
-                const float f = order_value(before & ~(unsigned)(NV - 1)), g = order_value(best & ~(unsigned)(NV - 1));
+                const float f = order_value(last & m), g = order_value(next & m);
                 doubt |= f - g <= 2.f * err + fmaxf(fabsf(f), fabsf(g)) * (1.1920929e-7f * (float)(1 + 2 * NV));
             } else {
-                doubt |= ((before ^ best) & ~(unsigned)(NV - 1)) == 0;
+                doubt |= ((last ^ next) & m) == 0;
             }
         }
-        before = best;
-        if (l == first && best != 0) {
-            const int i = NV - 1 - (int)(best & (unsigned)(NV - 1));
-            if (j < a.k) chosen[wave * R + sub][j] = l + L * i;
-        }
-        const unsigned gone = l == first ? best : 0u;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) key[i] = key[i] == gone ? 0u : key[i];
     }
     __builtin_amdgcn_wave_barrier();
     // weights: lane l has the places l, l + L, ...
@@ -394,13 +502,13 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a)
 #pragma unroll
         for (int q = 0; q < PL; ++q) {
             const int j = l + q * L;
-            id[q] = j < a.k ? chosen[wave * R + sub][j] : -1;
+            id[q] = j < a.k ? mine[j] : -1;
             xs[q] = id[q] >= 0 ? x[id[q]] : (T)-inf;
             if (sizeof(T) < 8) M = fmaxf(M, (float)xs[q]);
         }
         float sum = 0.f;
         if (sizeof(T) == 8) {               // without a bias: the first choice is the largest
-            const int lead = chosen[wave * R + sub][0];
+            const int lead = mine[0];
             double Md = lead >= 0 ? (double)x[lead] : 0.0;
             if (a.sigmoid && Md > 0.0) Md = 0.0;
 #pragma unroll
@@ -428,9 +536,29 @@ __global__ __launch_bounds__(256) void k_route(RouteArgs a)
 #pragma unroll
         for (int q = 0; q < PL; ++q) {
             const int j = l + q * L;
-            id[q] = j < a.k ? chosen[wave * R + sub][j] : -1;
+            id[q] = j < a.k ? mine[j] : -1;
             const float xs = id[q] >= 0 ? (float)x[id[q]] : -inf;
             t[q] = id[q] < 0 ? 0.f : a.scale * (a.sigmoid ? 1.f / (1.f + expf(-xs)) : expf(xs - top) / total);
+        }
+    }
+    if (!exact) {                           // neighbours in the choice
+#pragma unroll
+        for (int q = 0; q < PL; ++q) {
+            const int j = l + q * L;
+            const int i0 = id[q], i1 = j + 1 < a.k ? mine[j + 1] : -1;
+            if (i0 < 0 || i1 < 0) continue;
+            const T x0 = x[i0], x1 = x[i1];
+            if (!a.bias) {
+                doubt |= !(x0 > x1 || (x0 == x1 && i0 < i1));
+            } else if (a.sigmoid) {
+                const double c0 = 1.0 / (1.0 + exp(-(double)x0)) + (double)a.bias[i0];
+                const double c1 = 1.0 / (1.0 + exp(-(double)x1)) + (double)a.bias[i1];
+                doubt |= !(c0 > c1 || (c0 == c1 && i0 < i1));
+            } else {
+                const float inv = 1.f / total;
+                const float c0 = __expf((float)x0 - top) * inv + a.bias[i0], c1 = __expf((float)x1 - top) * inv + a.bias[i1];
+                doubt |= !(c0 - c1 > 2.f * err + 2.3841858e-7f * fmaxf(fabsf(c0), fabsf(c1)));
+            }
         }
     }
     const unsigned long long again = __ballot(bad || doubt);
@@ -540,9 +668,9 @@ static void route_go_wide(const RouteArgs &a, hipStream_t st)
 template <typename T>
 static void route_launch(const RouteArgs &a, hipStream_t st)
 {
-    // 16 lanes a row up to 256 experts (16 of them a lane), the whole wave above.
+    // 16 lanes a row up to 512 experts (32 of them a lane), the whole wave above.
     // In float64 throughout: probabilities of float64 logits; more groups than a row has lanes.
-    const bool wide = (sizeof(T) == 8 && (a.bias || a.groups > 1 || (!a.renorm && !a.sigmoid))) || a.groups > (a.E <= 256 ? 16 : 64);
+    const bool wide = (sizeof(T) == 8 && (a.bias || a.groups > 1 || (!a.renorm && !a.sigmoid))) || a.groups > (a.E <= 512 ? 16 : 64);
     if (wide) {
         if (a.E <= 64) route_go_wide<T, 1>(a, st);
         else if (a.E <= 256) route_go_wide<T, 4>(a, st);
@@ -555,7 +683,7 @@ static void route_launch(const RouteArgs &a, hipStream_t st)
     else if (a.E <= 64) route_go<T, 4, 16>(a, st);
     else if (a.E <= 128) route_go<T, 8, 16>(a, st);
     else if (a.E <= 256) route_go<T, 16, 16>(a, st);
-    else if (a.E <= 512) route_go<T, 8, 64>(a, st);
+    else if (a.E <= 512) route_go<T, 32, 16>(a, st);
     else if (a.E <= 1024) route_go<T, 16, 64>(a, st);
     else if (a.E <= 2048) route_go<T, 32, 64>(a, st);
     else route_go<T, 64, 64>(a, st);
