@@ -305,11 +305,12 @@ __device__ __forceinline__ void merge_down8(unsigned *a, const unsigned *b)
 //   in the lane (lower place = larger), so that one v_max keeps the expert with it.  A lane sorts its keys and keeps the 8
 //   largest; in each round the largest head of the row comes from four DPP steps, the lowest lane that holds it from a
 //   ballot, and that lane moves up.  A lane that has given all 8 leaves the row in doubt.
-//   The order itself is that of 64 bits.  Half-precision logits without a bias are exact in the key.  Otherwise the chosen
-//   ones are compared with their neighbours once more (logits as they are, 1 / (1 + exp(-x)) + bias in float64, softmax
-//   + bias in float32), and the choice is only trusted where they, and the last one and the first not taken, are further
-//   apart than what float32 arithmetic and (the latter) the cut bits can have moved them; other rows -- about one in a
-//   thousand for random logits, and those with NaN or infinities -- are done again by the whole wave in float64 (route_row).
+//   The order itself is that of 64 bits.  Half-precision logits without a bias are exact in the key.  Otherwise one more
+//   than k is taken, neighbours are compared without the cut bits, and where two are not further apart than what float32
+//   arithmetic and (the last one taken and the first that was not) the cut bits can have moved them, the row's choices are
+//   ranked again by their float64 values -- for random logits about one row in a thousand.  Only where the one after that
+//   is as near, and for NaN and infinities, the whole wave does the row again in float64 (route_row): that costs 6 us at
+//   least, for one row.
 //   Error of p: exp of a difference d <= 0 by exp2(d log2 e): (3 |d| + 2) 2^-24 of it, |d| exp(d) <= 0.37; the sum S of E
 //   terms: (NV + 6) additions and the terms' errors, in all (NV + 48) 2^-24 / S bounds it; 1 / (1 + exp(-x)):
 //   p (1 - p) |x| <= 0.23 and an approximate reciprocal, 8 2^-24.  Error of c = p + bias: that and |c| 2^-24; of the key: |c| 2^-(23 - bits).
@@ -320,7 +321,8 @@ __global__ __launch_bounds__(256, NV <= 16 ? 4 : NV == 32 ? (L == 16 ? 3 : 2) : 
     constexpr bool HALF = sizeof(T) == 2;
     constexpr int PL = (ROUTE_MAX_K + L - 1) / L;       // places of a lane
     constexpr int NV64 = (NV * L + 63) / 64;
-    __shared__ int32_t chosen[4 * R][ROUTE_MAX_K];
+    __shared__ int32_t chosen[4 * R][ROUTE_MAX_K + 2], ranked[4 * R][ROUTE_MAX_K];
+    __shared__ double value[4 * R][ROUTE_MAX_K + 2];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, l = lane % L, sub = lane / L;
     const long row0 = ((long)blockIdx.x * 4 + wave) * R;
     if (row0 >= a.T) return;                            // whole waves
@@ -438,7 +440,7 @@ __global__ __launch_bounds__(256, NV <= 16 ? 4 : NV == 32 ? (L == 16 ? 3 : 2) : 
         for (int g = 0; g < a.groups; ++g) {
             const float o = __shfl(score, sub * L + g);
             const bool ok = (all >> (sub * L + g)) & 1;
-            if (l < a.groups && ok != kept && (score != -inf || o != -inf)) doubt |= fabsf(score - o) <= near;
+            if (l < a.groups && ok != kept && (score != -inf || o != -inf)) bad |= fabsf(score - o) <= near;
         }
         const unsigned long long stay = L == 64 ? all : (all >> (sub * L)) & 0xFFFFull;
 #pragma unroll
@@ -462,15 +464,17 @@ __global__ __launch_bounds__(256, NV <= 16 ? 4 : NV == 32 ? (L == 16 ? 3 : 2) : 
     }
     const bool exact = HALF && !a.bias;
     int32_t *mine = chosen[wave * R + sub];
-    for (int j = l; j < a.k; j += L) mine[j] = -1;
+    const int take_n = exact ? a.k : a.k + 1;
+    for (int j = l; j < take_n + 1; j += L) mine[j] = -1;
     __builtin_amdgcn_wave_barrier();
-    unsigned last = 0;
+    unsigned last = 0, after = 0;           // keys of place k - 1 and k
     int given = 0;
-    for (int j = 0; j < a.k; ++j) {
+    for (int j = 0; j < take_n; ++j) {
         const unsigned best = row_max<L>(key[0]);
         const unsigned long long who = __ballot(key[0] == best);
         const int first = L == 64 ? __ffsll((long long)who) - 1 : __ffs((int)((who >> (sub * L)) & 0xFFFFu)) - 1;
-        last = best;
+        last = j == a.k ? last : best;
+        after = best;
         if (l == first && best != 0) {
             mine[j] = l + L * (NV - 1 - (int)(best & (unsigned)(NV - 1)));
             ++given;
@@ -479,20 +483,82 @@ __global__ __launch_bounds__(256, NV <= 16 ? 4 : NV == 32 ? (L == 16 ? 3 : 2) : 
             key[DEEP - 1] = 0;
         }
     }
-    if (NV > DEEP) doubt |= given == DEEP;
-    if (!exact) {                           // the last one taken and the first one that was not
-        const unsigned next = row_max<L>(key[0]);
+    bad |= NV > DEEP && given == DEEP;
+    __builtin_amdgcn_wave_barrier();
+    if (!exact) {
         const unsigned m = ~(unsigned)(NV - 1);
-        if (next != 0) {
-            if (a.bias) {
-                const float f = order_value(last & m), g = order_value(next & m);
-                doubt |= f - g <= 2.f * err + fmaxf(fabsf(f), fabsf(g)) * (1.1920929e-7f * (float)(1 + 2 * NV));
-            } else {
-                doubt |= ((last ^ next) & m) == 0;
+        // whether a choice b may belong in front of a
+        const auto close = [&](unsigned ka, unsigned kb) {
+            if (kb == 0) return false;
+            if (!a.bias) return ((ka ^ kb) & m) == 0;
+            const float f = order_value(ka & m), g = order_value(kb & m);
+            return f - g <= 2.f * err + fmaxf(fabsf(f), fabsf(g)) * (1.1920929e-7f * (float)(1 + 2 * NV));
+        };
+        bad |= close(last, row_max<L>(key[0]));
+        doubt |= close(last, after);
+        double *val = value[wave * R + sub];
+        const float inv = 1.f / total;
+        for (int j = l; j < a.k; j += L) {
+            const int i = mine[j];
+            if (i < 0) continue;
+            const T v = x[i];
+            float f = (float)v;
+            if (a.bias) f = (a.sigmoid ? __builtin_amdgcn_rcpf(1.f + __expf(-f)) : __expf(f - top) * inv) + a.bias[i];
+            val[j] = a.bias ? (double)f : (double)v;
+        }
+        __builtin_amdgcn_wave_barrier();
+        for (int j = l; j + 1 < a.k; j += L) {
+            const int i0 = mine[j], i1 = mine[j + 1];
+            if (i1 < 0) continue;
+            const double v0 = val[j], v1 = val[j + 1];
+            if (a.bias) doubt |= !((float)(v0 - v1) > 2.f * err + 2.3841858e-7f * fmaxf(fabsf((float)v0), fabsf((float)v1)));
+            else doubt |= !(v0 > v1 || (v0 == v1 && i0 < i1));
+        }
+        const unsigned long long rows = __ballot(doubt);
+        if (rows) {                         // uniform
+            double total64 = 1.0, top64 = 0.0;
+            if (a.bias && !a.sigmoid) {
+                top64 = (double)top;
+                double t = 0.0;
+#pragma unroll 4
+                for (int e = l; e < a.E; e += L) t += exp((double)x[e] - top64);
+                t = t + dpp_ror<0x128>(t);
+                t = t + dpp_ror<0x124>(t);
+                t = t + dpp_ror<0x122>(t);
+                t = t + dpp_ror<0x121>(t);
+                if (L == 64) t = (read_lane(t, 0) + read_lane(t, 16)) + (read_lane(t, 32) + read_lane(t, 48));
+                total64 = t;
             }
+            if (a.bias) {
+                for (int j = l; j < take_n; j += L) {
+                    const int i = mine[j];
+                    if (i < 0) continue;
+                    const double v = (double)x[i];
+                    val[j] = (a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - top64) / total64) + (double)a.bias[i];
+                }
+            } else if (l == a.k % L && mine[a.k] >= 0) {
+                val[a.k] = (double)x[mine[a.k]];
+            }
+            int32_t *to = ranked[wave * R + sub];
+            for (int j = l; j < a.k; j += L) to[j] = -1;
+            __builtin_amdgcn_wave_barrier();
+            for (int j = l; j < take_n; j += L) {
+                const int i = mine[j];
+                if (i < 0) continue;
+                const double v = val[j];
+                int rank = 0;
+                for (int o = 0; o < take_n; ++o) {
+                    const int io = mine[o];
+                    rank += io >= 0 && (val[o] > v || (val[o] == v && io < i)) ? 1 : 0;
+                }
+                if (rank < a.k) to[rank] = i;
+            }
+            __builtin_amdgcn_wave_barrier();
+            // a row without doubt has the same order
+            for (int j = l; j < a.k; j += L) mine[j] = to[j];
+            __builtin_amdgcn_wave_barrier();
         }
     }
-    __builtin_amdgcn_wave_barrier();
     // weights: lane l has the places l, l + L, ...
     int id[PL];
     float t[PL];
@@ -541,27 +607,7 @@ __global__ __launch_bounds__(256, NV <= 16 ? 4 : NV == 32 ? (L == 16 ? 3 : 2) : 
             t[q] = id[q] < 0 ? 0.f : a.scale * (a.sigmoid ? 1.f / (1.f + expf(-xs)) : expf(xs - top) / total);
         }
     }
-    if (!exact) {                           // neighbours in the choice
-#pragma unroll
-        for (int q = 0; q < PL; ++q) {
-            const int j = l + q * L;
-            const int i0 = id[q], i1 = j + 1 < a.k ? mine[j + 1] : -1;
-            if (i0 < 0 || i1 < 0) continue;
-            const T x0 = x[i0], x1 = x[i1];
-            if (!a.bias) {
-                doubt |= !(x0 > x1 || (x0 == x1 && i0 < i1));
-            } else if (a.sigmoid) {
-                const double c0 = 1.0 / (1.0 + exp(-(double)x0)) + (double)a.bias[i0];
-                const double c1 = 1.0 / (1.0 + exp(-(double)x1)) + (double)a.bias[i1];
-                doubt |= !(c0 > c1 || (c0 == c1 && i0 < i1));
-            } else {
-                const float inv = 1.f / total;
-                const float c0 = __expf((float)x0 - top) * inv + a.bias[i0], c1 = __expf((float)x1 - top) * inv + a.bias[i1];
-                doubt |= !(c0 - c1 > 2.f * err + 2.3841858e-7f * fmaxf(fabsf(c0), fabsf(c1)));
-            }
-        }
-    }
-    const unsigned long long again = __ballot(bad || doubt);
+    const unsigned long long again = __ballot(bad);
     const unsigned long long rowmask = (L == 64 ? ~0ull : 0xFFFFull << (sub * L));
     if (row0 + sub < a.T && !(again & rowmask)) {
 #pragma unroll
@@ -574,7 +620,7 @@ __global__ __launch_bounds__(256, NV <= 16 ? 4 : NV == 32 ? (L == 16 ? 3 : 2) : 
         }
     }
     if (!again) return;
-    for (int s = 0; s < R; ++s)             // the rows in doubt, one after the other
+    for (int s = 0; s < R; ++s)             // one after the other
         if (row0 + s < a.T && (again & (L == 64 ? ~0ull : 0xFFFFull << (s * L)))) route_row<T, NV64>(a, row0 + s, lane);
 }
 
