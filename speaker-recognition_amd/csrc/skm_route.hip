@@ -690,12 +690,149 @@ __global__ __launch_bounds__(256) void k_route_backward(RouteBackArgs a)
         A v = 0;
         if (D != (A)0 && e < a.E) v = -D * exp((A)x[e] - top) / total;
         for (int j = 0; j < a.k; ++j) {                 // in the order of the places: the same bits every time
-            const int at = __shfl(id, j);
-            const A dj = __shfl(d, j);
+            const int at = __builtin_amdgcn_readlane(id, j);
+            const A dj = (A)read_lane((double)d, j);
             if (at == e) v += dj;
         }
         if (e < a.E) dx[e] = (T)v;
     }
+}
+
+// The same for rows of up to EMAX experts: 16 lanes a row, four rows a wave.  What the chosen places add goes through a
+// row in LDS (places with the same expert are added first, in their order, by the first of them), so that the row leaves
+// in 16-byte stores; a wave per row with a comparison per place and element took twice as long.
+template <typename T, int EMAX>
+__global__ __launch_bounds__(256) void k_route_backward16(RouteBackArgs a, int vec)
+{
+    constexpr int PL = ROUTE_MAX_K / 16, V = 16 / sizeof(T);
+    __shared__ float buf[16][EMAX + 4];
+    __shared__ int32_t sid[16][ROUTE_MAX_K];
+    __shared__ float sd[16][ROUTE_MAX_K];
+    const int lane = threadIdx.x & 63, l = lane & 15, slot = threadIdx.x >> 4;
+    const long row0 = (long)blockIdx.x * 16 + slot;
+    if ((long)blockIdx.x * 16 + (threadIdx.x >> 6) * 4 >= a.T) return;      // whole waves
+    const bool live = row0 < a.T;
+    const long row = live ? row0 : a.T - 1;
+    const T *x = static_cast<const T *>(a.x) + row * a.ldx;
+    T *dx = static_cast<T *>(a.dx) + row * a.E;
+    const float inf = __builtin_inff();
+    int id[PL];
+    float xs[PL], g[PL], d[PL], top = -inf;
+#pragma unroll
+    for (int q = 0; q < PL; ++q) {
+        const int j = l + 16 * q;
+        id[q] = -1;
+        xs[q] = -inf;
+        g[q] = d[q] = 0.f;
+        if (j < a.k) {
+            const int i = a.ids[row * a.k + j];
+            if (i >= 0 && i < a.E) {
+                xs[q] = (float)x[i];
+                if (xs[q] != -inf) {
+                    id[q] = i;
+                    g[q] = a.g[row * a.k + j];
+                }
+            }
+        }
+        top = fmaxf(top, xs[q]);
+    }
+    float D = 0.f, total = 1.f;
+    if (a.renorm) {
+        float M = row_max<16>(top);
+        if (a.sigmoid && M > 0.f) M = 0.f;
+        float sum = 0.f, t[PL];
+#pragma unroll
+        for (int q = 0; q < PL; ++q) {
+            t[q] = id[q] >= 0 ? route_share(xs[q], M, a.sigmoid) : 0.f;
+            sum += t[q];
+        }
+        sum = row_sum<16>(sum);
+        float G = 0.f;
+#pragma unroll
+        for (int q = 0; q < PL; ++q) {
+            t[q] = sum > 0.f ? t[q] / sum : t[q];
+            G += t[q] * g[q];
+        }
+        G = row_sum<16>(G);
+#pragma unroll
+        for (int q = 0; q < PL; ++q) {
+            d[q] = id[q] >= 0 ? a.scale * t[q] * (g[q] - G) : 0.f;
+            if (a.sigmoid && id[q] >= 0) d[q] *= 1.f / (1.f + expf(xs[q]));
+        }
+    } else if (a.sigmoid) {
+#pragma unroll
+        for (int q = 0; q < PL; ++q)
+            if (id[q] >= 0) d[q] = a.scale * g[q] / (1.f + expf(-xs[q])) / (1.f + expf(xs[q]));
+    } else {
+        top = -inf;
+        for (int e = l; e < a.E; e += 16) top = fmaxf(top, (float)x[e]);
+        top = row_max<16>(top);
+        if (top == -inf) top = 0.f;
+        total = 0.f;
+        for (int e = l; e < a.E; e += 16) total += expf((float)x[e] - top);
+        total = row_sum<16>(total);
+#pragma unroll
+        for (int q = 0; q < PL; ++q) {
+            if (id[q] >= 0) d[q] = a.scale * g[q] * expf(xs[q] - top) / total;
+            D += d[q];
+        }
+        D = row_sum<16>(D);
+    }
+#pragma unroll
+    for (int q = 0; q < PL; ++q) {
+        const int j = l + 16 * q;
+        if (j < a.k) {
+            sid[slot][j] = id[q];
+            sd[slot][j] = d[q];
+        }
+    }
+    for (int e = l * 4; e < a.E; e += 64) *reinterpret_cast<float4 *>(&buf[slot][e]) = make_float4(0.f, 0.f, 0.f, 0.f);
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int q = 0; q < PL; ++q) {
+        if (16 * q >= a.k) break;
+        float sum = 0.f;
+        bool first = true;
+        for (int o = 0; o < a.k; ++o) {
+            const bool same = sid[slot][o] == id[q];
+            sum += same ? sd[slot][o] : 0.f;
+            first &= !(same && o < l + 16 * q);
+        }
+        if (id[q] >= 0 && first) buf[slot][id[q]] = sum;
+    }
+    __builtin_amdgcn_wave_barrier();
+    if (!live) return;
+    typedef T vt __attribute__((ext_vector_type(V)));
+    for (int e = l * V; e < a.E; e += 16 * V) {
+        float v[V];
+#pragma unroll
+        for (int q = 0; q < V; ++q) v[q] = e + q < a.E ? buf[slot][e + q] : 0.f;
+        if (D != 0.f) {
+#pragma unroll
+            for (int q = 0; q < V; ++q)
+                if (e + q < a.E) v[q] -= D * expf((float)x[e + q] - top) / total;
+        }
+        if (vec) {
+            vt o;
+#pragma unroll
+            for (int q = 0; q < V; ++q) o[q] = (T)v[q];
+            *reinterpret_cast<vt *>(dx + e) = o;
+        } else {
+#pragma unroll
+            for (int q = 0; q < V; ++q)
+                if (e + q < a.E) dx[e + q] = (T)v[q];
+        }
+    }
+}
+
+template <typename T>
+static void route_back_go(const RouteBackArgs &a, hipStream_t st)
+{
+    const bool vec = ((uintptr_t)a.dx & 15) == 0 && (a.E * sizeof(T)) % 16 == 0;
+    const dim3 grid((unsigned)((a.T + 15) / 16)), block(256);
+    if (a.E <= 128) hipLaunchKernelGGL((k_route_backward16<T, 128>), grid, block, 0, st, a, (int)vec);
+    else if (a.E <= 512) hipLaunchKernelGGL((k_route_backward16<T, 512>), grid, block, 0, st, a, (int)vec);
+    else hipLaunchKernelGGL((k_route_backward<T, float>), dim3((unsigned)((a.T + 3) / 4)), block, 0, st, a);
 }
 
 template <typename T, int NV, int L>
@@ -787,12 +924,11 @@ extern "C" int skm_route_backward(void *ctx_, const void *x, int dtype, long T, 
     hipStream_t st = (hipStream_t)stream;
     SkmProfScope ps(ctx, "k_route_backward", st);
     const RouteBackArgs a{x, T, ldx, E, k, ids, dweights, scores == SKM_ROUTE_SIGMOID, renorm != 0, scale, dx};
-    const dim3 grid((unsigned)((T + 3) / 4)), block(256);
     switch (dtype) {
-    case SKM_DT_F32: hipLaunchKernelGGL((k_route_backward<float, float>), grid, block, 0, st, a); break;
-    case SKM_DT_BF16: hipLaunchKernelGGL((k_route_backward<bf16_t, float>), grid, block, 0, st, a); break;
-    case SKM_DT_F16: hipLaunchKernelGGL((k_route_backward<f16_t, float>), grid, block, 0, st, a); break;
-    default: hipLaunchKernelGGL((k_route_backward<double, double>), grid, block, 0, st, a); break;
+    case SKM_DT_F32: route_back_go<float>(a, st); break;
+    case SKM_DT_BF16: route_back_go<bf16_t>(a, st); break;
+    case SKM_DT_F16: route_back_go<f16_t>(a, st); break;
+    default: hipLaunchKernelGGL((k_route_backward<double, double>), dim3((unsigned)((T + 3) / 4)), dim3(256), 0, st, a); break;
     }
     SKM_HIP(hipGetLastError());
     return SKM_OK;
