@@ -475,12 +475,12 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
         ob[i] = (unsigned)cc * (unsigned)g.ldb + FP8_PIECE(i);
     }
 #undef FP8_PIECE
-    // scales: 64 rows a load, the rows of A, then the columns of B; waves take turns
+    // scales: 64 rows a load, the rows of A, then the columns of B; waves take turns (one too many repeats the last)
     constexpr int CHUNKS = (BM + BN) / 64, MINE = (CHUNKS + 3) / 4;
     unsigned os[MINE];
 #pragma unroll
     for (int i = 0; i < MINE; ++i) {
-        int rr = (wave + 4 * i) * 64 + lane;
+        int rr = (wave + 4 * i < CHUNKS ? wave + 4 * i : CHUNKS - 1) * 64 + lane;
         if (rr < BM) {
             rr = rr < rows ? rr : rows - 1;
             if (by_pair) rr = g.pair[row0 + rr] / g.slots;
@@ -501,12 +501,11 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
     }
 #define FP8_ISSUE(S, BUF)                                                                                              \
     _Pragma("unroll") for (int l_ = 0; l_ < LOADS; ++l_) FP8_ISSUE1(S, l_, BUF)
-#define FP8_SCALES(G, BUF)                                                                                                \
+#define FP8_SCALES(G, BUF)                                                                                             \
     _Pragma("unroll") for (int i = 0; i < MINE; ++i) {                                                                 \
-        const int c = wave + 4 * i;                                                                                    \
+        const int c = wave + 4 * i < CHUNKS ? wave + 4 * i : CHUNKS - 1;                                               \
         const uint8_t *l = (c * 64 < BM ? bsa : bsb) + (long)(G) * 4;                                                  \
-        if (CHUNKS % 4 == 0 || c < CHUNKS)                                                                             \
-            __builtin_amdgcn_global_load_lds((glb_ptr)(l + os[i]), (lds_ptr)((BUF) + c * 256), 4, 0, 0);                \
+        __builtin_amdgcn_global_load_lds((glb_ptr)(l + os[i]), (lds_ptr)((BUF) + c * 256), 4, 0, 0);                   \
     }
 
     f32x16 acc[MT][NT];
@@ -545,25 +544,32 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
     }
 #define FP8_TILE(H, I, J)                                                                                              \
     acc[I][J] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[H][J], fa[H][I], acc[I][J], FB, FA, 0, sb[J], 0, sa[I]);
-    // rows I0 .. I1 - 1 of the wave's tiles times half H
-    bf16x8 xb[NT][4];
-#define FP8_CONVERT_B(H)                                                                                               \
-    if (sizeof(TO) == 4) {                                                                                             \
-        _Pragma("unroll") for (int j = 0; j < NT; ++j) _Pragma("unroll") for (int t = 0; t < 4; ++t)                   \
-            xb[j][t] = fp8_to_bf16<FB>(fb[H][j][2 * t], fb[H][j][2 * t + 1], fp8_pow2(sb[j] - 127));                   \
-    }
-#define FP8_MULTIPLY(H, I0, I1)                                                                                        \
-    _Pragma("unroll") for (int i = I0; i < I1; ++i) {                                                                  \
-        if (sizeof(TO) == 4) {                                                                                         \
-            _Pragma("unroll") for (int t = 0; t < 4; ++t) {                                                            \
-                const bf16x8 xa = fp8_to_bf16<FA>(fa[H][i][2 * t], fa[H][i][2 * t + 1], fp8_pow2(sa[i] - 127));        \
-                _Pragma("unroll") for (int j = 0; j < NT; ++j)                                                         \
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(xb[j][t], xa, acc[i][j], 0, 0, 0);             \
+    // Float32 results, a half in U units: unit u multiplies eight k of every lane of row u / 4 of the wave's tiles with its
+    // NT columns and converts for later: the next unit's row, and in the second half of the units the columns of the next
+    // half.  So the conversions (one instruction per two numbers) stand beside multiplications that do not need them.
+    constexpr int U = MT * 4;
+    bf16x8 xa[2], xb[2][NT][4];
+#define FP8_SCALE(S) __uint_as_float((unsigned)(S) << 23)
+#define FP8_XA(V, T, S) fp8_to_bf16<FA>((V)[2 * (T)], (V)[2 * (T) + 1], FP8_SCALE(S))
+#define FP8_XB(V, T, S) fp8_to_bf16<FB>((V)[2 * (T)], (V)[2 * (T) + 1], FP8_SCALE(S))
+#define FP8_UNIT(H, Q, SNA, SNB)                                                                                       \
+    {                                                                                                                  \
+        _Pragma("unroll") for (int j_ = 0; j_ < NT; ++j_) acc[(Q) / 4][j_] =                                           \
+            __builtin_amdgcn_mfma_f32_32x32x16_bf16(xb[H][j_][(Q) & 3], xa[(Q) & 1], acc[(Q) / 4][j_], 0, 0, 0);       \
+        if ((Q) + 1 < U) xa[((Q) + 1) & 1] = FP8_XA(fa[H][((Q) + 1) / 4 < MT ? ((Q) + 1) / 4 : 0], ((Q) + 1) & 3, sa[((Q) + 1) / 4 < MT ? ((Q) + 1) / 4 : 0]); \
+        else xa[((Q) + 1) & 1] = FP8_XA(fa[(H) ^ 1][0], 0, SNA[0]);                                                    \
+        constexpr int EACH_ = NT * 8 / U;                                                                              \
+        if ((Q) >= U / 2) {                                                                                            \
+            _Pragma("unroll") for (int c_ = 0; c_ < EACH_; ++c_) {                                                     \
+                const int n_ = ((Q) - U / 2) * EACH_ + c_;                                                             \
+                xb[(H) ^ 1][n_ / 4 < NT ? n_ / 4 : 0][n_ & 3] =                                                        \
+                    FP8_XB(fb[(H) ^ 1][n_ / 4 < NT ? n_ / 4 : 0], n_ & 3, SNB[n_ / 4 < NT ? n_ / 4 : 0]);              \
+                asm volatile("" : "+v"(xb[(H) ^ 1][n_ / 4 < NT ? n_ / 4 : 0][n_ & 3]));         /* not later */        \
             }                                                                                                          \
-        } else {                                                                                                       \
-            _Pragma("unroll") for (int j = 0; j < NT; ++j) FP8_TILE(H, i, j)                                           \
         }                                                                                                              \
     }
+    // the columns first
+#define FP8_READ1B(H, F, BUF) FP8_READ1(H, ((F) < NT ? MT + (F) : (F) - NT), BUF)
 #define FP8_STAGE(S) (sh + ((S) & 1) * STAGE)
 #define FP8_SCALE_GROUP(KB) (sh + 2 * STAGE + (((KB) >> 2) & 1) * GROUP)
     const int n = kb1 - kb0;
@@ -585,6 +591,13 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
         for (int i = 0; i < MT; ++i) sa[i] = na[i];
 #pragma unroll
         for (int j = 0; j < NT; ++j) sb[j] = nb[j];
+        if (sizeof(TO) == 4) {
+            xa[0] = FP8_XA(fa[0][0], 0, sa[0]);
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int t = 0; t < 4; ++t) xb[0][j][t] = FP8_XB(fb[0][j], t, sb[j]);
+        }
     }
     // Behind the barrier of a stage: the loads of stage s2 fill the buffer that it frees while the next stage is read.  The
     // two buffers (and the two groups of scales, or the same group with the same bytes) do not overlap: restrict lets the
@@ -593,12 +606,23 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
                     uint8_t *__restrict__ fill_scales, const uint8_t *__restrict__ next_scales) __attribute__((always_inline)) {
         FP8_SCALES((kb0 + s2) >> 2, fill_scales)
         if (sizeof(TO) == 4) {
-            FP8_ISSUE(s2, fill)
-            FP8_MULTIPLY(0, MT - 1, MT)
-            FP8_READ(0, next)
             FP8_READ_SCALES(kb + 1, next_scales)
-            FP8_CONVERT_B(1)
-            FP8_MULTIPLY(1, 0, MT)
+            constexpr int POST = 4 + U, EACH = (LOADS + POST - 1) / POST;
+#pragma unroll
+            for (int u = 0; u < POST; ++u) {
+                if (u < 4) {
+                    FP8_UNIT(0, U - 4 + u, sa, sb)
+                } else {
+                    FP8_UNIT(1, u - 4, na, nb)
+                }
+#pragma unroll
+                for (int l = u * EACH; l < (u + 1) * EACH; ++l)
+                    if (l < LOADS) FP8_ISSUE1(s2, l, fill)
+                if (u >= 4 && u < 4 + MT + NT) {
+                    FP8_READ1B(0, u - 4, next)
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
         } else {
             // In this order: the four waves' loads take 16 cycles each on the way to the cache, a wave that waits to issue
             // one multiplies nothing, so there is one beside every multiplication (64 cycles).
@@ -628,9 +652,15 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
     for (int s = 0; s < n; ++s) {
         const int kb = kb0 + s, s2 = s + 2 < n ? s + 2 : n - 1;
         if (sizeof(TO) == 4) {
-            FP8_READ(1, FP8_STAGE(s))
-            FP8_CONVERT_B(0)
-            FP8_MULTIPLY(0, 0, MT - 1)
+#pragma unroll
+            for (int u = 0; u < U - 4; ++u) {
+                FP8_UNIT(0, u, sa, sb)
+                constexpr int EACH = (MT + NT + U - 5) / (U - 4);
+#pragma unroll
+                for (int f = u * EACH; f < (u + 1) * EACH; ++f)
+                    if (f < MT + NT) FP8_READ1B(1, f, FP8_STAGE(s))
+                __builtin_amdgcn_sched_barrier(0);
+            }
         } else {
             constexpr int EACH = (MT + NT + (MT - 1) * NT - 1) / ((MT - 1) * NT);
 #pragma unroll
@@ -667,8 +697,11 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
 #undef FP8_SCALES
 #undef FP8_READ
 #undef FP8_READ_SCALES
-#undef FP8_CONVERT_B
-#undef FP8_MULTIPLY
+#undef FP8_SCALE
+#undef FP8_XA
+#undef FP8_XB
+#undef FP8_UNIT
+#undef FP8_READ1B
     // Result of a 32 x 32 tile (B's columns are the rows of the instruction): lane: row lane & 31 of C; register q: column
     // (q & 3) + 8 (q >> 2) + 4 (lane >> 5).  32 rows at a time go through the wave's own part of LDS, so that 16 bytes of a
     // row are stored by one lane and a row's bytes by neighbouring ones.
