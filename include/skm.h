@@ -454,7 +454,7 @@ int skm_route_backward(void *ctx, const void *x_dev, int dtype, long T, int E, l
  *   first[E+1]    first tile of an expert, tiles of at most 128 of its rows; [E] = tiles in all
  *   tiles[4 * skm_route_plan_tiles(n, E, 128)]       expert, first row, rows, 0 of every tile (behind them: untouched)
  *   small_tiles[4 * skm_route_plan_tiles(n, E, 16)]  the same with 16 rows a tile, or NULL; small_count[1] their number
- * all int32, dev.  Sizes stay on the device: nothing waits for it. */
+ * all int32, dev, the tile tables 16-byte aligned.  Sizes stay on the device: nothing waits for it. */
 size_t skm_route_plan_workspace_bytes(long n, int E);
 long   skm_route_plan_tiles(long n, int E, int rows);
 int skm_route_plan(void *ctx, const int32_t *ids_dev, long n, int E, int32_t *offsets_dev, int32_t *pair_dev,
@@ -501,8 +501,8 @@ int skm_fp8_columns(void *ctx, const void *x_dev, int dtype, long R, int C, long
  * 13 bits below the largest of them (1.4e-5 of a result of random operands, under the rounding to C's type).
  * accumulate adds to what is there, before the rounding to C's type.
  * a_dtype = -1: A is q, s (lda is not looked at).  a_dtype = SKM_DT_*: A is a float matrix in rows of lda that goes through
- * 8-bit floats of format fmt_a as skm_fp8_rows makes them (sA is not looked at); it needs the workspace (a_float = 1, 16-byte
- * aligned).  q 16-byte, s 4-byte aligned. */
+ * 8-bit floats of format fmt_a as skm_fp8_rows makes them (sA is not looked at).  q and the workspace 16-byte, s 4-byte
+ * aligned; workspace: a_float = 1 for a float A. */
 size_t skm_gemm_fp8_workspace_bytes(void *ctx, int M, int N, int K, int a_float);
 int skm_gemm_fp8(void *ctx, const void *A_dev, const void *sA_dev, int fmt_a, int a_dtype, long lda, const void *B_dev,
                  const void *sB_dev, int fmt_b, int M, int N, int K, void *C_dev, int c_dtype, long ldc, int accumulate,

@@ -131,7 +131,7 @@ template <typename T, int FMT, int COLS>
 __global__ __launch_bounds__(256) void k_fp8_tiles(TileArgs a)
 {
     __shared__ float red[16][FP8_BLOCK];
-    __shared__ __align__(16) uint8_t lt[FP8_BLOCK][FP8_BLOCK + 16];
+    __shared__ __align__(16) uint8_t lt[FP8_BLOCK][FP8_BLOCK];
     const int tid = threadIdx.x, cg = tid & 15, rg = tid >> 4;
     const int c0 = blockIdx.x * FP8_BLOCK, c = c0 + cg * 8;
     const long rb = blockIdx.y, z = blockIdx.z;
@@ -219,15 +219,18 @@ __global__ __launch_bounds__(256) void k_fp8_tiles(TileArgs a)
         uint2 o;
         o.x = fp8_pack4<FMT>(v[0][q], v[1][q], v[2][q], v[3][q]);
         o.y = fp8_pack4<FMT>(v[4][q], v[5][q], v[6][q], v[7][q]);
-        *reinterpret_cast<uint2 *>(&lt[cg * 8 + q][rg * 8]) = o;
+        *reinterpret_cast<uint2 *>(&lt[cg * 8 + q][(rg ^ cg) * 8]) = o;     // 16 lanes meet different banks
     }
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int col = i * 32 + (tid >> 3), piece = tid & 7;
-        if (c0 + col < a.C)
+        if (c0 + col < a.C) {
+            const int x = col >> 3;         // rows 16 piece .. + 7 and + 8 .. + 15: a pair of 8-byte pieces, in order or not
+            const i32x4 v = *reinterpret_cast<const i32x4 *>(&lt[col][((2 * piece) ^ (x & 14)) * 8]);
             *reinterpret_cast<i32x4 *>(a.qt + (z * a.C + c0 + col) * a.Rp + rb * FP8_BLOCK + piece * 16) =
-                *reinterpret_cast<const i32x4 *>(&lt[col][piece * 16]);
+                x & 1 ? __builtin_shufflevector(v, v, 2, 3, 0, 1) : v;
+        }
     }
     if (tid < FP8_BLOCK && c0 + tid < a.C) {
         const float m = red[0][tid];
@@ -343,11 +346,13 @@ struct Fp8Args {
     long ldc;
     int accumulate;
     int c_vec;              // C takes 16-byte stores
+    int c_bf16;             // (host) C's type
+    long experts;           // (host) experts of the plan
     int tiles_m, tiles_n;
     long zC;                // split over k: slab z holds the partial sums of its blocks, zC elements apart
     int slabs;
     // experts: row tiles from a table, the B operand by expert
-    const int32_t *tiles, *tile_count, *pair;
+    const int32_t *tiles, *tile_count, *tile_first, *pair;
     int slots;              // A row of a pair: pair / slots; 0: the plan's own order
     long eB, esB;           // B, sB of the next expert
     // weight gradient: blockIdx.y = expert, its blocks first[e] .. first[e + 1]
@@ -439,6 +444,10 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
         sB += t[0] * g.esB;
         row0 = t[1];
         rows = t[2];
+        if (BM == 256) {                    // two of the table's tiles: the even ones of an expert take the next
+            if ((tm - g.tile_first[t[0]]) & 1) return;
+            if (tm + 1 < g.tile_count[0] && t[4] == t[0]) rows += t[6];
+        }
     } else if (g.first) {
         const int e = blockIdx.y;
         kb0 = g.first[e];
@@ -975,16 +984,53 @@ static int rows16_run(SkmCtx *ctx, const Fp8Args &g, const Fp8Float &fx, int x_d
     }
 }
 
-static int fp8_run(SkmCtx *ctx, Fp8Args g, int fa, int fb, int dtype, unsigned gy, hipStream_t st, const char *tag)
+// the sum of the slabs, in their order, to the result's type
+template <typename TO>
+__global__ __launch_bounds__(256) void k_fp8_slabs(const float *__restrict__ part, int slabs, long zC, int M, int N,
+                                                   TO *__restrict__ C, long ldc, int accumulate)
 {
-    // 256 x 256 tiles (float32 results: 256 x 128, the converted operands need the registers) where they fill the GPU
-    const long wide = (long)((g.M + 255) / 256) * ((g.N + 255) / 256) * gy;
-    const bool big = !g.tiles && wide >= ctx->cu_count / 2;
-    const int bm = big ? 256 : 128, bn = big && dtype != SKM_DT_F32 ? 256 : 128;
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (long)M * N) return;
+    const long m = i / N;
+    TO *c = C + m * ldc + (i - m * N);
+    float v = 0.f;
+    for (int z = 0; z < slabs; ++z) v += part[z * zC + i];
+    *c = (TO)(accumulate ? (float)*c + v : v);
+}
+
+// Few tiles and a long k: slabs of k blocks, so that there are two workgroups per CU, four blocks a slab at least.
+// 1000 x 400 x 30720, float32: 394 us in one slab, 33 us (and 7 for their sum) in 16.
+static int fp8_slabs(const SkmCtx *ctx, long M, long N, long K)
+{
+    const long tiles = ((M + 127) / 128) * ((N + 127) / 128), kb = fp8_kpad(K) / FP8_BLOCK;
+    if (tiles > ctx->cu_count) return 1;
+    long z = 2L * ctx->cu_count / tiles;
+    if (z > kb / 4) z = kb / 4;
+    return z < 2 ? 1 : (int)z;
+}
+
+static int fp8_run(SkmCtx *ctx, Fp8Args g, int fa, int fb, int dtype, unsigned gy, hipStream_t st, const char *tag,
+                   void *ws = nullptr)
+{
+    // 256 x 256 tiles (float32 results: 256 x 128, the converted operands need the registers) where they fill half of the
+    // GPU, 128 x 128 else (8200 x 4096 x 4096: 157 against 250 us).  Experts: with 256 rows each on average.
+    const int wn = dtype != SKM_DT_F32 ? 256 : 128;
+    const long wide = (long)((g.M + 255) / 256) * ((g.N + wn - 1) / wn) * (g.tiles ? 1 : gy);
+    const bool big = wide >= ctx->cu_count / 2 && g.slabs == 1 && (!g.tiles || g.M >= 256 * g.experts);
+    const int bm = big ? 256 : 128, bn = big ? wn : 128;
+    const int csize = skm_dt_size(dtype);
+    const Fp8Args whole = g;
+    if (g.slabs > 1) {                      // partial sums
+        g.C = ws;
+        g.ldc = g.N;
+        g.zC = (long)g.M * g.N;
+        g.accumulate = 0;
+        dtype = SKM_DT_F32;
+    }
     if (!g.tiles) g.tiles_m = (g.M + bm - 1) / bm;
     g.tiles_n = (g.N + bn - 1) / bn;
-    const int csize = skm_dt_size(dtype);
-    g.c_vec = aligned16(g.C, g.ldc * csize) && (g.eC * csize) % 16 == 0 && (g.zC * csize) % 16 == 0;
+    const int esize = skm_dt_size(dtype);
+    g.c_vec = aligned16(g.C, g.ldc * esize) && (g.eC * esize) % 16 == 0 && (g.zC * esize) % 16 == 0;
     // a lane's offset inside a tile (by plan: inside A) is 32 bits wide
     const long reach = g.tiles && g.slots ? g.rowsA : 256;
     if (reach * g.lda > 0xFFFFFFFFL || reach * g.SA > 0x7FFFFFFFL || 256 * g.ldb > 0xFFFFFFFFL) {
@@ -994,16 +1040,33 @@ static int fp8_run(SkmCtx *ctx, Fp8Args g, int fa, int fb, int dtype, unsigned g
     const long total = (long)g.tiles_m * g.tiles_n;
     SKM_REQUIRE(total <= 0x7FFFFFFF && gy <= 65535, "%s: too many tiles", tag);
     if (total == 0 || gy == 0) return SKM_OK;
-    SkmProfScope ps(ctx, tag, st);
-    switch (dtype * 2 + big) {
-    case SKM_DT_F32 * 2: fp8_launch<2, 2, float>(g, fa, fb, (unsigned)total, gy, st); break;
-    case SKM_DT_F32 * 2 + 1: fp8_launch<4, 2, float>(g, fa, fb, (unsigned)total, gy, st); break;
-    case SKM_DT_BF16 * 2: fp8_launch<2, 2, bf16_t>(g, fa, fb, (unsigned)total, gy, st); break;
-    case SKM_DT_BF16 * 2 + 1: fp8_launch<4, 4, bf16_t>(g, fa, fb, (unsigned)total, gy, st); break;
-    case SKM_DT_F16 * 2: fp8_launch<2, 2, f16_t>(g, fa, fb, (unsigned)total, gy, st); break;
-    default: fp8_launch<4, 4, f16_t>(g, fa, fb, (unsigned)total, gy, st); break;
+    {
+        SkmProfScope ps(ctx, tag, st);
+        switch (dtype * 2 + big) {
+        case SKM_DT_F32 * 2: fp8_launch<2, 2, float>(g, fa, fb, (unsigned)total, gy, st); break;
+        case SKM_DT_F32 * 2 + 1: fp8_launch<4, 2, float>(g, fa, fb, (unsigned)total, gy, st); break;
+        case SKM_DT_BF16 * 2: fp8_launch<2, 2, bf16_t>(g, fa, fb, (unsigned)total, gy, st); break;
+        case SKM_DT_BF16 * 2 + 1: fp8_launch<4, 4, bf16_t>(g, fa, fb, (unsigned)total, gy, st); break;
+        case SKM_DT_F16 * 2: fp8_launch<2, 2, f16_t>(g, fa, fb, (unsigned)total, gy, st); break;
+        default: fp8_launch<4, 4, f16_t>(g, fa, fb, (unsigned)total, gy, st); break;
+        }
+        SKM_HIP(hipGetLastError());
     }
-    SKM_HIP(hipGetLastError());
+    if (g.slabs > 1) {
+        SkmProfScope ps(ctx, "k_fp8_slabs", st);
+        const dim3 grid((unsigned)((g.zC + 255) / 256)), block(256);
+        const float *part = static_cast<const float *>(ws);
+        if (csize == 4)
+            hipLaunchKernelGGL(k_fp8_slabs<float>, grid, block, 0, st, part, g.slabs, g.zC, g.M, g.N,
+                               static_cast<float *>(whole.C), whole.ldc, whole.accumulate);
+        else if (whole.c_bf16)
+            hipLaunchKernelGGL(k_fp8_slabs<bf16_t>, grid, block, 0, st, part, g.slabs, g.zC, g.M, g.N,
+                               static_cast<bf16_t *>(whole.C), whole.ldc, whole.accumulate);
+        else
+            hipLaunchKernelGGL(k_fp8_slabs<f16_t>, grid, block, 0, st, part, g.slabs, g.zC, g.M, g.N,
+                               static_cast<f16_t *>(whole.C), whole.ldc, whole.accumulate);
+        SKM_HIP(hipGetLastError());
+    }
     return SKM_OK;
 }
 
@@ -1026,11 +1089,17 @@ static size_t fp8_operand_bytes(long rows, long K)
     return skm_align_up((size_t)rows * fp8_kpad(K), 256) + skm_align_up((size_t)rows * fp8_sstride(K), 256);
 }
 
+static size_t fp8_slab_bytes(const SkmCtx *ctx, long M, long N, long K)
+{
+    if (M <= FP8_FEW_ROWS) return 0;
+    const int z = fp8_slabs(ctx, M, N, K);
+    return z > 1 ? skm_align_up((size_t)z * M * N * 4, 256) : 0;
+}
+
 extern "C" size_t skm_gemm_fp8_workspace_bytes(void *ctx, int M, int N, int K, int a_float)
 {
-    (void)ctx; (void)N;
-    if (M <= 0 || K <= 0) return 0;
-    return a_float && !fp8_on_the_way(M) ? fp8_operand_bytes(M, K) : 0;
+    if (!ctx || M <= 0 || N <= 0 || K <= 0) return 0;
+    return (a_float && !fp8_on_the_way(M) ? fp8_operand_bytes(M, K) : 0) + fp8_slab_bytes(static_cast<SkmCtx *>(ctx), M, N, K);
 }
 
 // A: q, s in 8-bit floats (a_dtype < 0), or a float matrix in rows of lda that goes through 8-bit floats of format fmt_a;
@@ -1081,8 +1150,34 @@ extern "C" int skm_gemm_fp8(void *ctx_, const void *A, const void *sA, int fmt_a
     g.SA = g.SB = (int)fp8_sstride(K);
     g.M = M; g.N = N; g.rowsA = M; g.kb1 = (int)(fp8_kpad(K) / FP8_BLOCK);
     g.C = C; g.ldc = ldc; g.accumulate = accumulate != 0; g.slabs = 1;
-    if (M <= FP8_FEW_ROWS) return rows16_run(ctx, g, fx, a_dtype, fmt_a, fmt_b, c_dtype, 1, (hipStream_t)stream);
-    return fp8_run(ctx, g, fmt_a, fmt_b, c_dtype, 1, (hipStream_t)stream, "k_gemm_fp8");
+    hipStream_t st = (hipStream_t)stream;
+    if (M <= FP8_FEW_ROWS) return rows16_run(ctx, g, fx, a_dtype, fmt_a, fmt_b, c_dtype, 1, st);
+    g.c_bf16 = c_dtype == SKM_DT_BF16;
+    g.slabs = fp8_slabs(ctx, M, N, K);
+    if (g.slabs > 1) {
+        if (!ws || ws_bytes < skm_gemm_fp8_workspace_bytes(ctx, M, N, K, a_dtype >= 0) || ((uintptr_t)ws & 15)) {
+            skm_set_error("skm_gemm_fp8: workspace too small or not aligned");
+            return SKM_ERR_WORKSPACE;
+        }
+        // behind the quantized A
+        char *part = static_cast<char *>(ws) + (a_dtype >= 0 ? fp8_operand_bytes(M, K) : 0);
+        return fp8_run(ctx, g, fmt_a, fmt_b, c_dtype, (unsigned)g.slabs, st, "k_gemm_fp8", part);
+    }
+    // A last row tile of up to 64 rows that would begin another round of workgroups goes to the kernel for few rows
+    // (8200 x 4096 x 4096: 157 -> 122 us)
+    const int wn = c_dtype != SKM_DT_F32 ? 256 : 128, rest = M % 256;
+    const long tn = (N + wn - 1) / wn, cu = ctx->cu_count;
+    if (rest && rest <= FP8_FEW_ROWS && M > 256 && (M / 256) * tn >= cu / 2 &&
+        ((M / 256 + 1) * tn + cu - 1) / cu > ((M / 256) * tn + cu - 1) / cu) {
+        Fp8Args tail = g;
+        g.M = g.rowsA = M - rest;
+        tail.M = tail.rowsA = rest;
+        tail.A += (long)g.M * g.lda;
+        tail.sA += (long)g.M * g.SA;
+        tail.C = static_cast<char *>(C) + (long)g.M * ldc * skm_dt_size(c_dtype);
+        if (int rc = rows16_run(ctx, tail, fx, a_dtype, fmt_a, fmt_b, c_dtype, 1, st)) return rc;
+    }
+    return fp8_run(ctx, g, fmt_a, fmt_b, c_dtype, 1, st, "k_gemm_fp8");
 }
 
 extern "C" size_t skm_gemm_fp8_experts_workspace_bytes(void *ctx, long rows, int K, int a_float, int few)
@@ -1117,7 +1212,7 @@ extern "C" int skm_gemm_fp8_experts(void *ctx_, const void *A, const void *sA, i
     g.SA = g.SB = (int)fp8_sstride(K);
     g.M = (int)n; g.N = N; g.rowsA = rows; g.kb1 = (int)(fp8_kpad(K) / FP8_BLOCK);
     g.C = C; g.ldc = N; g.slabs = 1;
-    g.tiles = tiles; g.tile_count = first + E; g.pair = pair; g.slots = slots;
+    g.tiles = tiles; g.tile_count = first + E; g.tile_first = first; g.pair = pair; g.slots = slots;
     g.eB = (long)N * g.ldb; g.esB = (long)N * g.SB;
     if (small_tiles) {
         g.tiles = small_tiles;
@@ -1126,6 +1221,7 @@ extern "C" int skm_gemm_fp8_experts(void *ctx_, const void *A, const void *sA, i
         SKM_REQUIRE(t <= 65535, "skm_gemm_fp8_experts: more than 65535 tiles of 16 rows");
         return rows16_run(ctx, g, fx, a_dtype, fmt_a, fmt_w, c_dtype, (unsigned)t, (hipStream_t)stream);
     }
+    g.experts = E;
     g.tiles_m = (int)skm_route_plan_tiles(n, E, 128);
     return fp8_run(ctx, g, fmt_a, fmt_w, c_dtype, 1, (hipStream_t)stream, "k_gemm_fp8_experts");
 }

@@ -1018,40 +1018,72 @@ __device__ int plan_scan_block(int v, int *sh, int &total)
     return before + s - v;
 }
 
-// From the histograms of all runs to the first row of every (run, expert), and the tile tables.  One workgroup.
-__device__ void plan_scan(const PlanArgs &a, int32_t *hist, int *sh)
+// From the histograms of all runs to the first row of every (run, expert), and the tile tables.  One workgroup of `threads`
+// (a power of two); `part` has room for that many numbers.  Up to that many experts the threads of one expert share its runs
+// and its tiles.
+__device__ void plan_scan(const PlanArgs &a, int32_t *hist, int *sh, int *part, int threads)
 {
+    int share = 1;                          // threads of an expert
+    while (share * 2 * a.E <= threads && share < a.nw) share *= 2;
+    const int wide = threads / share;       // experts at a time
+    const int s = threadIdx.x / wide, el = threadIdx.x - s * wide;
+    const int per = (a.nw + share - 1) / share;
     int rows0 = 0, tiles0 = 0, small0 = 0;
-    for (int e0 = 0; e0 < a.E; e0 += blockDim.x) {
-        const int e = e0 + threadIdx.x;
-        int count = 0;
+    for (int e0 = 0; e0 < a.E; e0 += wide) {
+        const int e = e0 + el;
+        const int r0 = s * per, r1 = r0 + per < a.nw ? r0 + per : a.nw;
+        int own = 0;
         if (e < a.E)
-            for (int r = 0; r < a.nw; ++r) count += hist[(long)r * a.E + e];
+            for (int r = r0; r < r1; ++r) own += hist[(long)r * a.E + e];
+        part[threadIdx.x] = own;
+        __syncthreads();
+        int count = 0, before = 0;
+        for (int o = 0; o < share; ++o) {
+            const int v = part[o * wide + el];
+            before += o < s ? v : 0;
+            count += v;
+        }
+        // only the first thread of an expert counts in the prefix sums; the others learn its result
+        const int mine = s == 0 ? count : 0;
         int nrows, ntiles, nsmall;
-        const int off = rows0 + plan_scan_block(count, sh, nrows);
-        const int t0 = tiles0 + plan_scan_block((count + 127) / 128, sh, ntiles);
-        const int s0 = small0 + plan_scan_block((count + 15) / 16, sh, nsmall);
+        int off = rows0 + plan_scan_block(mine, sh, nrows);
+        int t0 = tiles0 + plan_scan_block((mine + 127) / 128, sh, ntiles);
+        int s0 = small0 + plan_scan_block((mine + 15) / 16, sh, nsmall);
         rows0 += nrows;
         tiles0 += ntiles;
         small0 += nsmall;
+        if (share > 1) {
+            if (s == 0) part[el] = off;
+            __syncthreads();
+            off = part[el];
+            __syncthreads();
+            if (s == 0) part[el] = t0;
+            __syncthreads();
+            t0 = part[el];
+            __syncthreads();
+            if (s == 0) part[el] = s0;
+            __syncthreads();
+            s0 = part[el];
+        }
+        __syncthreads();
         if (e < a.E) {
-            a.offsets[e] = off;
-            a.first[e] = t0;
-            int at = off;
-            for (int r = 0; r < a.nw; ++r) {
+            if (s == 0) {
+                a.offsets[e] = off;
+                a.first[e] = t0;
+            }
+            int at = off + before;
+            for (int r = r0; r < r1; ++r) {
                 const int c = hist[(long)r * a.E + e];
                 hist[(long)r * a.E + e] = at;
                 at += c;
             }
-            for (int t = 0; t * 128 < count; ++t) {
-                int32_t *d = a.tiles + (long)(t0 + t) * 4;
-                d[0] = e; d[1] = off + t * 128; d[2] = count - t * 128 < 128 ? count - t * 128 : 128; d[3] = 0;
-            }
+            for (int t = s; t * 128 < count; t += share)
+                *reinterpret_cast<int4 *>(a.tiles + (long)(t0 + t) * 4) =
+                    make_int4(e, off + t * 128, count - t * 128 < 128 ? count - t * 128 : 128, 0);
             if (a.small)
-                for (int t = 0; t * 16 < count; ++t) {
-                    int32_t *d = a.small + (long)(s0 + t) * 4;
-                    d[0] = e; d[1] = off + t * 16; d[2] = count - t * 16 < 16 ? count - t * 16 : 16; d[3] = 0;
-                }
+                for (int t = s; t * 16 < count; t += share)
+                    *reinterpret_cast<int4 *>(a.small + (long)(s0 + t) * 4) =
+                        make_int4(e, off + t * 16, count - t * 16 < 16 ? count - t * 16 : 16, 0);
         }
     }
     if (threadIdx.x == 0) {
@@ -1065,14 +1097,14 @@ __device__ void plan_scan(const PlanArgs &a, int32_t *hist, int *sh)
 __global__ __launch_bounds__(64 * PLAN_WAVES) void k_plan_one(PlanArgs a)
 {
     extern __shared__ int32_t lds[];
-    __shared__ int sh[PLAN_WAVES];
+    __shared__ int sh[PLAN_WAVES], part[64 * PLAN_WAVES];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     int32_t *h = lds + (long)wave * a.E;
     plan_clear(h, a.E, lane);
     __syncthreads();
     plan_count(a, wave, lane, h);
     __syncthreads();
-    plan_scan(a, lds, sh);
+    plan_scan(a, lds, sh, part, 64 * PLAN_WAVES);
     __syncthreads();
     plan_place(a, wave, lane, h);
 }
@@ -1089,8 +1121,8 @@ __global__ __launch_bounds__(64) void k_plan_count(PlanArgs a)
 
 __global__ __launch_bounds__(1024) void k_plan_scan(PlanArgs a)
 {
-    __shared__ int sh[16];
-    plan_scan(a, a.hist, sh);
+    __shared__ int sh[16], part[1024];
+    plan_scan(a, a.hist, sh, part, 1024);
 }
 
 __global__ __launch_bounds__(64) void k_plan_place(PlanArgs a)
@@ -1136,7 +1168,7 @@ extern "C" int skm_route_plan(void *ctx_, const int32_t *ids, long n, int E, int
 {
     SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
     SKM_REQUIRE(ctx && n >= 0 && E >= 1 && offsets && first && (n == 0 || (ids && pair && pos && tiles)) &&
-                    (!small_tiles || small_count),
+                    (!small_tiles || small_count) && (((uintptr_t)tiles | (uintptr_t)small_tiles) & 15) == 0,
                 "skm_route_plan: bad argument");
     if (E > ROUTE_MAX_E || n > 0x3FFFFFFF) {
         skm_set_error("skm_route_plan: built for %d experts and 2^30 - 1 pairs", ROUTE_MAX_E);

@@ -1154,7 +1154,7 @@ class HipEngine(object):
             ldc = N
         else:
             ldc = self._matrix(out, "gemm_fp8: out", M, N, (dtype,) if dtype is not None else None)
-        need = self.lib.skm_gemm_fp8_workspace_bytes(self.ctx, M, N, K, 1) if a_dtype >= 0 else 0
+        need = self.lib.skm_gemm_fp8_workspace_bytes(self.ctx, M, N, K, 1 if a_dtype >= 0 else 0)
         ws = self._scratch(need)
         self._check(self.lib.skm_gemm_fp8(
             self.ctx, a, sa, fa, a_dtype, lda, B.q.data_ptr(), B.s.data_ptr(), B.code, M, N, K, out.data_ptr(),

@@ -174,6 +174,37 @@ def test_gemm(eng, M, N, K, dtype):
     assert torch.equal(c, eng.gemm_fp8(A, B, dtype=DT[dtype]))               # the same bits every time
 
 
+@pytest.mark.parametrize("M,N,K,dtype", [(4104, 4096, 256, "bf16"),      # a last row tile of 8 rows would begin another round
+                                         (4104, 2050, 130, "f32"), (2600, 3100, 384, "bf16"), (2600, 3100, 384, "f32")])
+def test_gemm_large_tiles(eng, M, N, K, dtype):
+    a, _ = _wild((M, K), "bf16", 11)
+    b, _ = _wild((N, K), "bf16", 12)
+    A, B = eng.fp8_rows(a.cuda()), eng.fp8_tiles(b.cuda())
+    out = torch.full((M + 1, N), 5.0, dtype=DT[dtype]).cuda()
+    eng.gemm_fp8(A, B, out=out[:M])
+    _product_close(out[:M], A.values().double().cpu().numpy(), B.values().double().cpu().numpy())
+    assert (out[M] == 5.0).all()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_experts_large_tiles(eng, dtype):
+    """hundreds of rows an expert: pairs of the plan's tiles, odd numbers of them among the experts"""
+    T, k, E, N, K = 3000, 2, 5, 3000, 256
+    r = np.random.RandomState(4)
+    ids = np.stack([r.choice(E, 2, replace=False, p=[0.35, 0.3, 0.2, 0.1, 0.05]) for _ in range(T)]).astype(np.int32)
+    ids[r.rand(T) < 0.1] = -1
+    x, _ = _wild((T, K), "bf16", 1)
+    w, _ = _wild((E * N, K), "bf16", 2)
+    X, W = eng.fp8_rows(x.cuda()), eng.fp8_tiles(w.view(E, N, K).cuda())
+    plan = eng.route_plan(torch.from_numpy(ids).cuda(), E)
+    rows = eng.gemm_fp8_experts(X, W, plan, dtype=DT[dtype])
+    pair, expert, _ = rc.plan(ids, E)
+    vx, vw = X.values().double().cpu().numpy(), W.values().double().cpu().numpy()
+    for e in range(E):
+        m = np.flatnonzero(expert == e)
+        _product_close(rows[torch.from_numpy(m).cuda()], vx[pair[m] // k], vw[e])
+
+
 @pytest.mark.parametrize("fa,fb", [("e4m3", "e5m2"), ("e5m2", "e4m3"), ("e5m2", "e5m2")])
 @pytest.mark.parametrize("M,N,K", [(1, 200, 700), (40, 200, 700), (130, 140, 700), (600, 520, 640)])
 def test_gemm_formats_and_blocks(eng, fa, fb, M, N, K):

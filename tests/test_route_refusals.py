@@ -129,6 +129,7 @@ def test_fp8_refusals(lib, ctx):
     assert lib.skm_fp8_columns(ctx, P, 0, 8, 8, 8, 0, P, None, 4, P, 2, None, P, P, None) == ARG
     assert lib.skm_fp8_columns(ctx, P, 0, 8, 8, 8, 0, None, None, 0, None, 0, P, P, P, None) == ARG
     gemm = lib.skm_gemm_fp8
+    odd = ctypes.c_void_p(0x1004)
     assert gemm(ctx, P, P, 0, -1, 0, P, P, 0, 8, 8, 0, P, 0, 8, 0, None, 0, None) == ARG          # no K
     assert gemm(ctx, P, P, 0, -1, 0, P, P, 0, 8, 8, 8, P, 3, 8, 0, None, 0, None) == ARG          # float64 result
     assert gemm(ctx, P, P, 2, -1, 0, P, P, 0, 8, 8, 8, P, 0, 8, 0, None, 0, None) == ARG          # format
@@ -137,7 +138,7 @@ def test_fp8_refusals(lib, ctx):
     assert gemm(ctx, P, P, 0, 3, 8, P, P, 0, 8, 8, 8, P, 0, 8, 0, None, 0, None) == ARG           # float64 A
     assert gemm(ctx, P, P, 0, 0, 7, P, P, 0, 8, 8, 8, P, 0, 8, 0, None, 0, None) == ARG           # rows overlap
     assert gemm(ctx, P, P, 0, 0, 8, P, P, 0, 99, 8, 8, P, 0, 8, 0, None, 0, None) == WORKSPACE
-    odd = ctypes.c_void_p(0x1004)
+    assert gemm(ctx, P, P, 0, 0, 8, P, P, 0, 99, 8, 8, P, 0, 8, 0, odd, 1 << 20, None) == WORKSPACE
     assert gemm(ctx, odd, P, 0, -1, 0, P, P, 0, 8, 8, 8, P, 0, 8, 0, None, 0, None) == ARG        # alignment
     assert gemm(ctx, P, P, 0, -1, 0, odd, P, 0, 8, 8, 8, P, 0, 8, 0, None, 0, None) == ARG
     assert gemm(ctx, P, P, 0, -1, 0, P, P, 0, 0, 8, 8, P, 0, 8, 0, None, 0, None) == 0
