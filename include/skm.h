@@ -453,13 +453,14 @@ int skm_route_backward(void *ctx, const void *x_dev, int dtype, long T, int E, l
  *   pos[n]        t * k + j -> row, -1 for a pair without an expert
  *   first[E+1]    first tile of an expert, tiles of at most 128 of its rows; [E] = tiles in all
  *   tiles[4 * skm_route_plan_tiles(n, E, 128)]       expert, first row, rows, 0 of every tile (behind them: untouched)
- *   small_tiles[4 * skm_route_plan_tiles(n, E, 16)]  the same with 16 rows a tile, or NULL; small_count[1] their number
+ *   more_tiles[4 * skm_route_plan_tiles(n, E, more_rows)]  the same with more_rows = 16 or 256 rows a tile, more_count[1]
+ *                 their number; more_rows = 0: not wanted
  * all int32, dev, the tile tables 16-byte aligned.  Sizes stay on the device: nothing waits for it. */
 size_t skm_route_plan_workspace_bytes(long n, int E);
 long   skm_route_plan_tiles(long n, int E, int rows);
 int skm_route_plan(void *ctx, const int32_t *ids_dev, long n, int E, int32_t *offsets_dev, int32_t *pair_dev,
-                   int32_t *pos_dev, int32_t *first_dev, int32_t *tiles_dev, int32_t *small_tiles_dev,
-                   int32_t *small_count_dev, void *ws_dev, size_t ws_bytes, void *stream);
+                   int32_t *pos_dev, int32_t *first_dev, int32_t *tiles_dev, int more_rows, int32_t *more_tiles_dev,
+                   int32_t *more_count_dev, void *ws_dev, size_t ws_bytes, void *stream);
 
 /* out[t] = sum_j weights[t*k + j] rows[pos[t*k + j]], summed in the order of j in float32; a pos of -1 is a row of zeros.
  * rows [.][N] and out [T][N] float32, bf16 or f16 (bf16 and f16 do not mix).  The gradient of the weights is
@@ -510,15 +511,15 @@ int skm_gemm_fp8(void *ctx, const void *A_dev, const void *sA_dev, int fmt_a, in
 
 /* The experts' products: C[row] = W_e A[row of A], W [E][N][K] (tiles), for the rows of a plan of n pairs.  A has `rows`
  * rows, as for skm_gemm_fp8.  slots = k: the row of A is the pair's token (rows * k = n); slots = 0: A is in the plan's order
- * already (rows = n).  With small_tiles and small_count (few = 1) the weights are read once per 16 rows of an expert straight
- * into registers, for up to about 16 rows an expert.  Rows of C behind the plan's last are left as they are.
+ * already (rows = n).  The plan's second table, if it has one, sets the tiles: 16 rows (the weights straight into registers,
+ * for up to about 16 rows an expert) or 256 (from about 256 rows an expert); 128 without it.  Rows of C behind the plan's last are left as they are.
  * skm_gemm_fp8_experts_wgrad: C[e] (+)= A_e B_e' (float32 [E][M][N]) over the rows of each expert, A [M], B [N] from
  * skm_fp8_columns with the same plan; an expert without rows has zeros. */
-size_t skm_gemm_fp8_experts_workspace_bytes(void *ctx, long rows, int K, int a_float, int few);
+size_t skm_gemm_fp8_experts_workspace_bytes(void *ctx, long rows, int K, int a_float, int more_rows);
 int skm_gemm_fp8_experts(void *ctx, const void *A_dev, const void *sA_dev, int fmt_a, int a_dtype, long lda, long rows,
                          const void *W_dev, const void *sW_dev, int fmt_w, int E, int N, int K, const int32_t *pair_dev,
-                         int slots, long n, const int32_t *first_dev, const int32_t *tiles_dev,
-                         const int32_t *small_tiles_dev, const int32_t *small_count_dev, void *C_dev, int c_dtype,
+                         int slots, long n, const int32_t *first_dev, const int32_t *tiles_dev, int more_rows,
+                         const int32_t *more_tiles_dev, const int32_t *more_count_dev, void *C_dev, int c_dtype,
                          void *ws_dev, size_t ws_bytes, void *stream);
 int skm_gemm_fp8_experts_wgrad(void *ctx, const void *A_dev, const void *sA_dev, int fmt_a, const void *B_dev,
                                const void *sB_dev, int fmt_b, int E, int M, int N, const int32_t *first_dev, long max_tiles,

@@ -347,12 +347,12 @@ struct Fp8Args {
     int accumulate;
     int c_vec;              // C takes 16-byte stores
     int c_bf16;             // (host) C's type
-    long experts;           // (host) experts of the plan
+    int tile_rows;          // (host) rows of a plan's tile
     int tiles_m, tiles_n;
     long zC;                // split over k: slab z holds the partial sums of its blocks, zC elements apart
     int slabs;
     // experts: row tiles from a table, the B operand by expert
-    const int32_t *tiles, *tile_count, *tile_first, *pair;
+    const int32_t *tiles, *tile_count, *pair;
     int slots;              // A row of a pair: pair / slots; 0: the plan's own order
     long eB, esB;           // B, sB of the next expert
     // weight gradient: blockIdx.y = expert, its blocks first[e] .. first[e + 1]
@@ -423,11 +423,13 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
 
     int tm, tn;
     {   // workgroups w, w + 8, ... share an XCD: an XCD takes a run of consecutive tiles, columns of 8 row tiles at a time
-        const int total = g.tiles_m * g.tiles_n;
+        const int tiles_m = g.tiles ? g.tile_count[0] : g.tiles_m;     // by plan: of the grid's, those that there are
+        const int total = tiles_m * g.tiles_n;
         const int q = total / 8, rem = total % 8, x = blockIdx.x % 8, i = blockIdx.x / 8;
+        if (i >= q + (x < rem ? 1 : 0)) return;
         int t = x * q + (x < rem ? x : rem) + i;
         const int group = 8 * g.tiles_n, gi = t / group, m0 = gi * 8;
-        const int gm = g.tiles_m - m0 < 8 ? g.tiles_m - m0 : 8;
+        const int gm = tiles_m - m0 < 8 ? tiles_m - m0 : 8;
         t -= gi * group;
         tm = m0 + t % gm;
         tn = t / gm;
@@ -438,16 +440,11 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
     const uint8_t *B = g.B, *sB = g.sB;
     TO *C = static_cast<TO *>(g.C);
     if (g.tiles) {
-        if (tm >= g.tile_count[0]) return;
         const int32_t *t = g.tiles + (long)tm * 4;
         B += t[0] * g.eB;
         sB += t[0] * g.esB;
         row0 = t[1];
         rows = t[2];
-        if (BM == 256) {                    // two of the table's tiles: the even ones of an expert take the next
-            if ((tm - g.tile_first[t[0]]) & 1) return;
-            if (tm + 1 < g.tile_count[0] && t[4] == t[0]) rows += t[6];
-        }
     } else if (g.first) {
         const int e = blockIdx.y;
         kb0 = g.first[e];
@@ -1013,10 +1010,10 @@ static int fp8_run(SkmCtx *ctx, Fp8Args g, int fa, int fb, int dtype, unsigned g
                    void *ws = nullptr)
 {
     // 256 x 256 tiles (float32 results: 256 x 128, the converted operands need the registers) where they fill half of the
-    // GPU, 128 x 128 else (8200 x 4096 x 4096: 157 against 250 us).  Experts: with 256 rows each on average.
+    // GPU, 128 x 128 else (8200 x 4096 x 4096: 157 against 250 us).  Experts: as the plan's tiles are.
     const int wn = dtype != SKM_DT_F32 ? 256 : 128;
-    const long wide = (long)((g.M + 255) / 256) * ((g.N + wn - 1) / wn) * (g.tiles ? 1 : gy);
-    const bool big = wide >= ctx->cu_count / 2 && g.slabs == 1 && (!g.tiles || g.M >= 256 * g.experts);
+    const long wide = (long)((g.M + 255) / 256) * ((g.N + wn - 1) / wn) * gy;
+    const bool big = g.tiles ? g.tile_rows == 256 : wide >= ctx->cu_count / 2 && g.slabs == 1;
     const int bm = big ? 256 : 128, bn = big ? wn : 128;
     const int csize = skm_dt_size(dtype);
     const Fp8Args whole = g;
@@ -1180,29 +1177,32 @@ extern "C" int skm_gemm_fp8(void *ctx_, const void *A, const void *sA, int fmt_a
     return fp8_run(ctx, g, fmt_a, fmt_b, c_dtype, 1, st, "k_gemm_fp8");
 }
 
-extern "C" size_t skm_gemm_fp8_experts_workspace_bytes(void *ctx, long rows, int K, int a_float, int few)
+extern "C" size_t skm_gemm_fp8_experts_workspace_bytes(void *ctx, long rows, int K, int a_float, int more_rows)
 {
     (void)ctx;
-    return a_float && !few && rows > 0 && K > 0 ? fp8_operand_bytes(rows, K) : 0;
+    return a_float && more_rows != 16 && rows > 0 && K > 0 ? fp8_operand_bytes(rows, K) : 0;
 }
 
 extern "C" int skm_gemm_fp8_experts(void *ctx_, const void *A, const void *sA, int fmt_a, int a_dtype, long lda, long rows,
                                     const void *W, const void *sW, int fmt_w, int E, int N, int K, const int32_t *pair,
-                                    int slots, long n, const int32_t *first, const int32_t *tiles,
-                                    const int32_t *small_tiles, const int32_t *small_count, void *C, int c_dtype, void *ws,
+                                    int slots, long n, const int32_t *first, const int32_t *tiles, int more_rows,
+                                    const int32_t *more_tiles, const int32_t *more_count, void *C, int c_dtype, void *ws,
                                     size_t ws_bytes, void *stream)
 {
     SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
-    SKM_REQUIRE(ctx && E >= 1 && n >= 0 && n <= 0x3FFFFFFF && slots >= 0 && !small_tiles == !small_count,
-                "skm_gemm_fp8_experts: bad argument");
+    SKM_REQUIRE(ctx && E >= 1 && n >= 0 && n <= 0x3FFFFFFF && slots >= 0, "skm_gemm_fp8_experts: bad argument");
+    SKM_REQUIRE(more_rows == 0 || ((more_rows == 16 || more_rows == 256) && more_tiles && more_count),
+                "skm_gemm_fp8_experts: a second table has tiles of 16 or 256 rows");
     if (int rc = fp8_check_product("skm_gemm_fp8_experts", fmt_a, fmt_w, c_dtype, (int)n, N, K)) return rc;
     if (n == 0 || N == 0) return SKM_OK;
     SKM_REQUIRE(K >= 1 && W && sW && C && pair && first && tiles && ((uintptr_t)W & 15) == 0 && ((uintptr_t)sW & 3) == 0,
                 "skm_gemm_fp8_experts: bad argument");
     SKM_REQUIRE(slots ? rows * slots == n : rows == n, "skm_gemm_fp8_experts: %ld rows of A for %ld pairs", rows, n);
+    const long most = skm_route_plan_tiles(n, E, more_rows ? more_rows : 128);
+    SKM_REQUIRE(more_rows != 16 || most <= 65535, "skm_gemm_fp8_experts: more than 65535 tiles of 16 rows");
     Fp8Float fx{};
-    if (int rc = fp8_take_a(ctx, "skm_gemm_fp8_experts", A, sA, a_dtype, lda, fmt_a, rows, K, small_tiles != nullptr, ws,
-                            ws_bytes, &fx, stream))
+    if (int rc = fp8_take_a(ctx, "skm_gemm_fp8_experts", A, sA, a_dtype, lda, fmt_a, rows, K, more_rows == 16, ws, ws_bytes,
+                            &fx, stream))
         return rc;
     SkmDeviceGuard guard(ctx);
     Fp8Args g{};
@@ -1212,17 +1212,14 @@ extern "C" int skm_gemm_fp8_experts(void *ctx_, const void *A, const void *sA, i
     g.SA = g.SB = (int)fp8_sstride(K);
     g.M = (int)n; g.N = N; g.rowsA = rows; g.kb1 = (int)(fp8_kpad(K) / FP8_BLOCK);
     g.C = C; g.ldc = N; g.slabs = 1;
-    g.tiles = tiles; g.tile_count = first + E; g.tile_first = first; g.pair = pair; g.slots = slots;
+    g.tiles = more_rows ? more_tiles : tiles;
+    g.tile_count = more_rows ? more_count : first + E;
+    g.tile_rows = more_rows ? more_rows : 128;
+    g.pair = pair; g.slots = slots;
     g.eB = (long)N * g.ldb; g.esB = (long)N * g.SB;
-    if (small_tiles) {
-        g.tiles = small_tiles;
-        g.tile_count = small_count;
-        const long t = skm_route_plan_tiles(n, E, 16);
-        SKM_REQUIRE(t <= 65535, "skm_gemm_fp8_experts: more than 65535 tiles of 16 rows");
-        return rows16_run(ctx, g, fx, a_dtype, fmt_a, fmt_w, c_dtype, (unsigned)t, (hipStream_t)stream);
-    }
-    g.experts = E;
-    g.tiles_m = (int)skm_route_plan_tiles(n, E, 128);
+    if (more_rows == 16)
+        return rows16_run(ctx, g, fx, a_dtype, fmt_a, fmt_w, c_dtype, (unsigned)most, (hipStream_t)stream);
+    g.tiles_m = (int)most;
     return fp8_run(ctx, g, fmt_a, fmt_w, c_dtype, 1, (hipStream_t)stream, "k_gemm_fp8_experts");
 }
 

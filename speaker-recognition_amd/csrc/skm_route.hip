@@ -943,7 +943,7 @@ extern "C" int skm_route_backward(void *ctx_, const void *x, int dtype, long T, 
 //   pair[n]         row -> t * k + j               pos[n]  t * k + j -> row, -1 without an expert
 //   first[E + 1]    first 128-row tile of an expert (its rows from a tile's start), [E] = number of tiles
 //   tiles[.][4]     per tile: expert, first row, rows (<= 128), 0
-//   small[.][4]     the same with 16 rows a tile (NULL: none), small_count[1]
+//   more[.][4]      the same with 16 or 256 rows a tile (more_rows; 0: none), more_count[1]
 #define PLAN_WAVES 4
 
 struct PlanArgs {
@@ -953,7 +953,8 @@ struct PlanArgs {
     int chunk;              // pairs per wave, a multiple of 64
     int nw;                 // waves (= runs)
     int32_t *hist;          // [nw][E]: counts, then first rows
-    int32_t *offsets, *pair, *pos, *first, *tiles, *small, *small_count;
+    int32_t *offsets, *pair, *pos, *first, *tiles, *more, *more_count;
+    int more_rows;
 };
 
 __device__ __forceinline__ void plan_clear(int32_t *h, int E, int lane)
@@ -1028,7 +1029,8 @@ __device__ void plan_scan(const PlanArgs &a, int32_t *hist, int *sh, int *part, 
     const int wide = threads / share;       // experts at a time
     const int s = threadIdx.x / wide, el = threadIdx.x - s * wide;
     const int per = (a.nw + share - 1) / share;
-    int rows0 = 0, tiles0 = 0, small0 = 0;
+    const int mr = a.more_rows ? a.more_rows : 1;
+    int rows0 = 0, tiles0 = 0, more0 = 0;
     for (int e0 = 0; e0 < a.E; e0 += wide) {
         const int e = e0 + el;
         const int r0 = s * per, r1 = r0 + per < a.nw ? r0 + per : a.nw;
@@ -1045,13 +1047,13 @@ __device__ void plan_scan(const PlanArgs &a, int32_t *hist, int *sh, int *part, 
         }
         // only the first thread of an expert counts in the prefix sums; the others learn its result
         const int mine = s == 0 ? count : 0;
-        int nrows, ntiles, nsmall;
+        int nrows, ntiles, nmore;
         int off = rows0 + plan_scan_block(mine, sh, nrows);
         int t0 = tiles0 + plan_scan_block((mine + 127) / 128, sh, ntiles);
-        int s0 = small0 + plan_scan_block((mine + 15) / 16, sh, nsmall);
+        int s0 = more0 + plan_scan_block((mine + mr - 1) / mr, sh, nmore);
         rows0 += nrows;
         tiles0 += ntiles;
-        small0 += nsmall;
+        more0 += nmore;
         if (share > 1) {
             if (s == 0) part[el] = off;
             __syncthreads();
@@ -1080,16 +1082,16 @@ __device__ void plan_scan(const PlanArgs &a, int32_t *hist, int *sh, int *part, 
             for (int t = s; t * 128 < count; t += share)
                 *reinterpret_cast<int4 *>(a.tiles + (long)(t0 + t) * 4) =
                     make_int4(e, off + t * 128, count - t * 128 < 128 ? count - t * 128 : 128, 0);
-            if (a.small)
-                for (int t = s; t * 16 < count; t += share)
-                    *reinterpret_cast<int4 *>(a.small + (long)(s0 + t) * 4) =
-                        make_int4(e, off + t * 16, count - t * 16 < 16 ? count - t * 16 : 16, 0);
+            if (a.more_rows)
+                for (int t = s; t * mr < count; t += share)
+                    *reinterpret_cast<int4 *>(a.more + (long)(s0 + t) * 4) =
+                        make_int4(e, off + t * mr, count - t * mr < mr ? count - t * mr : mr, 0);
         }
     }
     if (threadIdx.x == 0) {
         a.offsets[a.E] = rows0;
         a.first[a.E] = tiles0;
-        if (a.small) a.small_count[0] = small0;
+        if (a.more_rows) a.more_count[0] = more0;
     }
 }
 
@@ -1163,12 +1165,13 @@ extern "C" long skm_route_plan_tiles(long n, int E, int rows)
 }
 
 extern "C" int skm_route_plan(void *ctx_, const int32_t *ids, long n, int E, int32_t *offsets, int32_t *pair,
-                              int32_t *pos, int32_t *first, int32_t *tiles, int32_t *small_tiles, int32_t *small_count,
-                              void *ws, size_t ws_bytes, void *stream)
+                              int32_t *pos, int32_t *first, int32_t *tiles, int more_rows, int32_t *more_tiles,
+                              int32_t *more_count, void *ws, size_t ws_bytes, void *stream)
 {
     SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
     SKM_REQUIRE(ctx && n >= 0 && E >= 1 && offsets && first && (n == 0 || (ids && pair && pos && tiles)) &&
-                    (!small_tiles || small_count) && (((uintptr_t)tiles | (uintptr_t)small_tiles) & 15) == 0,
+                    (!more_rows || ((more_rows == 16 || more_rows == 256) && more_count && (n == 0 || more_tiles))) &&
+                    (((uintptr_t)tiles | (uintptr_t)more_tiles) & 15) == 0,
                 "skm_route_plan: bad argument");
     if (E > ROUTE_MAX_E || n > 0x3FFFFFFF) {
         skm_set_error("skm_route_plan: built for %d experts and 2^30 - 1 pairs", ROUTE_MAX_E);
@@ -1180,7 +1183,7 @@ extern "C" int skm_route_plan(void *ctx_, const int32_t *ids, long n, int E, int
     }
     SkmDeviceGuard guard(ctx);
     hipStream_t st = (hipStream_t)stream;
-    PlanArgs a{ids, n, E, 0, 0, static_cast<int32_t *>(ws), offsets, pair, pos, first, tiles, small_tiles, small_count};
+    PlanArgs a{ids, n, E, 0, 0, static_cast<int32_t *>(ws), offsets, pair, pos, first, tiles, more_tiles, more_count, more_rows};
     a.nw = plan_runs(n, E, &a.chunk);
     SkmProfScope ps(ctx, "k_plan", st);
     if (plan_is_one(n, E)) {

@@ -107,7 +107,8 @@ SIGNATURES = {
                                     ctypes.c_float, _c_void_p, _c_void_p, _c_void_p, _c_void_p]),
     "skm_route_plan_workspace_bytes": (_c_size_t, [_c_long, _c_int]),
     "skm_route_plan_tiles": (_c_long, [_c_long, _c_int, _c_int]),
-    "skm_route_plan": (_c_int, [_c_void_p, _c_void_p, _c_long, _c_int] + [_c_void_p] * 8 + [_c_size_t, _c_void_p]),
+    "skm_route_plan": (_c_int, [_c_void_p, _c_void_p, _c_long, _c_int] + [_c_void_p] * 5 + [_c_int] + [_c_void_p] * 3
+                       + [_c_size_t, _c_void_p]),
     "skm_route_combine": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_long, _c_int, _c_int,
                                    _c_void_p, _c_int, _c_void_p]),
     "skm_route_combine_backward": (_c_int, [_c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int, _c_long,
@@ -127,7 +128,7 @@ SIGNATURES = {
     "skm_gemm_fp8_experts_workspace_bytes": (_c_size_t, [_c_void_p, _c_long, _c_int, _c_int, _c_int]),
     "skm_gemm_fp8_experts": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_int, _c_long, _c_long, _c_void_p,
                                       _c_void_p, _c_int, _c_int, _c_int, _c_int, _c_void_p, _c_int, _c_long, _c_void_p,
-                                      _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_size_t,
+                                      _c_void_p, _c_int, _c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_size_t,
                                       _c_void_p]),
     "skm_gemm_fp8_experts_wgrad": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_int, _c_void_p, _c_void_p, _c_int,
                                             _c_int, _c_int, _c_int, _c_void_p, _c_long, _c_void_p, _c_int, _c_void_p]),
@@ -1030,8 +1031,7 @@ class HipEngine(object):
         p = plan._ptr
         self._check(self.lib.skm_route_plan(
             self.ctx, ids.data_ptr(), plan.n, E, p("offsets"), p("pair"), p("pos"), p("first"), p("tiles"),
-            p("small_tiles") if plan.few else None, p("small_count") if plan.few else None,
-            ws.data_ptr() if need else None, need, self._stream()))
+            plan.more_rows, p("more_tiles"), p("more_count"), ws.data_ptr() if need else None, need, self._stream()))
         return plan
 
     def route_combine(self, rows, weights, plan, dtype=None):
@@ -1175,13 +1175,12 @@ class HipEngine(object):
                            % ((M, K), W.shape, plan.T, plan.k, plan.E))
         dtype = dtype or self.torch.bfloat16
         out = self.torch.empty((plan.n, N), dtype=dtype, device=self.device)
-        need = self.lib.skm_gemm_fp8_experts_workspace_bytes(self.ctx, M, K, 1, plan.few) if a_dtype >= 0 else 0
+        need = self.lib.skm_gemm_fp8_experts_workspace_bytes(self.ctx, M, K, 1, plan.more_rows) if a_dtype >= 0 else 0
         ws = self._scratch(need)
         self._check(self.lib.skm_gemm_fp8_experts(
             self.ctx, a, sa, fa, a_dtype, lda, M, W.q.data_ptr(), W.s.data_ptr(), W.code, E, N, K,
             plan._ptr("pair"), plan.k if M == plan.T else 0, plan.n, plan._ptr("first"), plan._ptr("tiles"),
-            plan._ptr("small_tiles") if plan.few else None, plan._ptr("small_count") if plan.few else None,
-            out.data_ptr(), self._dt(dtype, (0, 1, 2), "gemm_fp8_experts"), ws.data_ptr() if need else None, need,
+            plan.more_rows, plan._ptr("more_tiles"), plan._ptr("more_count"), out.data_ptr(), self._dt(dtype, (0, 1, 2), "gemm_fp8_experts"), ws.data_ptr() if need else None, need,
             self._stream()))
         return out
 
@@ -1422,12 +1421,12 @@ class RoutePlan(object):
         if self.n > 0x3FFFFFFF:
             raise SkmError("route_plan: %d pairs" % self.n)
         self.max_tiles = engine.lib.skm_route_plan_tiles(self.n, E, 128)
-        # up to 16 rows an expert on average the products stream the weights past 16 rows at a time
-        self.few = self.n <= 16 * E
-        small = engine.lib.skm_route_plan_tiles(self.n, E, 16) if self.few else 0
+        # the second table: up to 16 rows an expert on average the products take 16 rows at a time, from 256 on 256
+        self.more_rows = 16 if self.n <= 16 * E else 256 if self.n >= 256 * E else 0
+        more = engine.lib.skm_route_plan_tiles(self.n, E, self.more_rows) if self.more_rows else 0
         self._at, at = {}, 0
         for name, size in (("offsets", E + 1), ("pair", self.n), ("pos", self.n), ("first", E + 1),
-                           ("tiles", 4 * self.max_tiles), ("small_tiles", 4 * small), ("small_count", 1)):
+                           ("tiles", 4 * self.max_tiles), ("more_tiles", 4 * more), ("more_count", 1)):
             self._at[name] = (at, size)
             at += (size + 3) // 4 * 4
         self._at["tile_count"] = (self._at["first"][0] + E, 1)

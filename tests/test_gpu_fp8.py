@@ -283,14 +283,14 @@ def test_experts_leave_rows_behind_the_last(eng, few):
     """the rows that no pair has keep what the memory held"""
     ids = torch.tensor([[0, -1], [-1, -1], [1, 0]], dtype=torch.int32)
     plan = eng.route_plan(ids.cuda(), 2)
-    assert plan.few
+    assert plan.more_rows == 16
     W = eng.fp8_tiles(torch.randn(2, 40, 128).cuda())
     X = eng.fp8_rows(torch.randn(3, 128).cuda())
     out = torch.full((6, 40), 7.0).cuda()
     eng._check(eng.lib.skm_gemm_fp8_experts(
         eng.ctx, X.q.data_ptr(), X.s.data_ptr(), 0, -1, 0, 3, W.q.data_ptr(), W.s.data_ptr(), 0, 2, 40, 128,
-        plan._ptr("pair"), 2, 6, plan._ptr("first"), plan._ptr("tiles"), plan._ptr("small_tiles") if few else None,
-        plan._ptr("small_count") if few else None, out.data_ptr(), 0, None, 0, eng._stream()))
+        plan._ptr("pair"), 2, 6, plan._ptr("first"), plan._ptr("tiles"), 16 if few else 0, plan._ptr("more_tiles"),
+        plan._ptr("more_count"), out.data_ptr(), 0, None, 0, eng._stream()))
     assert (out[3:] == 7.0).all() and not (out[:3] == 7.0).any()
 
 

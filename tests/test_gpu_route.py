@@ -214,14 +214,14 @@ def test_plan(eng, T, k, E):
     np.testing.assert_array_equal(plan.pos.cpu().numpy(), pos)
     count = np.bincount(expert, minlength=E)
     np.testing.assert_array_equal(plan.offsets.cpu().numpy(), np.concatenate([[0], count.cumsum()]))
-    for rows, name in ((128, "tiles"), (16, "small_tiles")):
+    for rows, name in ((128, "tiles"), (plan.more_rows, "more_tiles")):
+        if rows == 0:
+            continue
         nt = -(-count // rows)
         if name == "tiles":
             np.testing.assert_array_equal(plan.first.cpu().numpy(), np.concatenate([[0], nt.cumsum()]))
-        elif not plan.few:
-            continue
         else:
-            assert int(plan._view("small_count")[0]) == nt.sum()
+            assert int(plan._view("more_count")[0]) == nt.sum()
         want = [(e, count[:e].sum() + i * rows, min(rows, count[e] - i * rows), 0) for e in range(E) for i in range(nt[e])]
         got = plan._view(name).view(-1, 4).cpu().numpy()[:len(want)]
         np.testing.assert_array_equal(got, np.array(want, dtype=np.int64).reshape(-1, 4))

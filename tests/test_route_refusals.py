@@ -83,11 +83,14 @@ def test_route_backward_refusals(lib, ctx, kw, rc):
 @pytest.mark.parametrize("kw,rc", [(dict(ids=None), ARG), (dict(E=0), ARG), (dict(n=-1), ARG), (dict(E=4097), UNSUPPORTED),
                                    (dict(n=1 << 31), UNSUPPORTED), (dict(n=1 << 20, ws_bytes=8), WORKSPACE),
                                    (dict(n=1 << 20, ws=None, ws_bytes=1 << 40), WORKSPACE),
-                                   (dict(small=P, small_count=None), ARG)])
+                                   (dict(more=P, more_rows=16, more_count=None), ARG),
+                                   (dict(more=P, more_rows=32, more_count=P), ARG),
+                                   (dict(more=ctypes.c_void_p(0x1008), more_rows=16, more_count=P), ARG)])
 def test_route_plan_refusals(lib, ctx, kw, rc):
-    a = dict(ids=P, n=64, E=8, ws=P, ws_bytes=0, small=None, small_count=None)
+    a = dict(ids=P, n=64, E=8, ws=P, ws_bytes=0, more=None, more_rows=0, more_count=None)
     a.update(kw)
-    assert lib.skm_route_plan(ctx, a["ids"], a["n"], a["E"], P, P, P, P, P, a["small"], a["small_count"], a["ws"],
+    assert lib.skm_route_plan(ctx, a["ids"], a["n"], a["E"], P, P, P, P, P, a["more_rows"], a["more"],
+                              a["more_count"], a["ws"],
                               a["ws_bytes"], None) == rc
 
 
@@ -145,12 +148,12 @@ def test_fp8_refusals(lib, ctx):
     assert lib.skm_gemm_fp8_workspace_bytes(ctx, 99, 8, 8, 0) == 0
     assert lib.skm_gemm_fp8_workspace_bytes(ctx, 99, 8, 8, 1) >= 99 * (128 + 4)
     ex = lib.skm_gemm_fp8_experts
-    assert ex(ctx, P, P, 0, -1, 0, 4, P, P, 0, 0, 8, 8, P, 2, 8, P, P, None, None, P, 0, None, 0, None) == ARG     # E
-    assert ex(ctx, P, P, 0, -1, 0, 4, P, P, 0, 4, 8, 8, None, 2, 8, P, P, None, None, P, 0, None, 0, None) == ARG  # no pairs
-    assert ex(ctx, P, P, 0, -1, 0, 5, P, P, 0, 4, 8, 8, P, 2, 8, P, P, None, None, P, 0, None, 0, None) == ARG     # 5 x 2 != 8
-    assert ex(ctx, P, P, 0, -1, 0, 4, P, P, 0, 4, 8, 8, P, 0, 8, P, P, None, None, P, 0, None, 0, None) == ARG
-    assert ex(ctx, P, P, 0, -1, 0, 4, P, P, 0, 4, 8, 8, P, 2, 8, P, P, P, None, P, 0, None, 0, None) == ARG        # no count
-    assert ex(ctx, P, None, 0, 0, 8, 4, P, P, 0, 4, 8, 8, P, 2, 8, P, P, None, None, P, 0, None, 0, None) == WORKSPACE
+    assert ex(ctx, P, P, 0, -1, 0, 4, P, P, 0, 0, 8, 8, P, 2, 8, P, P, 0, None, None, P, 0, None, 0, None) == ARG     # E
+    assert ex(ctx, P, P, 0, -1, 0, 4, P, P, 0, 4, 8, 8, None, 2, 8, P, P, 0, None, None, P, 0, None, 0, None) == ARG  # no pairs
+    assert ex(ctx, P, P, 0, -1, 0, 5, P, P, 0, 4, 8, 8, P, 2, 8, P, P, 0, None, None, P, 0, None, 0, None) == ARG     # 5 x 2 != 8
+    assert ex(ctx, P, P, 0, -1, 0, 4, P, P, 0, 4, 8, 8, P, 0, 8, P, P, 0, None, None, P, 0, None, 0, None) == ARG
+    assert ex(ctx, P, P, 0, -1, 0, 4, P, P, 0, 4, 8, 8, P, 2, 8, P, P, 16, P, None, P, 0, None, 0, None) == ARG        # no count
+    assert ex(ctx, P, None, 0, 0, 8, 4, P, P, 0, 4, 8, 8, P, 2, 8, P, P, 0, None, None, P, 0, None, 0, None) == WORKSPACE
     assert lib.skm_gemm_fp8_experts_wgrad(ctx, P, P, 0, P, P, 0, 4, 8, 8, P, 2, None, 0, None) == ARG
     assert lib.skm_gemm_fp8_experts_wgrad(ctx, P, P, 0, P, P, 0, 70000, 8, 8, P, 2, P, 0, None) == ARG
 
