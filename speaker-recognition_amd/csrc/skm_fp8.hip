@@ -83,6 +83,14 @@ struct RowsArgs {
     uint8_t *q, *s;
 };
 
+// a lane's value from another lane of its 16 (CTRL 0x120 + n: n lanes on)
+template <int CTRL>
+__device__ __forceinline__ float lanes16_ror(float v)
+{
+    const int i = __float_as_int(v);
+    return __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xF, 0xF, false));
+}
+
 // blocks of 1 x 128: 16 lanes per block, 8 numbers a lane
 template <typename T, int FMT>
 __global__ __launch_bounds__(256) void k_fp8_rows(RowsArgs a)
@@ -98,8 +106,10 @@ __global__ __launch_bounds__(256) void k_fp8_rows(RowsArgs a)
     float top = 0.f;
 #pragma unroll
     for (int q = 0; q < 8; ++q) top = fmaxf(top, fp8_finite_abs(v[q]));
-#pragma unroll
-    for (int m = 8; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
+    top = fmaxf(top, lanes16_ror<0x128>(top));
+    top = fmaxf(top, lanes16_ror<0x124>(top));
+    top = fmaxf(top, lanes16_ror<0x122>(top));
+    top = fmaxf(top, lanes16_ror<0x121>(top));
     const int e = fp8_exponent(top, FMT);
     const float f = fp8_pow2(-e);
     uint2 o;
@@ -348,6 +358,7 @@ struct Fp8Args {
     int c_vec;              // C takes 16-byte stores
     int c_bf16;             // (host) C's type
     int tile_rows;          // (host) rows of a plan's tile
+    long mean_blocks;       // (host) blocks of an expert on average
     int tiles_m, tiles_n;
     long zC;                // split over k: slab z holds the partial sums of its blocks, zC elements apart
     int slabs;
@@ -782,32 +793,22 @@ struct Fp8Float {
     int vec;                // 16-byte loads are allowed
 };
 
-// 16 consecutive numbers of a row; k behind K counts as 0
-template <typename T>
-__device__ __forceinline__ void load16(const T *row, int k, int K, int vec, float *v)
-{
-    float a[8], b[8];
-    load8(row + k, vec, K - k, a);
-    load8(row + k + 8, vec, K - k - 8, b);
-#pragma unroll
-    for (int q = 0; q < 8; ++q) {
-        v[q] = a[q];
-        v[8 + q] = b[q];
-    }
-}
-
 // C = A B' for up to 16 MT rows of A (or tiles of up to 16 rows of an expert): the bytes of B are what counts, each is
 // read once, straight into registers.  A workgroup holds 16 NT columns, its waves share the k blocks in groups of four
 // (one scale dword per row and group) and add their parts through LDS in a fixed order.  v_mfma_scale_f32_16x16x128:
 // B's columns are the rows of the instruction, so a lane ends with 4 consecutive columns of one row of C.
 // A lane (row r of 16, quarter g) holds bytes 16 g .. and 64 + 16 g .. of a block's 128: a load covers 64 consecutive
 // bytes of 16 rows.
-// XT = uint8_t: A is quantized already.  Otherwise a float type: A is quantized in registers, as k_fp8_rows does it --
-// with one row tile the same work in every workgroup costs less than a launch before this one.
+// XT = uint8_t: A is quantized already.  Otherwise a float type: every wave quantizes the blocks of its four k blocks, as
+// k_fp8_rows does it (16 lanes a block, so one row's four blocks at a time), into LDS -- the same work in every workgroup,
+// under the latency of B's bytes, costs less than a launch before this one.  LDS: a row's 512 bytes, the 16-byte pieces of
+// each 256 exchanged by the row, so that the 16 rows that read the same piece meet different banks.
 template <int MT, int NT, int FA, int FB, typename TO, typename XT>
 __global__ __launch_bounds__(512, 2) void k_gemm_fp8_rows16(Fp8Args g, Fp8Float fx)
 {
-    __shared__ float part[8][MT * NT * 4][64];
+    constexpr bool FLOAT = sizeof(XT) > 1;
+    static_assert(!FLOAT || MT == 1, "float rows are quantized for one row tile");
+    __shared__ __align__(16) float part[8][FLOAT && MT * NT * 4 < 33 ? 33 : MT * NT * 4][64];    // also 8 KB + 64 bytes a wave
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int r = lane & 15, q4 = lane >> 4;
     int rows = g.M;
@@ -823,7 +824,7 @@ __global__ __launch_bounds__(512, 2) void k_gemm_fp8_rows16(Fp8Args g, Fp8Float 
     }
     const int col0 = blockIdx.x * 16 * NT;
     const uint8_t *pb[NT], *qb[NT], *pa[MT], *qa[MT];
-    const XT *px[MT];
+    int src_row = 0;                        // of row r of the tile
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
         const int n = col0 + j * 16 + r < g.N ? col0 + j * 16 + r : g.N - 1;
@@ -835,11 +836,10 @@ __global__ __launch_bounds__(512, 2) void k_gemm_fp8_rows16(Fp8Args g, Fp8Float 
         const int m = i * 16 + r < rows ? i * 16 + r : rows - 1;
         long src = row0 + m;
         if (g.tiles && g.slots) src = g.pair[src] / g.slots;
-        if (sizeof(XT) == 1) {
+        src_row = (int)src;
+        if (!FLOAT) {
             pa[i] = g.A + src * g.lda + q4 * 16;
             qa[i] = g.sA + src * g.SA;
-        } else {
-            px[i] = static_cast<const XT *>(fx.x) + src * fx.ldx;
         }
     }
     f32x4 acc[MT][NT];
@@ -849,72 +849,91 @@ __global__ __launch_bounds__(512, 2) void k_gemm_fp8_rows16(Fp8Args g, Fp8Float 
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int q = 0; q < 4; ++q) acc[i][j][q] = 0.f;
+    uint8_t *lw = reinterpret_cast<uint8_t *>(part[wave]);
+    uint8_t *ls = lw + 16 * 512;            // scales [16][4]
 
     const int groups = (g.kb1 + 3) / 4;
     for (int gr = wave; gr < groups; gr += waves) {
         const int nb = g.kb1 - gr * 4 < 4 ? g.kb1 - gr * 4 : 4;
-        i32x8 w[NT][4];
-        int sw[NT];
+        i32x8 w[NT][4], a[MT][4];
+        int sw[NT], sx[MT];
+        // a short group repeats its first block, unused
+#define ROWS16_LOAD(DST, PTR)                                                                                          \
+    _Pragma("unroll") for (int b = 0; b < 4; ++b) {                                                                    \
+        const uint8_t *p_ = (PTR) + (long)(gr * 4 + (b < nb ? b : 0)) * FP8_BLOCK;                                     \
+        const i32x4 lo_ = *reinterpret_cast<const i32x4 *>(p_), hi_ = *reinterpret_cast<const i32x4 *>(p_ + 64);       \
+        (DST)[b] = __builtin_shufflevector(lo_, hi_, 0, 1, 2, 3, 4, 5, 6, 7);                                          \
+    }
 #pragma unroll
         for (int j = 0; j < NT; ++j) {
             sw[j] = *reinterpret_cast<const int *>(qb[j] + gr * 4);
-#pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const int kb = gr * 4 + (b < nb ? b : 0);        // a short group repeats its first block, unused
-                const i32x4 lo = *reinterpret_cast<const i32x4 *>(pb[j] + (long)kb * FP8_BLOCK);
-                const i32x4 hi = *reinterpret_cast<const i32x4 *>(pb[j] + (long)kb * FP8_BLOCK + 64);
-                w[j][b] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            }
+            ROWS16_LOAD(w[j], pb[j])
         }
+        if (!FLOAT) {
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            int sx = 0;
-            if (sizeof(XT) == 1) sx = *reinterpret_cast<const int *>(qa[i] + gr * 4);
+            for (int i = 0; i < MT; ++i) {
+                sx[i] = *reinterpret_cast<const int *>(qa[i] + gr * 4);
+                ROWS16_LOAD(a[i], pa[i])
+            }
+        } else {
+            // lane: block q4 of the group, numbers 8 r .. 8 r + 7 of it
+            const int k = (gr * 4 + q4) * FP8_BLOCK + r * 8;
+            const int piece = (q4 & 1) * 8 + (r >> 1), line = (q4 >> 1) * 256;
+            for (int m = 0; m < rows; ++m) {
+                const XT *x = static_cast<const XT *>(fx.x) + (long)__builtin_amdgcn_readlane(src_row, m) * fx.ldx;
+                float v[8];
+                load8(x + k, fx.vec, fx.K - k, v);
+                float top = 0.f;
 #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                if (b >= nb) break;
-                const int kb = gr * 4 + b;
-                i32x8 a;
-                int sa;
-                if (sizeof(XT) == 1) {
-                    const i32x4 lo = *reinterpret_cast<const i32x4 *>(pa[i] + (long)kb * FP8_BLOCK);
-                    const i32x4 hi = *reinterpret_cast<const i32x4 *>(pa[i] + (long)kb * FP8_BLOCK + 64);
-                    a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-                    sa = (sx >> (8 * b)) & 255;
-                } else {
-                    float v[32];
-                    load16(px[i], kb * FP8_BLOCK + q4 * 16, fx.K, fx.vec, v);
-                    load16(px[i], kb * FP8_BLOCK + 64 + q4 * 16, fx.K, fx.vec, v + 16);
-                    float top = 0.f;
+                for (int q = 0; q < 8; ++q) top = fmaxf(top, fp8_finite_abs(v[q]));
+                top = fmaxf(top, lanes16_ror<0x128>(top));
+                top = fmaxf(top, lanes16_ror<0x124>(top));
+                top = fmaxf(top, lanes16_ror<0x122>(top));
+                top = fmaxf(top, lanes16_ror<0x121>(top));
+                const int e = fp8_exponent(top, FA);
+                const float f = fp8_pow2(-e);
+                uint2 o;
+                o.x = fp8_pack4<FA>(v[0] * f, v[1] * f, v[2] * f, v[3] * f);
+                o.y = fp8_pack4<FA>(v[4] * f, v[5] * f, v[6] * f, v[7] * f);
+                *reinterpret_cast<uint2 *>(lw + m * 512 + line + (piece ^ m) * 16 + (r & 1) * 8) = o;
+                if (r == 0) ls[m * 4 + q4] = (uint8_t)(e + 127);
+            }
+            __builtin_amdgcn_wave_barrier();            // a wave's LDS instructions are carried out in order
+            sx[0] = *reinterpret_cast<const int *>(ls + r * 4);
 #pragma unroll
-                    for (int q = 0; q < 32; ++q) top = fmaxf(top, fp8_finite_abs(v[q]));
-                    top = fmaxf(top, __shfl_xor(top, 16));
-                    top = fmaxf(top, __shfl_xor(top, 32));
-                    const int e = fp8_exponent(top, FA);
-                    const float f = fp8_pow2(-e);
-                    sa = e + 127;
+            for (int b = 0; b < 4; ++b) {               // rows behind the last: whatever is there, for columns not stored
+                const uint8_t *p = lw + r * 512 + (b >> 1) * 256;
+                const i32x4 lo = *reinterpret_cast<const i32x4 *>(p + (((b & 1) * 8 + q4) ^ r) * 16);
+                const i32x4 hi = *reinterpret_cast<const i32x4 *>(p + (((b & 1) * 8 + 4 + q4) ^ r) * 16);
+                a[0][b] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
+#undef ROWS16_LOAD
 #pragma unroll
-                    for (int q = 0; q < 8; ++q)
-                        a[q] = (int)fp8_pack4<FA>(v[4 * q] * f, v[4 * q + 1] * f, v[4 * q + 2] * f, v[4 * q + 3] * f);
-                }
+        for (int b = 0; b < 4; ++b) {
+            if (b < nb) {
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    const int sb = (sw[j] >> (8 * b)) & 255;
-                    if (sizeof(TO) == 4) {
+                for (int i = 0; i < MT; ++i)
 #pragma unroll
-                        for (int t = 0; t < 4; ++t) {
-                            const bf16x8 xa = fp8_to_bf16<FA>(a[2 * t], a[2 * t + 1], fp8_pow2(sa - 127));
-                            const bf16x8 xb = fp8_to_bf16<FB>(w[j][b][2 * t], w[j][b][2 * t + 1], fp8_pow2(sb - 127));
-                            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb, xa, acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < NT; ++j) {
+                        const int sa = (sx[i] >> (8 * b)) & 255, sb = (sw[j] >> (8 * b)) & 255;
+                        if (sizeof(TO) == 4) {
+#pragma unroll
+                            for (int t = 0; t < 4; ++t) {
+                                const bf16x8 xa = fp8_to_bf16<FA>(a[i][b][2 * t], a[i][b][2 * t + 1], fp8_pow2(sa - 127));
+                                const bf16x8 xb = fp8_to_bf16<FB>(w[j][b][2 * t], w[j][b][2 * t + 1], fp8_pow2(sb - 127));
+                                acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(xb, xa, acc[i][j], 0, 0, 0);
+                            }
+                        } else {
+                            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[j][b], a[i][b], acc[i][j], FB, FA,
+                                                                                         0, sb, 0, sa);
                         }
-                    } else {
-                        acc[i][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w[j][b], a, acc[i][j], FB, FA, 0, sb, 0,
-                                                                                     sa);
                     }
-                }
             }
         }
     }
+    if (FLOAT) __syncthreads();             // the parts of the sums go where the rows were (a wave's own: others' are read)
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -970,8 +989,13 @@ static int rows16_run(SkmCtx *ctx, const Fp8Args &g, const Fp8Float &fx, int x_d
 {
     SkmProfScope ps(ctx, "k_gemm_fp8_rows16", st);
     if (g.A) {
-        if (g.M > 32 && !g.tiles) return rows16_types<4, 2, uint8_t>(g, fx, fa, fb, dtype, gy, st);
-        if (g.M > 16 && !g.tiles) return rows16_types<2, 2, uint8_t>(g, fx, fa, fb, dtype, gy, st);
+        // two column tiles a workgroup (A's rows are read once per workgroup) where they are enough for every CU:
+        // 61 x 8192 x 4096 18.5 us against 27.8, 61 x 4096 x 4096 16.7 against 14.5
+        const bool two = (g.N + 31) / 32 >= ctx->cu_count;
+        if (g.M > 32 && !g.tiles)
+            return two ? rows16_types<4, 2, uint8_t>(g, fx, fa, fb, dtype, gy, st) : rows16_types<4, 1, uint8_t>(g, fx, fa, fb, dtype, gy, st);
+        if (g.M > 16 && !g.tiles)
+            return two ? rows16_types<2, 2, uint8_t>(g, fx, fa, fb, dtype, gy, st) : rows16_types<2, 1, uint8_t>(g, fx, fa, fb, dtype, gy, st);
         return rows16_types<1, 1, uint8_t>(g, fx, fa, fb, dtype, gy, st);
     }
     switch (x_dtype) {
@@ -1010,10 +1034,12 @@ static int fp8_run(SkmCtx *ctx, Fp8Args g, int fa, int fb, int dtype, unsigned g
                    void *ws = nullptr)
 {
     // 256 x 256 tiles (float32 results: 256 x 128, the converted operands need the registers) where they fill half of the
-    // GPU, 128 x 128 else (8200 x 4096 x 4096: 157 against 250 us).  Experts: as the plan's tiles are.
+    // GPU, 128 x 128 else (8200 x 4096 x 4096: 157 against 250 us).  Float32 results of up to 8 blocks are written more than
+    // multiplied: two small workgroups on a CU, one writes while the other multiplies (8192 x 8192 x 512: 93 against 108 us).  Experts: as the plan's tiles are.
     const int wn = dtype != SKM_DT_F32 ? 256 : 128;
     const long wide = (long)((g.M + 255) / 256) * ((g.N + wn - 1) / wn) * gy;
-    const bool big = g.tiles ? g.tile_rows == 256 : wide >= ctx->cu_count / 2 && g.slabs == 1;
+    const bool brief = dtype == SKM_DT_F32 && !g.tiles && (g.first ? g.mean_blocks : g.kb1) <= 8;
+    const bool big = g.tiles ? g.tile_rows == 256 : wide >= ctx->cu_count / 2 && g.slabs == 1 && !brief;
     const int bm = big ? 256 : 128, bn = big ? wn : 128;
     const int csize = skm_dt_size(dtype);
     const Fp8Args whole = g;
@@ -1075,8 +1101,11 @@ static int fp8_check_product(const char *who, int fa, int fb, int dtype, int M, 
     return SKM_OK;
 }
 
-// Up to this many rows the weights are read straight into registers, a workgroup's waves splitting k.
+// Up to this many rows the weights are read straight into registers, a workgroup's waves splitting k ...
 #define FP8_FEW_ROWS 64
+// ... with more than 32 rows only where the columns make a workgroup for every CU (64 x 2048 x 8192: 24 us against 14 in
+// slabs, 64 x 4096 x 4096: 14.5 against 17)
+static bool fp8_few(const SkmCtx *ctx, long M, long N) { return M <= 32 || (M <= FP8_FEW_ROWS && (N + 15) / 16 >= ctx->cu_count); }
 
 // a float A is quantized on the way (no memory for it) up to one row tile
 static bool fp8_on_the_way(long rows) { return rows <= 16; }
@@ -1088,7 +1117,7 @@ static size_t fp8_operand_bytes(long rows, long K)
 
 static size_t fp8_slab_bytes(const SkmCtx *ctx, long M, long N, long K)
 {
-    if (M <= FP8_FEW_ROWS) return 0;
+    if (fp8_few(ctx, M, N)) return 0;
     const int z = fp8_slabs(ctx, M, N, K);
     return z > 1 ? skm_align_up((size_t)z * M * N * 4, 256) : 0;
 }
@@ -1148,7 +1177,7 @@ extern "C" int skm_gemm_fp8(void *ctx_, const void *A, const void *sA, int fmt_a
     g.M = M; g.N = N; g.rowsA = M; g.kb1 = (int)(fp8_kpad(K) / FP8_BLOCK);
     g.C = C; g.ldc = ldc; g.accumulate = accumulate != 0; g.slabs = 1;
     hipStream_t st = (hipStream_t)stream;
-    if (M <= FP8_FEW_ROWS) return rows16_run(ctx, g, fx, a_dtype, fmt_a, fmt_b, c_dtype, 1, st);
+    if (fp8_few(ctx, M, N)) return rows16_run(ctx, g, fx, a_dtype, fmt_a, fmt_b, c_dtype, 1, st);
     g.c_bf16 = c_dtype == SKM_DT_BF16;
     g.slabs = fp8_slabs(ctx, M, N, K);
     if (g.slabs > 1) {
@@ -1243,6 +1272,6 @@ extern "C" int skm_gemm_fp8_experts_wgrad(void *ctx_, const void *A, const void 
     g.SA = g.SB = (int)fp8_sstride(g.lda);
     g.M = M; g.N = N; g.rowsA = M;
     g.C = C; g.ldc = N; g.accumulate = accumulate != 0; g.slabs = 1;
-    g.first = first; g.eC = (long)M * N;
+    g.first = first; g.eC = (long)M * N; g.mean_blocks = max_tiles / E;
     return fp8_run(ctx, g, fmt_a, fmt_b, SKM_DT_F32, (unsigned)E, (hipStream_t)stream, "k_gemm_fp8_wgrad");
 }

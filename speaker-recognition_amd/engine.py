@@ -237,6 +237,11 @@ class HipEngine(object):
     def _stream(self):
         return _c_void_p(self.torch.cuda.current_stream(self.device).cuda_stream)
 
+    def _raw_stream(self):
+        """the current stream as a number: what _stream gives without the objects around it (a tenth of the time, which is
+        what a call for one row is made of)"""
+        return self.torch._C._cuda_getCurrentRawStream(self.device_index)
+
     def workspace(self, nbytes):
         if nbytes > self._ws_bytes:
             self._ws = None
@@ -996,7 +1001,7 @@ class HipEngine(object):
             self.ctx, logits.data_ptr(), self._dt(logits.dtype, (0, 1, 2, 3), "route: logits"), T, E, ldx, k,
             self._scores(scores), bias.data_ptr() if bias is not None else None, int(groups),
             int(groups if group_k is None else group_k), int(group_top), 1 if renorm else 0, float(scale),
-            ids.data_ptr(), weights.data_ptr(), self._stream()))
+            ids.data_ptr(), weights.data_ptr(), self._raw_stream()))
         return ids, weights
 
     def route_backward(self, logits, ids, dweights, scores="softmax", renorm=True, scale=1.0):
@@ -1011,7 +1016,7 @@ class HipEngine(object):
         self._check(self.lib.skm_route_backward(
             self.ctx, logits.data_ptr(), self._dt(logits.dtype, (0, 1, 2, 3), "route_backward: logits"), T, E, ldx, k,
             self._scores(scores), 1 if renorm else 0, float(scale), ids.data_ptr(), dweights.data_ptr(), dx.data_ptr(),
-            self._stream()))
+            self._raw_stream()))
         return dx
 
     def route_plan(self, ids, E):
@@ -1031,7 +1036,7 @@ class HipEngine(object):
         p = plan._ptr
         self._check(self.lib.skm_route_plan(
             self.ctx, ids.data_ptr(), plan.n, E, p("offsets"), p("pair"), p("pos"), p("first"), p("tiles"),
-            plan.more_rows, p("more_tiles"), p("more_count"), ws.data_ptr() if need else None, need, self._stream()))
+            plan.more_rows, p("more_tiles"), p("more_count"), ws.data_ptr() if need else None, need, self._raw_stream()))
         return plan
 
     def route_combine(self, rows, weights, plan, dtype=None):
@@ -1045,7 +1050,7 @@ class HipEngine(object):
         self._check(self.lib.skm_route_combine(
             self.ctx, rows.data_ptr(), self._dt(rows.dtype, (0, 1, 2), "route_combine: rows"), plan._ptr("pos"),
             weights.data_ptr(), plan.T, plan.k, N, out.data_ptr(), self._dt(dtype, (0, 1, 2), "route_combine"),
-            self._stream()))
+            self._raw_stream()))
         return out
 
     def route_combine_backward(self, rows, dout, plan):
@@ -1058,7 +1063,7 @@ class HipEngine(object):
         self._check(self.lib.skm_route_combine_backward(
             self.ctx, rows.data_ptr(), self._dt(rows.dtype, (0, 1, 2), "route_combine_backward: rows"), plan._ptr("pos"),
             dout.data_ptr(), self._dt(dout.dtype, (0, 1, 2), "route_combine_backward: dout"), plan.T, plan.k, N,
-            dw.data_ptr(), self._stream()))
+            dw.data_ptr(), self._raw_stream()))
         return dw
 
     @staticmethod
@@ -1075,7 +1080,7 @@ class HipEngine(object):
             raise SkmError("fp8_rows: rows of no elements")
         out = Fp8Matrix(self, (M,), K, fmt)
         self._check(self.lib.skm_fp8_rows(self.ctx, x.data_ptr(), self._dt(x.dtype, (0, 1, 2), "fp8_rows: x"), M, K, ldx,
-                                          self._fmt(fmt), out.q.data_ptr(), out.s.data_ptr(), self._stream()))
+                                          self._fmt(fmt), out.q.data_ptr(), out.s.data_ptr(), self._raw_stream()))
         return out
 
     def fp8_tiles(self, w, fmt="e4m3", transposed=False):
@@ -1093,7 +1098,7 @@ class HipEngine(object):
         self._check(self.lib.skm_fp8_tiles(
             self.ctx, w.data_ptr(), self._dt(w.dtype, (0, 1, 2), "fp8_tiles: w"), batch[0] if batch else 1, N, K, K, N * K,
             self._fmt(fmt), out.q.data_ptr(), out.s.data_ptr(), outt.q.data_ptr() if transposed else None,
-            outt.s.data_ptr() if transposed else None, self._stream()))
+            outt.s.data_ptr() if transposed else None, self._raw_stream()))
         return (out, outt) if transposed else out
 
     def fp8_columns(self, x, fmt="e4m3", plan=None, weights=None):
@@ -1116,7 +1121,7 @@ class HipEngine(object):
             plan._ptr("tiles") if plan is not None else None, plan._ptr("tile_count") if plan is not None else None,
             plan.max_tiles if plan is not None else 0, plan._ptr("pair") if plan is not None else None,
             plan.k if plan is not None else 0, weights.data_ptr() if weights is not None else None, out.q.data_ptr(),
-            out.s.data_ptr(), self._stream()))
+            out.s.data_ptr(), self._raw_stream()))
         return out
 
     def _fp8(self, m, what, dims=1):
@@ -1159,7 +1164,7 @@ class HipEngine(object):
         self._check(self.lib.skm_gemm_fp8(
             self.ctx, a, sa, fa, a_dtype, lda, B.q.data_ptr(), B.s.data_ptr(), B.code, M, N, K, out.data_ptr(),
             self._dt(out.dtype, (0, 1, 2), "gemm_fp8"), ldc, 1 if accumulate else 0, ws.data_ptr() if need else None, need,
-            self._stream()))
+            self._raw_stream()))
         return out
 
     def gemm_fp8_experts(self, A, W, plan, dtype=None):
@@ -1181,7 +1186,7 @@ class HipEngine(object):
             self.ctx, a, sa, fa, a_dtype, lda, M, W.q.data_ptr(), W.s.data_ptr(), W.code, E, N, K,
             plan._ptr("pair"), plan.k if M == plan.T else 0, plan.n, plan._ptr("first"), plan._ptr("tiles"),
             plan.more_rows, plan._ptr("more_tiles"), plan._ptr("more_count"), out.data_ptr(), self._dt(dtype, (0, 1, 2), "gemm_fp8_experts"), ws.data_ptr() if need else None, need,
-            self._stream()))
+            self._raw_stream()))
         return out
 
     def gemm_fp8_experts_wgrad(self, A, B, plan, out=None, accumulate=False):
@@ -1201,7 +1206,7 @@ class HipEngine(object):
             raise SkmError("gemm_fp8_experts_wgrad: out is a contiguous float32 tensor %s" % ((plan.E, M, N),))
         self._check(self.lib.skm_gemm_fp8_experts_wgrad(
             self.ctx, A.q.data_ptr(), A.s.data_ptr(), A.code, B.q.data_ptr(), B.s.data_ptr(), B.code, plan.E, M, N,
-            plan._ptr("first"), plan.max_tiles, out.data_ptr(), 1 if accumulate else 0, self._stream()))
+            plan._ptr("first"), plan.max_tiles, out.data_ptr(), 1 if accumulate else 0, self._raw_stream()))
         return out
 
     # ------------------------------------------------------------------ profiling, copies
@@ -1418,26 +1423,32 @@ class RoutePlan(object):
 
     def __init__(self, engine, T, k, E):
         self.engine, self.T, self.k, self.E, self.n = engine, T, k, E, T * k
-        if self.n > 0x3FFFFFFF:
-            raise SkmError("route_plan: %d pairs" % self.n)
-        self.max_tiles = engine.lib.skm_route_plan_tiles(self.n, E, 128)
+        n = self.n
+        if n > 0x3FFFFFFF:
+            raise SkmError("route_plan: %d pairs" % n)
         # the second table: up to 16 rows an expert on average the products take 16 rows at a time, from 256 on 256
-        self.more_rows = 16 if self.n <= 16 * E else 256 if self.n >= 256 * E else 0
-        more = engine.lib.skm_route_plan_tiles(self.n, E, self.more_rows) if self.more_rows else 0
-        self._at, at = {}, 0
-        for name, size in (("offsets", E + 1), ("pair", self.n), ("pos", self.n), ("first", E + 1),
-                           ("tiles", 4 * self.max_tiles), ("more_tiles", 4 * more), ("more_count", 1)):
-            self._at[name] = (at, size)
-            at += (size + 3) // 4 * 4
-        self._at["tile_count"] = (self._at["first"][0] + E, 1)
-        self._buf = engine.torch.empty(at, dtype=engine.torch.int32, device=engine.device)
+        self.more_rows = 16 if n <= 16 * E else 256 if n >= 256 * E else 0
+        self.max_tiles = n // 128 + min(n, E)                   # skm_route_plan_tiles
+        more = n // self.more_rows + min(n, E) if self.more_rows else 0
+        # places of the tensors in the allocation, each at a multiple of 16 bytes
+        e4, n4 = (E + 4) // 4 * 4, (n + 3) // 4 * 4
+        first = e4 + 2 * n4
+        tiles = first + e4
+        more_tiles = tiles + 4 * self.max_tiles
+        self._at = {"offsets": 0, "pair": e4, "pos": e4 + n4, "first": first, "tile_count": first + E, "tiles": tiles,
+                    "more_tiles": more_tiles, "more_count": more_tiles + 4 * more}
+        self._buf = engine.torch.empty(more_tiles + 4 * more + 1, dtype=engine.torch.int32, device=engine.device)
         self._base = self._buf.data_ptr()
 
     def _ptr(self, name):
-        return self._base + 4 * self._at[name][0]
+        return self._base + 4 * self._at[name]
 
     def _view(self, name):
-        at, size = self._at[name]
+        """one of the tensors of include/skm.h, flat"""
+        more = (self._at["more_count"] - self._at["more_tiles"])
+        size = {"offsets": self.E + 1, "first": self.E + 1, "pair": self.n, "pos": self.n, "tiles": 4 * self.max_tiles,
+                "more_tiles": more, "more_count": 1}[name]
+        at = self._at[name]
         return self._buf[at:at + size]
 
     offsets = property(lambda self: self._view("offsets"))

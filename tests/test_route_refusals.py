@@ -33,6 +33,9 @@ class _CpuEngine(sk.HipEngine):
     def _stream(self):
         return None
 
+    def _raw_stream(self):
+        return None
+
     def close(self):
         pass
 
@@ -205,6 +208,26 @@ def test_engine_refusals(eng):
     _refused(eng.route_combine_backward, torch.zeros(8, 6), torch.zeros(4, 5), plan)
     # a valid call reaches the library, which wants a context
     _refused(eng.route, x, 2)
+
+
+@pytest.mark.parametrize("T,k,E", [(0, 2, 5), (1, 1, 1), (7, 3, 4), (8, 4, 64), (300, 2, 4), (5000, 3, 130)])
+def test_plan_layout(eng, lib, T, k, E):
+    """the plan's tensors do not overlap, fit and are aligned as the library wants them"""
+    p = sk.RoutePlan(eng, T, k, E)
+    n = T * k
+    assert p.max_tiles == lib.skm_route_plan_tiles(n, E, 128)
+    if p.more_rows:
+        assert p._view("more_tiles").numel() == 4 * lib.skm_route_plan_tiles(n, E, p.more_rows)
+    spans = []
+    for name in ("offsets", "pair", "pos", "first", "tiles", "more_tiles", "more_count"):
+        v = p._view(name)
+        assert v.numel() == 0 or v.data_ptr() == p._ptr(name)
+        if name in ("tiles", "more_tiles"):
+            assert (p._ptr(name) - p._base) % 16 == 0
+        spans.append((p._at[name], p._at[name] + v.numel()))
+    spans.sort()
+    assert all(a[1] <= b[0] for a, b in zip(spans, spans[1:])) and spans[-1][1] <= p._buf.numel()
+    assert p._ptr("tile_count") == p._ptr("first") + 4 * E
 
 
 def test_values_of_a_matrix(eng):
