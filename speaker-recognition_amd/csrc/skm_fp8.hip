@@ -44,16 +44,12 @@ __device__ __forceinline__ float fp8_finite_abs(float x)
     return a < __builtin_inff() ? a : 0.f;      // NaN and infinities do not set the scale
 }
 
-// four scaled numbers -> four bytes, to nearest even.  e4m3 has no infinity: an infinite number becomes NaN
+// four scaled numbers -> four bytes, to nearest even.  The scale keeps finite numbers inside the format; the instruction
+// makes NaN of an infinity in e4m3, which has none.
 template <int FMT>
 __device__ __forceinline__ unsigned fp8_pack4(float a, float b, float c, float d)
 {
     if (FMT == SKM_FP8_E4M3) {
-        const float inf = __builtin_inff(), nan = __builtin_nanf("");
-        a = fabsf(a) == inf ? nan : a;
-        b = fabsf(b) == inf ? nan : b;
-        c = fabsf(c) == inf ? nan : c;
-        d = fabsf(d) == inf ? nan : d;
         const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
         return (unsigned)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, lo, true);
     }
@@ -400,7 +396,7 @@ typedef __attribute__((address_space(3))) void *lds_ptr;
 typedef __attribute__((address_space(1))) const void *glb_ptr;
 
 // C = A B'.  Workgroup: 4 waves as 2 x 2, a wave MT x NT tiles of 32 x 32 (v_mfma_scale_f32_32x32x64_f8f6f4), one block
-// of 128 k a stage, two stages in LDS filled by global loads that go there directly.
+// of 128 k a stage, DEPTH (2, 3) stages in LDS filled by global loads that go there directly.
 //   LDS: a row's 128 bytes of a stage are one line; its 16-byte pieces are stored at piece ^ ((row >> 1) & 7), so that the
 //   lanes of a read phase (16 rows, the same piece) meet different bank groups (row & 7 costs 4 cycles more per read,
 //   measured).  The loads put consecutive lanes'
@@ -415,20 +411,22 @@ typedef __attribute__((address_space(1))) const void *glb_ptr;
 //   scale covers all of them: a lane's 32 bytes are 32 consecutive k of its row here.
 // A stage is two halves of 64 k in two sets of fragments: while one set is multiplied, the other is read.  Stage s:
 //   read half 1 of s; multiply half 0 (all but the last row of tiles)
-//   wait for the own reads and for the own loads of stage s + 1; barrier: nobody reads buffer s & 1 any more, stage s + 1 is
+//   wait for the own reads and for the own loads of stage s + 1; barrier: nobody reads stage s any more, stage s + 1 is
 //   complete
-//   issue the loads of stage s + 2 into buffer s & 1; multiply the rest of half 0
+//   issue the loads of stage s + DEPTH into the buffer that is free; multiply the rest of half 0
 //   read half 0 of s + 1; multiply half 1
-// so a load has one and a half stages to arrive, an LDS read half a stage, and the barrier stands among multiplications
+// so a load has DEPTH - 1/2 stages to arrive, an LDS read half a stage, and the barrier stands among multiplications
 // that are under way already.
 template <int MT, int NT, int FA, int FB, typename TO>
 __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args g)
 {
     constexpr int BM = MT * 64, BN = NT * 64, LOADS = (MT + NT) * 2;
     // One array: with two of them hipcc waits for the loads in flight in front of every read of LDS.
-    // [two stages of (BM + BN) rows of 128 bytes][two groups of four blocks of (BM + BN) scale dwords]
+    // [DEPTH stages of (BM + BN) rows of 128 bytes][two groups of four blocks of (BM + BN) scale dwords]
+    // 256 x 128 has room for three stages, and a load then has two and a half to arrive.
+    constexpr int DEPTH = MT == 4 && NT == 2 ? 3 : 2;
     constexpr int STAGE = (BM + BN) * FP8_BLOCK, GROUP = (BM + BN) * 4;
-    __shared__ __align__(16) uint8_t sh[2 * STAGE + 2 * GROUP];
+    __shared__ __align__(16) uint8_t sh[DEPTH * STAGE + 2 * GROUP];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 1, wn = wave & 1, r = lane & 31, h = lane >> 5;
 
@@ -587,19 +585,16 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
     }
     // the columns first
 #define FP8_READ1B(H, F, BUF) FP8_READ1(H, ((F) < NT ? MT + (F) : (F) - NT), BUF)
-#define FP8_STAGE(S) (sh + ((S) & 1) * STAGE)
-#define FP8_SCALE_GROUP(KB) (sh + 2 * STAGE + (((KB) >> 2) & 1) * GROUP)
+#define FP8_SCALE_GROUP(KB) (sh + DEPTH * STAGE + (((KB) >> 2) & 1) * GROUP)
     const int n = kb1 - kb0;
     if (n > 0) {
-        FP8_SCALES(kb0 >> 2, FP8_SCALE_GROUP(kb0))
-        if (n > 1 && ((kb0 + 1) >> 2) != (kb0 >> 2)) { FP8_SCALES((kb0 + 1) >> 2, FP8_SCALE_GROUP(kb0 + 1)) }
-        FP8_ISSUE(0, sh)
-        if (n > 1) {
-            FP8_ISSUE(1, sh + STAGE)
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(LOADS) : "memory");
-        } else {
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < DEPTH; ++i) {   // behind the last stage the last one again: every stage has as many loads
+            const int si = i < n ? i : n - 1;
+            FP8_SCALES((kb0 + si) >> 2, FP8_SCALE_GROUP(kb0 + si))
+            FP8_ISSUE(si, sh + i * STAGE)
         }
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"((DEPTH - 1) * (LOADS + MINE)) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         FP8_READ(0, sh)
@@ -666,8 +661,9 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
     };
     // One straight block per stage, without a branch: behind the last stage the last one is loaded again into the free
     // buffer, and what is read of it is not used; a group's scales are loaded again with each of its stages.
+    int cur = 0, nxt = STAGE;               // where stages s and s + 1 are
     for (int s = 0; s < n; ++s) {
-        const int kb = kb0 + s, s2 = s + 2 < n ? s + 2 : n - 1;
+        const int kb = kb0 + s, s2 = s + DEPTH < n ? s + DEPTH : n - 1;
         if (sizeof(TO) == 4) {
 #pragma unroll
             for (int u = 0; u < U - 4; ++u) {
@@ -675,7 +671,7 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
                 constexpr int EACH = (MT + NT + U - 5) / (U - 4);
 #pragma unroll
                 for (int f = u * EACH; f < (u + 1) * EACH; ++f)
-                    if (f < MT + NT) FP8_READ1B(1, f, FP8_STAGE(s))
+                    if (f < MT + NT) FP8_READ1B(1, f, sh + cur)
                 __builtin_amdgcn_sched_barrier(0);
             }
         } else {
@@ -685,7 +681,7 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
                 FP8_TILE(0, u / NT, u % NT)
 #pragma unroll
                 for (int f = u * EACH; f < (u + 1) * EACH; ++f)
-                    if (f < MT + NT) FP8_READ1(1, f, FP8_STAGE(s))
+                    if (f < MT + NT) FP8_READ1(1, f, sh + cur)
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -695,9 +691,11 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
 #pragma unroll
             for (int j = 0; j < NT; ++j) asm volatile("" : "+a"(acc[i][j]));
         __builtin_amdgcn_sched_barrier(0);
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"((DEPTH - 2) * (LOADS + MINE)) : "memory");
         __builtin_amdgcn_sched_barrier(0);
-        late(s2, kb, FP8_STAGE(s), FP8_STAGE(s + 1), FP8_SCALE_GROUP(kb0 + s2), FP8_SCALE_GROUP(kb + 1));
+        late(s2, kb, sh + cur, sh + nxt, FP8_SCALE_GROUP(kb0 + s2), FP8_SCALE_GROUP(kb + 1));
+        cur = nxt;
+        nxt = nxt + STAGE == DEPTH * STAGE ? 0 : nxt + STAGE;
         __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int i = 0; i < MT; ++i) sa[i] = na[i];
@@ -705,7 +703,6 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
         for (int j = 0; j < NT; ++j) sb[j] = nb[j];
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");       // nothing lands in LDS behind the loop
-#undef FP8_STAGE
 #undef FP8_SCALE_GROUP
 #undef FP8_READ1
 #undef FP8_ISSUE1
@@ -1034,11 +1031,11 @@ static int fp8_run(SkmCtx *ctx, Fp8Args g, int fa, int fb, int dtype, unsigned g
                    void *ws = nullptr)
 {
     // 256 x 256 tiles (float32 results: 256 x 128, the converted operands need the registers) where they fill half of the
-    // GPU, 128 x 128 else (8200 x 4096 x 4096: 157 against 250 us).  Float32 results of up to 8 blocks are written more than
+    // GPU, 128 x 128 else (8200 x 4096 x 4096: 157 against 250 us).  Float32 results of up to 10 blocks are written more than
     // multiplied: two small workgroups on a CU, one writes while the other multiplies (8192 x 8192 x 512: 93 against 108 us).  Experts: as the plan's tiles are.
     const int wn = dtype != SKM_DT_F32 ? 256 : 128;
     const long wide = (long)((g.M + 255) / 256) * ((g.N + wn - 1) / wn) * gy;
-    const bool brief = dtype == SKM_DT_F32 && !g.tiles && (g.first ? g.mean_blocks : g.kb1) <= 8;
+    const bool brief = dtype == SKM_DT_F32 && !g.tiles && (g.first ? g.mean_blocks : g.kb1) <= 10;
     const bool big = g.tiles ? g.tile_rows == 256 : wide >= ctx->cu_count / 2 && g.slabs == 1 && !brief;
     const int bm = big ? 256 : 128, bn = big ? wn : 128;
     const int csize = skm_dt_size(dtype);

@@ -1211,30 +1211,38 @@ struct CombineArgs {
 
 // out[t] = sum_j w[t][j] rows[pos[t][j]], in the order of j, float32.  An empty place adds w * 0: nothing, or the NaN
 // that a row without a choice carries in its weights.
+// A workgroup has one token (or, of short rows, several): its places and weights are the same for all lanes of a row, four
+// rows are in flight.
 template <typename TR, typename TO, int VEC>
-__global__ __launch_bounds__(256) void k_route_combine(CombineArgs a)
+__global__ __launch_bounds__(256) void k_route_combine(CombineArgs a, int per, int tokens)
 {
-    const long per = (a.N + VEC - 1) / VEC;
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= a.T * per) return;
-    const long t = i / per;
-    const int c = (int)(i - t * per) * VEC;
     typedef TR vr __attribute__((ext_vector_type(VEC)));
     typedef TO vo __attribute__((ext_vector_type(VEC)));
+    const int sub = tokens > 1 ? threadIdx.x / per : 0;         // per: threads of a row, where a workgroup has several
+    const long t = (long)blockIdx.x * tokens + sub;
+    const int c = (tokens > 1 ? (int)threadIdx.x - sub * per : (int)(blockIdx.y * 256 + threadIdx.x)) * VEC;
+    if (t >= a.T || sub >= tokens || c >= a.N) return;
+    const int32_t *pos = a.pos + t * a.k;
+    const float *w = a.w + t * a.k;
+    const TR *rows = static_cast<const TR *>(a.rows) + c;
     float s[VEC];
 #pragma unroll
     for (int q = 0; q < VEC; ++q) s[q] = 0.f;
-    for (int j = 0; j < a.k; ++j) {
-        const int p = a.pos[t * a.k + j];
-        const float w = a.w[t * a.k + j];
-        if (p < 0) {
+    for (int j0 = 0; j0 < a.k; j0 += 4) {
+        vr v[4];
+        float f[4];
 #pragma unroll
-            for (int q = 0; q < VEC; ++q) s[q] += w * 0.f;
-            continue;
+        for (int u = 0; u < 4; ++u) {
+            const int p = j0 + u < a.k ? pos[j0 + u] : -1;
+            f[u] = j0 + u < a.k ? w[j0 + u] : 0.f;
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) v[u][q] = (TR)0.f;
+            if (p >= 0) v[u] = *reinterpret_cast<const vr *>(rows + (long)p * a.N);
         }
-        const vr v = *reinterpret_cast<const vr *>(static_cast<const TR *>(a.rows) + (long)p * a.N + c);
 #pragma unroll
-        for (int q = 0; q < VEC; ++q) s[q] += w * (float)v[q];
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) s[q] += f[u] * (float)v[u][q];
     }
     vo o;
 #pragma unroll
@@ -1243,9 +1251,11 @@ __global__ __launch_bounds__(256) void k_route_combine(CombineArgs a)
 }
 
 // dw[t][j] = <dout[t], rows[pos[t][j]]>: one wave per pair
-template <typename TR, typename TO>
+template <typename TR, typename TO, int VEC>
 __global__ __launch_bounds__(256) void k_route_combine_backward(CombineArgs a)
 {
+    typedef TR vr __attribute__((ext_vector_type(VEC)));
+    typedef TO vo __attribute__((ext_vector_type(VEC)));
     const int lane = threadIdx.x & 63;
     const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (i >= a.T * a.k) return;
@@ -1254,7 +1264,18 @@ __global__ __launch_bounds__(256) void k_route_combine_backward(CombineArgs a)
     if (p >= 0) {
         const TR *r = static_cast<const TR *>(a.rows) + (long)p * a.N;
         const TO *d = static_cast<const TO *>(a.dout) + (i / a.k) * a.N;
-        for (int c = lane; c < a.N; c += 64) s += (float)r[c] * (float)d[c];
+        float part[VEC];
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) part[q] = 0.f;
+#pragma unroll 4
+        for (int c = lane * VEC; c < a.N; c += 64 * VEC) {
+            const vr x = *reinterpret_cast<const vr *>(r + c);
+            const vo y = *reinterpret_cast<const vo *>(d + c);
+#pragma unroll
+            for (int q = 0; q < VEC; ++q) part[q] += (float)x[q] * (float)y[q];
+        }
+#pragma unroll
+        for (int q = 0; q < VEC; ++q) s += part[q];
         s = wave_sum(s);
     }
     if (lane == 0) a.dw[i] = s;
@@ -1263,17 +1284,24 @@ __global__ __launch_bounds__(256) void k_route_combine_backward(CombineArgs a)
 template <typename TR, typename TO>
 static void combine_launch(const CombineArgs &a, hipStream_t st)
 {
-    const bool vec = a.N % 4 == 0 && (((uintptr_t)a.rows | (uintptr_t)a.out) & 15) == 0;
-    const long n = a.T * (vec ? a.N / 4 : a.N);
-    const dim3 grid((unsigned)((n + 255) / 256));
-    if (vec) hipLaunchKernelGGL((k_route_combine<TR, TO, 4>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_route_combine<TR, TO, 1>), grid, dim3(256), 0, st, a);
+    // 16 bytes of the narrower type a thread
+    constexpr int V = sizeof(TR) == 4 && sizeof(TO) == 4 ? 4 : 8;
+    const bool vec = a.N % V == 0 && (((uintptr_t)a.rows | (uintptr_t)a.out) & 15) == 0;
+    const int v = vec ? V : 1, per = (a.N + v - 1) / v;
+    const int tokens = per <= 128 ? 256 / per : 1;
+    const dim3 grid((unsigned)((a.T + tokens - 1) / tokens), tokens > 1 ? 1u : (unsigned)((per + 255) / 256));
+    if (vec) hipLaunchKernelGGL((k_route_combine<TR, TO, V>), grid, dim3(256), 0, st, a, per, tokens);
+    else hipLaunchKernelGGL((k_route_combine<TR, TO, 1>), grid, dim3(256), 0, st, a, per, tokens);
 }
 
 template <typename TR, typename TO>
 static void combine_back_launch(const CombineArgs &a, hipStream_t st)
 {
-    hipLaunchKernelGGL((k_route_combine_backward<TR, TO>), dim3((unsigned)((a.T * a.k + 3) / 4)), dim3(256), 0, st, a);
+    const dim3 grid((unsigned)((a.T * a.k + 3) / 4)), block(256);
+    if (a.N % 4 == 0 && (((uintptr_t)a.rows | (uintptr_t)a.dout) & 15) == 0)
+        hipLaunchKernelGGL((k_route_combine_backward<TR, TO, 4>), grid, block, 0, st, a);
+    else
+        hipLaunchKernelGGL((k_route_combine_backward<TR, TO, 1>), grid, block, 0, st, a);
 }
 
 #define COMBINE_TYPES(F, TR_CODE, TO_CODE)                                                                       \
@@ -1295,7 +1323,7 @@ extern "C" int skm_route_combine(void *ctx_, const void *rows, int rows_dtype, c
     SkmCtx *ctx = static_cast<SkmCtx *>(ctx_);
     SKM_REQUIRE(ctx && T >= 0 && k >= 1 && N >= 1 && (T == 0 || (rows && pos && weights && out)),
                 "skm_route_combine: bad argument");
-    SKM_REQUIRE(T * N < 0x7FFFFFFFL * 256, "skm_route_combine: too many elements");
+    SKM_REQUIRE(T <= 0x7FFFFFFF && (N + 255) / 256 <= 65535, "skm_route_combine: too many elements");
     if (T == 0) return SKM_OK;
     SkmDeviceGuard guard(ctx);
     hipStream_t st = (hipStream_t)stream;
