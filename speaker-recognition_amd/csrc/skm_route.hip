@@ -306,7 +306,8 @@ __device__ __forceinline__ void merge_down8(unsigned *a, const unsigned *b)
 //   largest; in each round the largest head of the row comes from four DPP steps, the lowest lane that holds it from a
 //   ballot, and that lane moves up.  A lane that has given all 8 leaves the row in doubt.
 //   The order itself is that of 64 bits.  Half-precision logits without a bias are exact in the key.  Otherwise one more
-//   than k is taken, neighbours are compared without the cut bits, and where two are not further apart than what float32
+//   than k is taken, groups that are as near on either side of the choice are settled by their float64 scores, neighbours
+//   are compared without the cut bits, and where two are not further apart than what float32
 //   arithmetic and (the last one taken and the first that was not) the cut bits can have moved them, the row's choices are
 //   ranked again by their float64 values -- for random logits about one row in a thousand.  Only where the one after that
 //   is as near, and for NaN and infinities, the whole wave does the row again in float64 (route_row): that costs 6 us at
@@ -314,7 +315,8 @@ __device__ __forceinline__ void merge_down8(unsigned *a, const unsigned *b)
 //   Error of p: exp of a difference d <= 0 by exp2(d log2 e): (3 |d| + 2) 2^-24 of it, |d| exp(d) <= 0.37; the sum S of E
 //   terms: (NV + 6) additions and the terms' errors, in all (NV + 48) 2^-24 / S bounds it; 1 / (1 + exp(-x)):
 //   p (1 - p) |x| <= 0.23 and an approximate reciprocal, 8 2^-24.  Error of c = p + bias: that and |c| 2^-24; of the key: |c| 2^-(23 - bits).
-template <typename T, int NV, int L>
+// GROUPED: with groups of experts (without, those take registers that the rows in flight need).
+template <typename T, int NV, int L, bool GROUPED>
 __global__ __launch_bounds__(256, NV <= 16 ? 4 : NV == 32 ? (L == 16 ? 3 : 2) : 1) void k_route(RouteArgs a)
 {
     constexpr int R = 64 / L, BITS = NV == 1 ? 0 : NV == 2 ? 1 : NV == 4 ? 2 : NV == 8 ? 3 : NV == 16 ? 4 : NV == 32 ? 5 : 6;
@@ -344,7 +346,7 @@ __global__ __launch_bounds__(256, NV <= 16 ? 4 : NV == 32 ? (L == 16 ? 3 : 2) : 
     }
     bad |= !a.sigmoid && top == inf;
     float total = 1.f, err = 0.f;
-    if (!a.sigmoid && (a.bias || a.groups > 1 || !a.renorm)) {
+    if (!a.sigmoid && (a.bias || GROUPED || !a.renorm)) {
         top = row_max<L>(top);
         total = 0.f;
 #pragma unroll
@@ -354,7 +356,7 @@ __global__ __launch_bounds__(256, NV <= 16 ? 4 : NV == 32 ? (L == 16 ? 3 : 2) : 
     } else if (a.sigmoid) {
         err = 8.f * 5.9604645e-8f;
     }
-    if (a.bias || a.groups > 1) {           // c becomes the probability, with the bias
+    if (a.bias || GROUPED) {                // c becomes the probability, with the bias
         const float inv = 1.f / total;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
@@ -372,7 +374,7 @@ __global__ __launch_bounds__(256, NV <= 16 ? 4 : NV == 32 ? (L == 16 ? 3 : 2) : 
         }
     }
     bool doubt = false;
-    if (a.groups > 1) {
+    if constexpr (GROUPED) {
         // the two largest c of a group in every lane of the row; lane g keeps those of group g
         const int per = a.E / a.groups;
         const unsigned inv = per > 1 ? (unsigned)(((1ull << 32) + per - 1) / per) : 0;
@@ -431,16 +433,93 @@ __global__ __launch_bounds__(256, NV <= 16 ? 4 : NV == 32 ? (L == 16 ? 3 : 2) : 
         float near = s1 == -inf ? 0.f : 4.f * err + 2.3841858e-7f * (fabsf(s1) + (pair ? fabsf(s2) : 0.f));
         near = row_max<L>(near);
         int ahead = 0;
-        for (int g = 0; g < a.groups; ++g) {
-            const float o = __shfl(score, sub * L + g);
-            ahead += (o > score || (o == score && g < l)) ? 1 : 0;
-        }
-        const bool kept = l < a.groups && ahead < a.group_k;
-        const unsigned long long all = __ballot(kept);
-        for (int g = 0; g < a.groups; ++g) {
-            const float o = __shfl(score, sub * L + g);
-            const bool ok = (all >> (sub * L + g)) & 1;
-            if (l < a.groups && ok != kept && (score != -inf || o != -inf)) bad |= fabsf(score - o) <= near;
+        bool kept;
+        unsigned long long all;
+        if (L == 16) {                      // the other groups' scores by turning the row's lanes
+#define ROUTE_TURNS(SEE)                                                                                              \
+    SEE(1) SEE(2) SEE(3) SEE(4) SEE(5) SEE(6) SEE(7) SEE(8) SEE(9) SEE(10) SEE(11) SEE(12) SEE(13) SEE(14) SEE(15)
+#define ROUTE_AHEAD(N)                                                                                                 \
+    {                                                                                                                  \
+        const float o = dpp_ror<0x120 + N>(score);                                                                     \
+        const int g = dpp_ror<0x120 + N>(l);                                                                           \
+        ahead += g < a.groups && (o > score || (o == score && g < l)) ? 1 : 0;                                         \
+    }
+            ROUTE_TURNS(ROUTE_AHEAD)
+            kept = l < a.groups && ahead < a.group_k;
+            bool open = false;              // near a group on the other side of the choice
+#define ROUTE_NEAR(N)                                                                                                  \
+    {                                                                                                                  \
+        const float o = dpp_ror<0x120 + N>(score);                                                                     \
+        const int g = dpp_ror<0x120 + N>(l);                                                                           \
+        open |= l < a.groups && g < a.groups && (dpp_ror<0x120 + N>((int)kept) != 0) != kept && fabsf(score - o) <= near; \
+    }
+            ROUTE_TURNS(ROUTE_NEAR)
+            const unsigned long long rows = __ballot(open);
+            if (rows) {                     // uniform: the open groups' scores in float64, the best of them for what is left
+                unsigned todo = (unsigned)((rows | rows >> 16 | rows >> 32 | rows >> 48) & 0xFFFFull);
+                double total64 = 1.0;
+                const double top64 = (double)top;
+                if (!a.sigmoid) {
+                    double t = 0.0;
+#pragma unroll 4
+                    for (int e = l; e < a.E; e += 16) t += exp((double)x[e] - top64);
+                    t = t + dpp_ror<0x128>(t);
+                    t = t + dpp_ror<0x124>(t);
+                    t = t + dpp_ror<0x122>(t);
+                    t = t + dpp_ror<0x121>(t);
+                    total64 = t;
+                }
+                const double dinf = __builtin_inf();
+                double best64 = -dinf;
+                while (todo) {
+                    const int g = __ffs((int)todo) - 1;
+                    todo &= todo - 1;
+                    double d1 = -dinf, d2 = -dinf;
+                    for (int e = g * per + l; e < (g + 1) * per; e += 16) {
+                        const double v = (double)x[e], b = a.bias ? (double)a.bias[e] : 0.0;
+                        const double p = a.sigmoid ? 1.0 / (1.0 + exp(-v)) : exp(v - top64) / total64;
+                        const double w = v == -dinf || b == -dinf ? -dinf : p + b;
+                        d2 = fmax(d2, fmin(d1, w));
+                        d1 = fmax(d1, w);
+                    }
+#define ROUTE_TOP2(CTRL)                                              \
+    {                                                                 \
+        const double o1 = dpp_ror<CTRL>(d1), o2 = dpp_ror<CTRL>(d2);  \
+        d2 = fmax(fmax(d2, o2), fmin(d1, o1));                        \
+        d1 = fmax(d1, o1);                                            \
+    }
+                    ROUTE_TOP2(0x128) ROUTE_TOP2(0x124) ROUTE_TOP2(0x122) ROUTE_TOP2(0x121)
+#undef ROUTE_TOP2
+                    if (l == g) best64 = a.group_top == 2 && d2 != -dinf ? d1 + d2 : d1;
+                }
+                int settled = 0, before = 0;
+#define ROUTE_SETTLE(N)                                                                                                \
+    {                                                                                                                  \
+        const double o = dpp_ror<0x120 + N>(best64);                                                                   \
+        const int g = dpp_ror<0x120 + N>(l);                                                                           \
+        const bool oopen = dpp_ror<0x120 + N>((int)open) != 0, okept = dpp_ror<0x120 + N>((int)kept) != 0;             \
+        settled += okept && !oopen ? 1 : 0;                                                                            \
+        before += oopen && (o > best64 || (o == best64 && g < l)) ? 1 : 0;                                             \
+    }
+                ROUTE_TURNS(ROUTE_SETTLE)
+                if (open) kept = before < a.group_k - settled;
+            }
+#undef ROUTE_TURNS
+#undef ROUTE_AHEAD
+#undef ROUTE_NEAR
+#undef ROUTE_SETTLE
+            all = __ballot(kept);
+        } else {
+            for (int g = 0; g < a.groups; ++g) {
+                const float o = __shfl(score, g);
+                ahead += (o > score || (o == score && g < l)) ? 1 : 0;
+            }
+            kept = l < a.groups && ahead < a.group_k;
+            all = __ballot(kept);
+            for (int g = 0; g < a.groups; ++g) {
+                const float o = __shfl(score, g);
+                bad |= l < a.groups && (((all >> g) & 1) != 0) != kept && fabsf(score - o) <= near;
+            }
         }
         const unsigned long long stay = L == 64 ? all : (all >> (sub * L)) & 0xFFFFull;
 #pragma unroll
@@ -839,7 +918,14 @@ template <typename T, int NV, int L>
 static void route_go(const RouteArgs &a, hipStream_t st)
 {
     const long per = 4 * (64 / L);
-    hipLaunchKernelGGL((k_route<T, NV, L>), dim3((unsigned)((a.T + per - 1) / per)), dim3(256), 0, st, a);
+    const dim3 grid((unsigned)((a.T + per - 1) / per)), block(256);
+    if constexpr (sizeof(T) < 8) {
+        if (a.groups > 1) {
+            hipLaunchKernelGGL((k_route<T, NV, L, true>), grid, block, 0, st, a);
+            return;
+        }
+    }
+    hipLaunchKernelGGL((k_route<T, NV, L, false>), grid, block, 0, st, a);
 }
 
 template <typename T, int NV>
