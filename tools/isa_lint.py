@@ -10,10 +10,10 @@ and checks, per kernel, linearly over the instruction stream:
         later MFMA that reads it as SrcA / SrcB (or as a SrcC that is not the very same tuple), fewer than W wait states
         behind it.  W as in LLVM's GCNHazardRecognizer for gfx940 / gfx950: passes + 2 for the float32 MFMAs
         (32x32x2: 18, 16x16x4: 10), 11 for the float64 16x16x4 (18 when a store reads it), passes + 4 for the
-        bf16 32x32x16 (12).
+        bf16 32x32x16 (12) and the 8-bit 16x16x128 (12) and 32x32x64 (20).
   (ii)  VALU write -> MFMA read.  A vector-ALU instruction (v_accvgpr_write / v_mov included) that writes a register an
         MFMA reads fewer than 2 wait states later.
-  (iii) LDS-direct loads.  `buffer_load ... lds` whose data a `ds_read` of the NEXT loop iteration (or, outside a loop,
+  (iii) LDS-direct loads.  `buffer_load ... lds` (or `global_load_lds_*`) whose data a `ds_read` of the NEXT loop iteration (or, outside a loop,
         any later `ds_read`) can reach before an `s_waitcnt vmcnt(n)` that covers the load: hipcc emits no such wait
         for this load kind.  (A `ds_read` in the SAME iteration belongs to the other buffer of the ring by design.)
         Kernels listed in RING_DEPTH keep their loads in flight longer -- a ring of three LDS stages filled two
@@ -48,6 +48,8 @@ MFMA_WAIT = [
     (re.compile(r"^v_mfma_f64_4x4x4"), 6, 9),
     (re.compile(r"^v_mfma_f32_32x32x16_"), 12, 12),
     (re.compile(r"^v_mfma_f32_16x16x32_"), 8, 8),
+    (re.compile(r"^v_mfma_(scale_)?f32_16x16x128_"), 12, 12),      # 8 passes with 8-bit operands
+    (re.compile(r"^v_mfma_(scale_)?f32_32x32x64_"), 20, 20),       # 16 passes
     (re.compile(r"^v_mfma_"), 19, 19),          # anything else: the longest XDL case
 ]
 # passes (4 clocks each) the matrix pipe is busy with one instruction
@@ -56,11 +58,14 @@ MFMA_PASSES = [
     (re.compile(r"^v_mfma_f32_16x16x4_?f32"), 8),
     (re.compile(r"^v_mfma_f64_16x16x4_?f64"), 8),
     (re.compile(r"^v_mfma_f32_32x32x16_"), 8),
+    (re.compile(r"^v_mfma_(scale_)?f32_32x32x64_"), 16),
 ]
 STRICT = False
 # LDS-direct loads: iterations between a load and the first ds_read of its data (default 1: a ring of two buffers)
 RING_DEPTH = [
     (re.compile(r"k_gemm_b3"), 2),      # csrc/skm_gemm_b3.hip: three stages, loads issued two stages ahead, vmcnt(6)
+    (re.compile(r"k_gemm_fp8I"), 2),    # csrc/skm_fp8.hip: two stages; half of a stage is read in front of the wait
+    (re.compile(r"k_gemm_fp8ILi4ELi2"), 3),     # 256 x 128 tiles: three stages, vmcnt(14)
 ]
 REG = re.compile(r"\b([va])(?:(\d+)|\[(\d+):(\d+)\])(?![\w\[])")
 LINE = re.compile(r"^\s+(\S+)\s*(.*?)\s*//\s*([0-9A-Fa-f]+):")
@@ -98,7 +103,7 @@ class Ins(object):
         self.is_mfma = op.startswith("v_mfma") or op.startswith("v_smfma")
         self.is_valu = op.startswith("v_") and not self.is_mfma
         self.vmem = op.startswith(("buffer_", "global_", "flat_", "scratch_"))
-        self.lds_direct = self.vmem and "load" in op and re.search(r"\blds\b", args) is not None
+        self.lds_direct = self.vmem and "load" in op and ("load_lds" in op or re.search(r"\blds\b", args) is not None)
         self.is_store = ("store" in op) or op.startswith("ds_write") or op.startswith("ds_store")
 
 
