@@ -805,7 +805,10 @@ __global__ __launch_bounds__(512, 2) void k_gemm_fp8_rows16(Fp8Args g, Fp8Float 
 {
     constexpr bool FLOAT = sizeof(XT) > 1;
     static_assert(!FLOAT || MT == 1, "float rows are quantized for one row tile");
-    __shared__ __align__(16) float part[8][FLOAT && MT * NT * 4 < 33 ? 33 : MT * NT * 4][64];    // also 8 KB + 64 bytes a wave
+    // a wave's part of the sums; with float rows also 8 KB + 64 bytes of them.  As many as there are waves: a fixed eight
+    // would leave room for two workgroups on a CU where four waves are enough for k
+    constexpr int PART = (FLOAT && MT * NT * 4 < 33 ? 33 : MT * NT * 4) * 64;
+    extern __shared__ __align__(16) float lds[];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
     const int r = lane & 15, q4 = lane >> 4;
     int rows = g.M;
@@ -846,7 +849,7 @@ __global__ __launch_bounds__(512, 2) void k_gemm_fp8_rows16(Fp8Args g, Fp8Float 
         for (int j = 0; j < NT; ++j)
 #pragma unroll
             for (int q = 0; q < 4; ++q) acc[i][j][q] = 0.f;
-    uint8_t *lw = reinterpret_cast<uint8_t *>(part[wave]);
+    uint8_t *lw = reinterpret_cast<uint8_t *>(lds + wave * PART);
     uint8_t *ls = lw + 16 * 512;            // scales [16][4]
 
     const int groups = (g.kb1 + 3) / 4;
@@ -936,16 +939,16 @@ __global__ __launch_bounds__(512, 2) void k_gemm_fp8_rows16(Fp8Args g, Fp8Float 
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) part[wave][(i * NT + j) * 4 + q][lane] = acc[i][j][q];
+            for (int q = 0; q < 4; ++q) lds[wave * PART + ((i * NT + j) * 4 + q) * 64 + lane] = acc[i][j][q];
     __syncthreads();
     // one wave per 16 x 16 tile of the result, in turn
     for (int t = wave; t < MT * NT; t += waves) {
         float v[4];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) v[q] = part[0][t * 4 + q][lane];
+        for (int q = 0; q < 4; ++q) v[q] = lds[(t * 4 + q) * 64 + lane];
         for (int w = 1; w < waves; ++w)
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] += part[w][t * 4 + q][lane];
+            for (int q = 0; q < 4; ++q) v[q] += lds[w * PART + (t * 4 + q) * 64 + lane];
         const int m = t / NT * 16 + r, n = col0 + t % NT * 16 + 4 * q4;
         if (m >= rows) continue;
         TO *c = static_cast<TO *>(g.C) + (row0 + m) * g.ldc + n;
@@ -960,11 +963,12 @@ static void rows16_launch(const Fp8Args &g, const Fp8Float &fx, int fa, int fb, 
 {
     const int groups = (g.kb1 + 3) / 4;
     const dim3 grid((unsigned)((g.N + 16 * NT - 1) / (16 * NT)), gy), block(64u * (groups < 8 ? groups : 8));
+    const size_t lds = (block.x / 64) * (sizeof(XT) > 1 && MT * NT * 4 < 33 ? 33 : MT * NT * 4) * 256;
     switch (fa * 2 + fb) {
-    case 0: hipLaunchKernelGGL((k_gemm_fp8_rows16<MT, NT, 0, 0, TO, XT>), grid, block, 0, st, g, fx); break;
-    case 1: hipLaunchKernelGGL((k_gemm_fp8_rows16<MT, NT, 0, 1, TO, XT>), grid, block, 0, st, g, fx); break;
-    case 2: hipLaunchKernelGGL((k_gemm_fp8_rows16<MT, NT, 1, 0, TO, XT>), grid, block, 0, st, g, fx); break;
-    default: hipLaunchKernelGGL((k_gemm_fp8_rows16<MT, NT, 1, 1, TO, XT>), grid, block, 0, st, g, fx); break;
+    case 0: hipLaunchKernelGGL((k_gemm_fp8_rows16<MT, NT, 0, 0, TO, XT>), grid, block, lds, st, g, fx); break;
+    case 1: hipLaunchKernelGGL((k_gemm_fp8_rows16<MT, NT, 0, 1, TO, XT>), grid, block, lds, st, g, fx); break;
+    case 2: hipLaunchKernelGGL((k_gemm_fp8_rows16<MT, NT, 1, 0, TO, XT>), grid, block, lds, st, g, fx); break;
+    default: hipLaunchKernelGGL((k_gemm_fp8_rows16<MT, NT, 1, 1, TO, XT>), grid, block, lds, st, g, fx); break;
     }
 }
 

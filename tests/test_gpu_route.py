@@ -200,7 +200,8 @@ def test_route_backward_against_differences(eng):
 
 
 @pytest.mark.parametrize("T,k,E", [(1, 1, 1), (1, 4, 64), (0, 2, 5), (9, 3, 5), (700, 6, 64), (1025, 4, 4), (3000, 8, 130),
-                                   (40000, 2, 16), (5000, 3, 4096), (300, 2, 2500), (70001, 8, 257)])
+                                   (40000, 2, 16), (30001, 2, 512), (20000, 3, 600), (65536, 1, 3), (65537, 1, 3),
+                                   (5000, 3, 4096), (300, 2, 2500), (70001, 8, 257)])
 def test_plan(eng, T, k, E):
     r = np.random.RandomState(T + E)
     ids = r.randint(-1, E, (T, k)).astype(np.int32)
