@@ -57,12 +57,13 @@ __device__ __forceinline__ unsigned fp8_pack4(float a, float b, float c, float d
     return (unsigned)__builtin_amdgcn_cvt_pk_bf8_f32(c, d, lo, true);
 }
 
+// n numbers from p on, 8 at most, zeros behind them
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, bool vec, int n, float (&v)[8])
+__device__ __forceinline__ void load8(const T *p, int n, float (&v)[8])
 {
     typedef T v8 __attribute__((ext_vector_type(8)));
-    if (vec && n >= 8) {
-        const v8 x = *reinterpret_cast<const v8 *>(p);
+    if (n >= 8) {
+        const v8 x = load_any<v8>(p);
 #pragma unroll
         for (int q = 0; q < 8; ++q) v[q] = (float)x[q];
     } else {
@@ -75,7 +76,6 @@ struct RowsArgs {
     const void *x;
     long M, ldx;
     int K, KB, S;           // blocks of a row, scale bytes of a row
-    int vec;                // 16-byte loads are allowed
     uint8_t *q, *s;
 };
 
@@ -98,7 +98,7 @@ __global__ __launch_bounds__(256) void k_fp8_rows(RowsArgs a)
     if (row >= a.M) return;                 // whole blocks of 16 lanes
     const int k = kb * FP8_BLOCK + l * 8;
     float v[8];
-    load8(static_cast<const T *>(a.x) + row * a.ldx + k, a.vec, a.K - k, v);
+    load8(static_cast<const T *>(a.x) + row * a.ldx + k, a.K - k, v);
     float top = 0.f;
 #pragma unroll
     for (int q = 0; q < 8; ++q) top = fmaxf(top, fp8_finite_abs(v[q]));
@@ -120,7 +120,6 @@ struct TileArgs {
     const void *x;
     long R, ldx, sx;        // rows, their stride, distance between matrices
     int C;                  // columns
-    int vec;
     uint8_t *q, *s;         // [z][R][Cp], [z][R][Sc]              (tiles only)
     uint8_t *qt, *st;       // [z][C][Rp], [z][C][Sr]              NULL: not wanted
     long Cp, Rp;
@@ -161,7 +160,7 @@ __global__ __launch_bounds__(256) void k_fp8_tiles(TileArgs a)
                 src = pr / a.slots;
                 if (a.w) w = a.w[pr];
             }
-            load8(x + src * a.ldx + c, a.vec, a.C - c, v[i]);
+            load8(x + src * a.ldx + c, a.C - c, v[i]);
             if (COLS && a.w)
 #pragma unroll
                 for (int q = 0; q < 8; ++q) v[i][q] *= w;
@@ -247,8 +246,6 @@ __global__ __launch_bounds__(256) void k_fp8_tiles(TileArgs a)
     }
 }
 
-static bool aligned16(const void *p, long ld_bytes) { return ((uintptr_t)p & 15) == 0 && ld_bytes % 16 == 0; }
-
 #define FP8_IN_TYPES(F, ...)                                                             \
     switch (dtype * 2 + fmt) {                                                           \
     case SKM_DT_F32 * 2 + SKM_FP8_E4M3: F(float, SKM_FP8_E4M3, ##__VA_ARGS__); break;    \
@@ -273,8 +270,8 @@ extern "C" int skm_fp8_rows(void *ctx_, const void *x, int dtype, long M, int K,
     SKM_REQUIRE(ctx && M >= 0 && K >= 1 && ldx >= K && (M == 0 || (x && q && s)), "skm_fp8_rows: bad argument");
     if (int rc = fp8_check_types("skm_fp8_rows", dtype, fmt)) return rc;
     if (M == 0) return SKM_OK;
-    RowsArgs a{x, M, ldx, K, (int)(fp8_kpad(K) / FP8_BLOCK), (int)fp8_sstride(K),
-               aligned16(x, ldx * skm_dt_size(dtype)), static_cast<uint8_t *>(q), static_cast<uint8_t *>(s)};
+    RowsArgs a{x, M, ldx, K, (int)(fp8_kpad(K) / FP8_BLOCK), (int)fp8_sstride(K), static_cast<uint8_t *>(q),
+               static_cast<uint8_t *>(s)};
     const long grid = (M * a.KB + 15) / 16;
     SKM_REQUIRE(grid <= 0x7FFFFFFF, "skm_fp8_rows: too many blocks");
     SkmDeviceGuard guard(ctx);
@@ -297,7 +294,6 @@ extern "C" int skm_fp8_tiles(void *ctx_, const void *w, int dtype, int batch, in
     SKM_REQUIRE(batch <= 65535 && fp8_kpad(N) / FP8_BLOCK <= 65535, "skm_fp8_tiles: too large");
     TileArgs a{};
     a.x = w; a.R = N; a.ldx = ldw; a.sx = sw; a.C = K;
-    a.vec = aligned16(w, ldw * skm_dt_size(dtype)) && (sw * skm_dt_size(dtype)) % 16 == 0;
     a.q = static_cast<uint8_t *>(q); a.s = static_cast<uint8_t *>(s);
     a.qt = static_cast<uint8_t *>(qt); a.st = static_cast<uint8_t *>(st_);
     a.Cp = fp8_kpad(K); a.Rp = fp8_kpad(N); a.Sc = (int)fp8_sstride(K); a.Sr = (int)fp8_sstride(N);
@@ -326,7 +322,6 @@ extern "C" int skm_fp8_columns(void *ctx_, const void *x, int dtype, long R, int
     SKM_REQUIRE(blocks <= 65535, "skm_fp8_columns: more than 65535 blocks of rows");
     TileArgs a{};
     a.x = x; a.R = R; a.ldx = ldx; a.C = C;
-    a.vec = aligned16(x, ldx * skm_dt_size(dtype));
     a.qt = static_cast<uint8_t *>(qt); a.st = static_cast<uint8_t *>(st_);
     a.Rp = blocks * FP8_BLOCK; a.Sr = (int)fp8_sstride(a.Rp);
     a.tiles = tiles; a.count = tile_count; a.pair = tiles ? pair : nullptr; a.slots = slots; a.w = weights;
@@ -351,7 +346,6 @@ struct Fp8Args {
     void *C;
     long ldc;
     int accumulate;
-    int c_vec;              // C takes 16-byte stores
     int c_bf16;             // (host) C's type
     int tile_rows;          // (host) rows of a plan's tile
     long mean_blocks;       // (host) blocks of an expert on average
@@ -723,7 +717,6 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
     static_assert(sizeof(sh) >= 4 * 32 * PITCH * sizeof(float), "the result's rows fit where the stages were");
     float *lw = reinterpret_cast<float *>(sh) + wave * 32 * PITCH;
     typedef TO vo __attribute__((ext_vector_type(VE)));
-    const bool vec = g.c_vec;
     __syncthreads();                        // the other waves have read their last stage
     const int sr = lane / PER, scol = (lane % PER) * VE, gc = wn * CW + scol;
     // cols - gc columns from here on: VE of them or fewer
@@ -748,16 +741,16 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
             }
             if (rr < rows && gc < cols) {
                 TO *d = C + (row0 + rr) * g.ldc + col0 + gc;
-                if (vec && gc + VE <= cols) {
+                if (gc + VE <= cols) {
                     vo o;
                     if (g.accumulate) {
-                        o = *reinterpret_cast<const vo *>(d);
+                        o = load_any<vo>(d);
 #pragma unroll
                         for (int q = 0; q < VE; ++q) v[q] += (float)o[q];
                     }
 #pragma unroll
                     for (int q = 0; q < VE; ++q) o[q] = (TO)v[q];
-                    *reinterpret_cast<vo *>(d) = o;
+                    store_any(d, o);
                 } else {
 #pragma unroll
                     for (int q = 0; q < VE; ++q)
@@ -787,7 +780,6 @@ struct Fp8Float {
     const void *x;
     long ldx;
     int K;
-    int vec;                // 16-byte loads are allowed
 };
 
 // C = A B' for up to 16 MT rows of A (or tiles of up to 16 rows of an expert): the bytes of B are what counts, each is
@@ -882,7 +874,7 @@ __global__ __launch_bounds__(512, 2) void k_gemm_fp8_rows16(Fp8Args g, Fp8Float 
             for (int m = 0; m < rows; ++m) {
                 const XT *x = static_cast<const XT *>(fx.x) + (long)__builtin_amdgcn_readlane(src_row, m) * fx.ldx;
                 float v[8];
-                load8(x + k, fx.vec, fx.K - k, v);
+                load8(x + k, fx.K - k, v);
                 float top = 0.f;
 #pragma unroll
                 for (int q = 0; q < 8; ++q) top = fmaxf(top, fp8_finite_abs(v[q]));
@@ -1053,8 +1045,6 @@ static int fp8_run(SkmCtx *ctx, Fp8Args g, int fa, int fb, int dtype, unsigned g
     }
     if (!g.tiles) g.tiles_m = (g.M + bm - 1) / bm;
     g.tiles_n = (g.N + bn - 1) / bn;
-    const int esize = skm_dt_size(dtype);
-    g.c_vec = aligned16(g.C, g.ldc * esize) && (g.eC * esize) % 16 == 0 && (g.zC * esize) % 16 == 0;
     // a lane's offset inside a tile (by plan: inside A) is 32 bits wide
     const long reach = g.tiles && g.slots ? g.rowsA : 256;
     if (reach * g.lda > 0xFFFFFFFFL || reach * g.SA > 0x7FFFFFFFL || 256 * g.ldb > 0xFFFFFFFFL) {
@@ -1141,7 +1131,7 @@ static int fp8_take_a(SkmCtx *ctx, const char *who, const void *&q, const void *
     if (int rc = fp8_check_types(who, a_dtype, fmt_a)) return rc;
     SKM_REQUIRE(q && lda >= K, "%s: A is missing or its rows overlap", who);
     if (on_the_way) {
-        *fx = Fp8Float{q, lda, K, aligned16(q, lda * skm_dt_size(a_dtype))};
+        *fx = Fp8Float{q, lda, K};
         q = s = nullptr;
         return SKM_OK;
     }

@@ -25,6 +25,21 @@ struct SkmDeviceGuard {
     }
 };
 
+// 16 bytes and the like at any address that a T may have: global memory takes unaligned vector accesses, one instruction
+// where a loop over the elements is one each
+template <typename V, typename T>
+__device__ __forceinline__ V load_any(const T *p)
+{
+    V v;
+    __builtin_memcpy(&v, p, sizeof(V));
+    return v;
+}
+template <typename V, typename T>
+__device__ __forceinline__ void store_any(T *p, const V &v)
+{
+    __builtin_memcpy(p, &v, sizeof(V));
+}
+
 template <typename T>
 __device__ __forceinline__ T wave_max(T v)
 {

@@ -781,7 +781,7 @@ __global__ __launch_bounds__(256) void k_route_backward(RouteBackArgs a)
 // row in LDS (places with the same expert are added first, in their order, by the first of them), so that the row leaves
 // in 16-byte stores; a wave per row with a comparison per place and element took twice as long.
 template <typename T, int EMAX>
-__global__ __launch_bounds__(256) void k_route_backward16(RouteBackArgs a, int vec)
+__global__ __launch_bounds__(256) void k_route_backward16(RouteBackArgs a)
 {
     constexpr int PL = ROUTE_MAX_K / 16, V = 16 / sizeof(T);
     __shared__ float buf[16][EMAX + 4];
@@ -891,11 +891,11 @@ __global__ __launch_bounds__(256) void k_route_backward16(RouteBackArgs a, int v
             for (int q = 0; q < V; ++q)
                 if (e + q < a.E) v[q] -= D * expf((float)x[e + q] - top) / total;
         }
-        if (vec) {
+        if (e + V <= a.E) {
             vt o;
 #pragma unroll
             for (int q = 0; q < V; ++q) o[q] = (T)v[q];
-            *reinterpret_cast<vt *>(dx + e) = o;
+            store_any(dx + e, o);
         } else {
 #pragma unroll
             for (int q = 0; q < V; ++q)
@@ -907,10 +907,9 @@ __global__ __launch_bounds__(256) void k_route_backward16(RouteBackArgs a, int v
 template <typename T>
 static void route_back_go(const RouteBackArgs &a, hipStream_t st)
 {
-    const bool vec = ((uintptr_t)a.dx & 15) == 0 && (a.E * sizeof(T)) % 16 == 0;
     const dim3 grid((unsigned)((a.T + 15) / 16)), block(256);
-    if (a.E <= 128) hipLaunchKernelGGL((k_route_backward16<T, 128>), grid, block, 0, st, a, (int)vec);
-    else if (a.E <= 512) hipLaunchKernelGGL((k_route_backward16<T, 512>), grid, block, 0, st, a, (int)vec);
+    if (a.E <= 128) hipLaunchKernelGGL((k_route_backward16<T, 128>), grid, block, 0, st, a);
+    else if (a.E <= 512) hipLaunchKernelGGL((k_route_backward16<T, 512>), grid, block, 0, st, a);
     else hipLaunchKernelGGL((k_route_backward<T, float>), dim3((unsigned)((a.T + 3) / 4)), block, 0, st, a);
 }
 
@@ -1315,6 +1314,15 @@ __global__ __launch_bounds__(256) void k_route_combine(CombineArgs a, int per, i
     const int32_t *pos = a.pos + t * a.k;
     const float *w = a.w + t * a.k;
     const TR *rows = static_cast<const TR *>(a.rows) + c;
+    TO *out = static_cast<TO *>(a.out) + t * a.N + c;
+    if (c + VEC > a.N) {                    // the end of a row
+        for (int q = 0; c + q < a.N; ++q) {
+            float s = 0.f;
+            for (int j = 0; j < a.k; ++j) s += w[j] * (pos[j] >= 0 ? (float)rows[(long)pos[j] * a.N + q] : 0.f);
+            out[q] = (TO)s;
+        }
+        return;
+    }
     float s[VEC];
 #pragma unroll
     for (int q = 0; q < VEC; ++q) s[q] = 0.f;
@@ -1327,7 +1335,7 @@ __global__ __launch_bounds__(256) void k_route_combine(CombineArgs a, int per, i
             f[u] = j0 + u < a.k ? w[j0 + u] : 0.f;
 #pragma unroll
             for (int q = 0; q < VEC; ++q) v[u][q] = (TR)0.f;
-            if (p >= 0) v[u] = *reinterpret_cast<const vr *>(rows + (long)p * a.N);
+            if (p >= 0) v[u] = load_any<vr>(rows + (long)p * a.N);
         }
 #pragma unroll
         for (int u = 0; u < 4; ++u)
@@ -1337,13 +1345,14 @@ __global__ __launch_bounds__(256) void k_route_combine(CombineArgs a, int per, i
     vo o;
 #pragma unroll
     for (int q = 0; q < VEC; ++q) o[q] = (TO)s[q];
-    *reinterpret_cast<vo *>(static_cast<TO *>(a.out) + t * a.N + c) = o;
+    store_any(out, o);
 }
 
 // dw[t][j] = <dout[t], rows[pos[t][j]]>: one wave per pair
-template <typename TR, typename TO, int VEC>
+template <typename TR, typename TO>
 __global__ __launch_bounds__(256) void k_route_combine_backward(CombineArgs a)
 {
+    constexpr int VEC = 4;
     typedef TR vr __attribute__((ext_vector_type(VEC)));
     typedef TO vo __attribute__((ext_vector_type(VEC)));
     const int lane = threadIdx.x & 63;
@@ -1357,13 +1366,15 @@ __global__ __launch_bounds__(256) void k_route_combine_backward(CombineArgs a)
         float part[VEC];
 #pragma unroll
         for (int q = 0; q < VEC; ++q) part[q] = 0.f;
+        const int whole = a.N / VEC * VEC;
 #pragma unroll 4
-        for (int c = lane * VEC; c < a.N; c += 64 * VEC) {
-            const vr x = *reinterpret_cast<const vr *>(r + c);
-            const vo y = *reinterpret_cast<const vo *>(d + c);
+        for (int c = lane * VEC; c < whole; c += 64 * VEC) {
+            const vr x = load_any<vr>(r + c);
+            const vo y = load_any<vo>(d + c);
 #pragma unroll
             for (int q = 0; q < VEC; ++q) part[q] += (float)x[q] * (float)y[q];
         }
+        if (whole + lane < a.N) s = (float)r[whole + lane] * (float)d[whole + lane];
 #pragma unroll
         for (int q = 0; q < VEC; ++q) s += part[q];
         s = wave_sum(s);
@@ -1376,22 +1387,15 @@ static void combine_launch(const CombineArgs &a, hipStream_t st)
 {
     // 16 bytes of the narrower type a thread
     constexpr int V = sizeof(TR) == 4 && sizeof(TO) == 4 ? 4 : 8;
-    const bool vec = a.N % V == 0 && (((uintptr_t)a.rows | (uintptr_t)a.out) & 15) == 0;
-    const int v = vec ? V : 1, per = (a.N + v - 1) / v;
-    const int tokens = per <= 128 ? 256 / per : 1;
+    const int per = (a.N + V - 1) / V, tokens = per <= 128 ? 256 / per : 1;
     const dim3 grid((unsigned)((a.T + tokens - 1) / tokens), tokens > 1 ? 1u : (unsigned)((per + 255) / 256));
-    if (vec) hipLaunchKernelGGL((k_route_combine<TR, TO, V>), grid, dim3(256), 0, st, a, per, tokens);
-    else hipLaunchKernelGGL((k_route_combine<TR, TO, 1>), grid, dim3(256), 0, st, a, per, tokens);
+    hipLaunchKernelGGL((k_route_combine<TR, TO, V>), grid, dim3(256), 0, st, a, per, tokens);
 }
 
 template <typename TR, typename TO>
 static void combine_back_launch(const CombineArgs &a, hipStream_t st)
 {
-    const dim3 grid((unsigned)((a.T * a.k + 3) / 4)), block(256);
-    if (a.N % 4 == 0 && (((uintptr_t)a.rows | (uintptr_t)a.dout) & 15) == 0)
-        hipLaunchKernelGGL((k_route_combine_backward<TR, TO, 4>), grid, block, 0, st, a);
-    else
-        hipLaunchKernelGGL((k_route_combine_backward<TR, TO, 1>), grid, block, 0, st, a);
+    hipLaunchKernelGGL((k_route_combine_backward<TR, TO>), dim3((unsigned)((a.T * a.k + 3) / 4)), dim3(256), 0, st, a);
 }
 
 #define COMBINE_TYPES(F, TR_CODE, TO_CODE)                                                                       \
