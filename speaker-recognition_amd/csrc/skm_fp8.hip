@@ -87,7 +87,8 @@ __device__ __forceinline__ float lanes16_ror(float v)
     return __int_as_float(__builtin_amdgcn_update_dpp(i, i, CTRL, 0xF, 0xF, false));
 }
 
-// blocks of 1 x 128: 16 lanes per block, 8 numbers a lane
+// Blocks of 1 x 128: 16 lanes per block, 8 numbers a lane, the block's largest by four DPP steps; no LDS, no barrier.
+// Bound by memory: 8192 x 4096 bf16 in 19.4 us, 5.2 TB/s (a large copy: 5.0); rows at odd addresses (4095) 22.8 us.
 template <typename T, int FMT>
 __global__ __launch_bounds__(256) void k_fp8_rows(RowsArgs a)
 {
@@ -131,7 +132,9 @@ struct TileArgs {
 };
 
 // blocks of 128 x 128 (COLS = 0) or 128 x 1 (COLS = 1): one workgroup per 128 x 128; a thread holds 8 columns of 8
-// consecutive rows, so that a transposed block goes through LDS in 8-byte pieces
+// consecutive rows, so that a transposed block goes through LDS in 8-byte pieces.  One read of x serves both results of
+// weights.  Bound by memory: 8192 x 4096 bf16 tiles 21.9 us (4.6 TB/s), tiles and their transpose 26.5 us (5.1), columns
+// 21.9 us (4.6); rows at odd addresses (4095) 41-46 us, an 8-byte piece then lies in two cache lines more often.
 template <typename T, int FMT, int COLS>
 __global__ __launch_bounds__(256) void k_fp8_tiles(TileArgs a)
 {
@@ -411,6 +414,11 @@ typedef __attribute__((address_space(1))) const void *glb_ptr;
 //   read half 0 of s + 1; multiply half 1
 // so a load has DEPTH - 1/2 stages to arrive, an LDS read half a stage, and the barrier stands among multiplications
 // that are under way already.
+// Why 256 x 256: a stage's 64 KB of LDS reads (128 x 128: 32 KB a quarter of the products) fit under its multiplications,
+// and every operand byte is loaded half as often.
+// Measured: 8192 x 8192 x 8192 to bf16 471 us, 2335 TFLOP/s (matrix pipe busy 62 % of the cycles at 1.95 GHz: the engine
+// clock gives way to power on random operands); 4096 x 8192 x 4096 at 2600.  To float32 887 us, 1240 TFLOP/s (60 %, 1.92
+// GHz), as fast as a plain bf16 product of the size on this GPU (1241).
 template <int MT, int NT, int FA, int FB, typename TO>
 __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args g)
 {
@@ -729,7 +737,7 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
                 const f32x4 v = {acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
                 *reinterpret_cast<f32x4 *>(lw + r * PITCH + j * 32 + 8 * q + 4 * h) = v;
             }
-        __builtin_amdgcn_wave_barrier();    // a wave's LDS instructions are carried out in order
+        wave_sync();
 #pragma unroll
         for (int t = 0; t < 32 / RSTEP; ++t) {
             const int lrow = t * RSTEP + sr, rr = (wm * MT + i) * 32 + lrow;
@@ -758,7 +766,7 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
                 }
             }
         }
-        __builtin_amdgcn_wave_barrier();
+        wave_sync();
     }
 }
 
@@ -792,6 +800,8 @@ struct Fp8Float {
 // k_fp8_rows does it (16 lanes a block, so one row's four blocks at a time), into LDS -- the same work in every workgroup,
 // under the latency of B's bytes, costs less than a launch before this one.  LDS: a row's 512 bytes, the 16-byte pieces of
 // each 256 exchanged by the row, so that the 16 rows that read the same piece meet different banks.
+// Bound by the bytes of B and, for one row, by the launch: 1 x 4096 x 4096 6.7 us, 64 x 8192 x 4096 18.5 us, 8 tokens of 4
+// places over 64 experts of 2048 x 2048 24 us (about 105 MB, 4.4 TB/s).
 template <int MT, int NT, int FA, int FB, typename TO, typename XT>
 __global__ __launch_bounds__(512, 2) void k_gemm_fp8_rows16(Fp8Args g, Fp8Float fx)
 {
@@ -890,7 +900,7 @@ __global__ __launch_bounds__(512, 2) void k_gemm_fp8_rows16(Fp8Args g, Fp8Float 
                 *reinterpret_cast<uint2 *>(lw + m * 512 + line + (piece ^ m) * 16 + (r & 1) * 8) = o;
                 if (r == 0) ls[m * 4 + q4] = (uint8_t)(e + 127);
             }
-            __builtin_amdgcn_wave_barrier();            // a wave's LDS instructions are carried out in order
+            wave_sync();
             sx[0] = *reinterpret_cast<const int *>(ls + r * 4);
 #pragma unroll
             for (int b = 0; b < 4; ++b) {               // rows behind the last: whatever is there, for columns not stored
@@ -899,7 +909,7 @@ __global__ __launch_bounds__(512, 2) void k_gemm_fp8_rows16(Fp8Args g, Fp8Float 
                 const i32x4 hi = *reinterpret_cast<const i32x4 *>(p + (((b & 1) * 8 + 4 + q4) ^ r) * 16);
                 a[0][b] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
             }
-            __builtin_amdgcn_wave_barrier();
+            wave_sync();
         }
 #undef ROWS16_LOAD
 #pragma unroll
@@ -983,7 +993,7 @@ static int rows16_run(SkmCtx *ctx, const Fp8Args &g, const Fp8Float &fx, int x_d
     SkmProfScope ps(ctx, "k_gemm_fp8_rows16", st);
     if (g.A) {
         // two column tiles a workgroup (A's rows are read once per workgroup) where they are enough for every CU:
-        // 61 x 8192 x 4096 18.5 us against 27.8, 61 x 4096 x 4096 16.7 against 14.5
+        // 64 x 8192 x 4096 18.5 us against 27.8, 64 x 4096 x 4096 16.7 against 14.5
         const bool two = (g.N + 31) / 32 >= ctx->cu_count;
         if (g.M > 32 && !g.tiles)
             return two ? rows16_types<4, 2, uint8_t>(g, fx, fa, fb, dtype, gy, st) : rows16_types<4, 1, uint8_t>(g, fx, fa, fb, dtype, gy, st);
@@ -1013,7 +1023,7 @@ __global__ __launch_bounds__(256) void k_fp8_slabs(const float *__restrict__ par
 }
 
 // Few tiles and a long k: slabs of k blocks, so that there are two workgroups per CU, four blocks a slab at least.
-// 1000 x 400 x 30720, float32: 394 us in one slab, 33 us (and 7 for their sum) in 16.
+// 1000 x 400 x 30720, float32: 394 us in one slab, 41.5 us (and 7 for their sum) in 16.
 static int fp8_slabs(const SkmCtx *ctx, long M, long N, long K)
 {
     const long tiles = ((M + 127) / 128) * ((N + 127) / 128), kb = fp8_kpad(K) / FP8_BLOCK;

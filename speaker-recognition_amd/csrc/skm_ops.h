@@ -40,6 +40,15 @@ __device__ __forceinline__ void store_any(T *p, const V &v)
     __builtin_memcpy(p, &v, sizeof(V));
 }
 
+// What the lanes of a wave wrote to LDS before is what its lanes read behind it.  The hardware carries a wave's LDS
+// instructions out in order; this keeps the compiler from exchanging them (no instruction comes of it).
+__device__ __forceinline__ void wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <typename T>
 __device__ __forceinline__ T wave_max(T v)
 {
