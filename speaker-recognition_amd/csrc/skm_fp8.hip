@@ -419,55 +419,23 @@ typedef __attribute__((address_space(1))) const void *glb_ptr;
 // Measured: 8192 x 8192 x 8192 to bf16 471 us, 2335 TFLOP/s (matrix pipe busy 62 % of the cycles at 1.95 GHz: the engine
 // clock gives way to power on random operands); 4096 x 8192 x 4096 at 2600.  To float32 887 us, 1240 TFLOP/s (60 %, 1.92
 // GHz), as fast as a plain bf16 product of the size on this GPU (1241).
-template <int MT, int NT, int FA, int FB, typename TO>
-__global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args g)
-{
-    constexpr int BM = MT * 64, BN = NT * 64, LOADS = (MT + NT) * 2;
-    // One array: with two of them hipcc waits for the loads in flight in front of every read of LDS.
+template <int MT, int NT> struct Fp8Lds {
     // [DEPTH stages of (BM + BN) rows of 128 bytes][two groups of four blocks of (BM + BN) scale dwords]
     // 256 x 128 has room for three stages, and a load then has two and a half to arrive.
-    constexpr int DEPTH = MT == 4 && NT == 2 ? 3 : 2;
-    constexpr int STAGE = (BM + BN) * FP8_BLOCK, GROUP = (BM + BN) * 4;
-    __shared__ __align__(16) uint8_t sh[DEPTH * STAGE + 2 * GROUP];
+    static constexpr int BM = MT * 64, BN = NT * 64, DEPTH = MT == 4 && NT == 2 ? 3 : 2;
+    static constexpr int STAGE = (BM + BN) * FP8_BLOCK, GROUP = (BM + BN) * 4, BYTES = DEPTH * STAGE + 2 * GROUP;
+};
+
+// one tile: `rows` rows from row0 on, the columns from col0 on, blocks kb0 .. kb1
+template <int MT, int NT, int FA, int FB, typename TO>
+__device__ __forceinline__ void fp8_tile(const Fp8Args &g, uint8_t *sh, int rows, long row0, int col0, int kb0, int kb1,
+                                         const uint8_t *B, const uint8_t *sB, TO *C)
+{
+    typedef Fp8Lds<MT, NT> Lds;
+    constexpr int BM = Lds::BM, BN = Lds::BN, DEPTH = Lds::DEPTH, STAGE = Lds::STAGE, GROUP = Lds::GROUP, LOADS = (MT + NT) * 2;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 1, wn = wave & 1, r = lane & 31, h = lane >> 5;
-
-    int tm, tn;
-    {   // workgroups w, w + 8, ... share an XCD: an XCD takes a run of consecutive tiles, columns of 8 row tiles at a time
-        const int tiles_m = g.tiles ? g.tile_count[0] : g.tiles_m;     // by plan: of the grid's, those that there are
-        const int total = tiles_m * g.tiles_n;
-        const int q = total / 8, rem = total % 8, x = blockIdx.x % 8, i = blockIdx.x / 8;
-        if (i >= q + (x < rem ? 1 : 0)) return;
-        int t = x * q + (x < rem ? x : rem) + i;
-        const int group = 8 * g.tiles_n, gi = t / group, m0 = gi * 8;
-        const int gm = tiles_m - m0 < 8 ? tiles_m - m0 : 8;
-        t -= gi * group;
-        tm = m0 + t % gm;
-        tn = t / gm;
-    }
-    int kb0 = g.kb0, kb1 = g.kb1;
-    int rows = g.M - tm * BM;               // rows of this tile
-    long row0 = (long)tm * BM;
-    const uint8_t *B = g.B, *sB = g.sB;
-    TO *C = static_cast<TO *>(g.C);
-    if (g.tiles) {
-        const int32_t *t = g.tiles + (long)tm * 4;
-        B += t[0] * g.eB;
-        sB += t[0] * g.esB;
-        row0 = t[1];
-        rows = t[2];
-    } else if (g.first) {
-        const int e = blockIdx.y;
-        kb0 = g.first[e];
-        kb1 = g.first[e + 1];
-        C += e * g.eC;
-    } else if (g.slabs > 1) {
-        const int z = blockIdx.y, n = kb1 - kb0;
-        kb1 = kb0 + (int)((long)n * (z + 1) / g.slabs);
-        kb0 += (int)((long)n * z / g.slabs);
-        C += z * g.zC;
-    }
-    const int col0 = tn * BN, cols = g.N - col0;
+    const int cols = g.N - col0;
 
     // From this tile's first row (A by plan: from A's first), so that a lane's offset is 32 bits wide.
     const bool by_pair = g.tiles && g.slots;
@@ -722,7 +690,7 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
     // (q & 3) + 8 (q >> 2) + 4 (lane >> 5).  32 rows at a time go through the wave's own part of LDS, so that 16 bytes of a
     // row are stored by one lane and a row's bytes by neighbouring ones.
     constexpr int CW = NT * 32, PITCH = CW + 4, VE = 16 / sizeof(TO), PER = CW / VE, RSTEP = 64 / PER;
-    static_assert(sizeof(sh) >= 4 * 32 * PITCH * sizeof(float), "the result's rows fit where the stages were");
+    static_assert(Lds::BYTES >= 4 * 32 * PITCH * sizeof(float), "the result's rows fit where the stages were");
     float *lw = reinterpret_cast<float *>(sh) + wave * 32 * PITCH;
     typedef TO vo __attribute__((ext_vector_type(VE)));
     __syncthreads();                        // the other waves have read their last stage
@@ -768,6 +736,58 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
         }
         wave_sync();
     }
+}
+
+template <int MT, int NT, int FA, int FB, typename TO>
+__global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args g)
+{
+    constexpr int BM = MT * 64, BN = NT * 64;
+    // One array: with two of them hipcc waits for the loads in flight in front of every read of LDS.
+    __shared__ __align__(16) uint8_t sh[Fp8Lds<MT, NT>::BYTES];
+
+    int tm, tn;
+    {   // workgroups w, w + 8, ... share an XCD: an XCD takes a run of consecutive tiles, columns of 8 row tiles at a time
+        const int tiles_m = g.tiles ? g.tile_count[0] : g.tiles_m;     // by plan: of the grid's, those that there are
+        const int total = tiles_m * g.tiles_n;
+        const int q = total / 8, rem = total % 8, x = blockIdx.x % 8, i = blockIdx.x / 8;
+        if (i >= q + (x < rem ? 1 : 0)) return;
+        int t = x * q + (x < rem ? x : rem) + i;
+        const int group = 8 * g.tiles_n, gi = t / group, m0 = gi * 8;
+        const int gm = tiles_m - m0 < 8 ? tiles_m - m0 : 8;
+        t -= gi * group;
+        tm = m0 + t % gm;
+        tn = t / gm;
+    }
+    int kb0 = g.kb0, kb1 = g.kb1;
+    int rows = g.M - tm * BM;               // rows of this tile
+    long row0 = (long)tm * BM;
+    const uint8_t *B = g.B, *sB = g.sB;
+    TO *C = static_cast<TO *>(g.C);
+    if (g.tiles) {
+        const int32_t *t = g.tiles + (long)tm * 4;
+        B += t[0] * g.eB;
+        sB += t[0] * g.esB;
+        row0 = t[1];
+        rows = t[2];
+    } else if (g.first) {
+        const int e = blockIdx.y;
+        kb0 = g.first[e];
+        kb1 = g.first[e + 1];
+        C += e * g.eC;
+    } else if (g.slabs > 1) {
+        const int z = blockIdx.y, n = kb1 - kb0;
+        kb1 = kb0 + (int)((long)n * (z + 1) / g.slabs);
+        kb0 += (int)((long)n * z / g.slabs);
+        C += z * g.zC;
+    }
+    // A last tile of half the rows or less is half the work: experts of about 1000 rows often have one (8191 tokens, 4 of 32
+    // experts, 2048 x 4096, with the whole chain: 355 -> 343 us)
+    if constexpr (MT == 4)
+        if (rows <= BM / 2) {
+            fp8_tile<MT / 2, NT, FA, FB, TO>(g, sh, rows, row0, tn * BN, kb0, kb1, B, sB, C);
+            return;
+        }
+    fp8_tile<MT, NT, FA, FB, TO>(g, sh, rows, row0, tn * BN, kb0, kb1, B, sB, C);
 }
 
 template <int MT, int NT, typename TO>
@@ -1190,7 +1210,7 @@ extern "C" int skm_gemm_fp8(void *ctx_, const void *A, const void *sA, int fmt_a
         char *part = static_cast<char *>(ws) + (a_dtype >= 0 ? fp8_operand_bytes(M, K) : 0);
         return fp8_run(ctx, g, fmt_a, fmt_b, c_dtype, (unsigned)g.slabs, st, "k_gemm_fp8", part);
     }
-    // A last row tile of up to 64 rows that would begin another round of workgroups goes to the kernel for few rows
+    // A last row tile of up to 64 rows that would put a few workgroups behind all the others goes to the kernel for few rows
     // (8200 x 4096 x 4096: 157 -> 122 us)
     const int wn = c_dtype != SKM_DT_F32 ? 256 : 128, rest = M % 256;
     const long tn = (N + wn - 1) / wn, cu = ctx->cu_count;

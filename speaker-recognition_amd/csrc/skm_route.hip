@@ -1073,7 +1073,7 @@ __device__ void plan_place(const PlanArgs &a, int run, int lane, int32_t *h)
     for (long i0 = lo; i0 < hi; i0 += 64) {
         const long i = i0 + lane;
         const int e = ahead;
-        ahead = i + 64 < hi ? a.ids[i + 64] : -1;           // the next 64, under this round's work
+        ahead = i + 64 < hi ? a.ids[i + 64] : -1;           // the next 64, under this step's work
         const bool ok = e >= 0 && e < a.E;
         unsigned long long same = __ballot(ok);
         for (int b = 0; b < bits; ++b) {
