@@ -1283,10 +1283,10 @@ extern "C" int skm_route_plan(void *ctx_, const int32_t *ids, long n, int E, int
     SkmProfScope ps(ctx, "k_plan", st);
     if (plan_is_one(n, E)) {
         hipLaunchKernelGGL(k_plan_one, dim3(1), dim3(64 * PLAN_WAVES), (size_t)PLAN_WAVES * E * 4, st, a);
-    } else {
-        hipLaunchKernelGGL(k_plan_count, dim3((unsigned)a.nw), dim3(64), (size_t)E * 4, st, a);
+    } else {                                // no pairs, no runs: only the scan, which writes the tables' zeros
+        if (a.nw) hipLaunchKernelGGL(k_plan_count, dim3((unsigned)a.nw), dim3(64), (size_t)E * 4, st, a);
         hipLaunchKernelGGL(k_plan_scan, dim3(1), dim3(1024), 0, st, a);
-        hipLaunchKernelGGL(k_plan_place, dim3((unsigned)a.nw), dim3(64), (size_t)E * 4, st, a);
+        if (a.nw) hipLaunchKernelGGL(k_plan_place, dim3((unsigned)a.nw), dim3(64), (size_t)E * 4, st, a);
     }
     SKM_HIP(hipGetLastError());
     return SKM_OK;
