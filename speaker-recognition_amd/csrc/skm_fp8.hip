@@ -275,14 +275,20 @@ extern "C" int skm_fp8_rows(void *ctx_, const void *x, int dtype, long M, int K,
     if (M == 0) return SKM_OK;
     RowsArgs a{x, M, ldx, K, (int)(fp8_kpad(K) / FP8_BLOCK), (int)fp8_sstride(K), static_cast<uint8_t *>(q),
                static_cast<uint8_t *>(s)};
-    const long grid = (M * a.KB + 15) / 16;
-    SKM_REQUIRE(grid <= 0x7FFFFFFF, "skm_fp8_rows: too many blocks");
     SkmDeviceGuard guard(ctx);
     hipStream_t st = (hipStream_t)stream;
     SkmProfScope ps(ctx, "k_fp8_rows", st);
-#define ROWS_LAUNCH(T, FMT) hipLaunchKernelGGL((k_fp8_rows<T, FMT>), dim3((unsigned)grid), dim3(256), 0, st, a)
-    FP8_IN_TYPES(ROWS_LAUNCH)
-    SKM_HIP(hipGetLastError());
+    const long most = SKM_MAX_GROUPS * 16 / a.KB;       // rows of a launch
+    for (long m = 0; m < M; m += most) {
+        a.M = M - m < most ? M - m : most;
+        a.x = static_cast<const char *>(x) + m * ldx * skm_dt_size(dtype);
+        a.q = static_cast<uint8_t *>(q) + m * a.KB * FP8_BLOCK;
+        a.s = static_cast<uint8_t *>(s) + m * a.S;
+        const unsigned grid = (unsigned)((a.M * a.KB + 15) / 16);
+#define ROWS_LAUNCH(T, FMT) hipLaunchKernelGGL((k_fp8_rows<T, FMT>), dim3(grid), dim3(256), 0, st, a)
+        FP8_IN_TYPES(ROWS_LAUNCH)
+        SKM_HIP(hipGetLastError());
+    }
     return SKM_OK;
 }
 
@@ -294,7 +300,8 @@ extern "C" int skm_fp8_tiles(void *ctx_, const void *w, int dtype, int batch, in
                 "skm_fp8_tiles: bad argument");
     if (int rc = fp8_check_types("skm_fp8_tiles", dtype, fmt)) return rc;
     if (batch == 0) return SKM_OK;
-    SKM_REQUIRE(batch <= 65535 && fp8_kpad(N) / FP8_BLOCK <= 65535, "skm_fp8_tiles: too large");
+    SKM_REQUIRE(batch <= 65535 && fp8_kpad(N) / FP8_BLOCK <= 65535 && fp8_kpad(K) / FP8_BLOCK <= SKM_MAX_GROUPS,
+                "skm_fp8_tiles: too large");
     TileArgs a{};
     a.x = w; a.R = N; a.ldx = ldw; a.sx = sw; a.C = K;
     a.q = static_cast<uint8_t *>(q); a.s = static_cast<uint8_t *>(s);
@@ -322,7 +329,8 @@ extern "C" int skm_fp8_columns(void *ctx_, const void *x, int dtype, long R, int
     const long blocks = tiles ? max_tiles : fp8_kpad(R) / FP8_BLOCK;
     if (blocks == 0) return SKM_OK;
     SKM_REQUIRE(x && qt && st_, "skm_fp8_columns: bad argument");
-    SKM_REQUIRE(blocks <= 65535, "skm_fp8_columns: more than 65535 blocks of rows");
+    SKM_REQUIRE(blocks <= 65535 && fp8_kpad(C) / FP8_BLOCK <= SKM_MAX_GROUPS,
+                "skm_fp8_columns: more than 65535 blocks of rows or 2^31 - 128 columns");
     TileArgs a{};
     a.x = x; a.R = R; a.ldx = ldx; a.C = C;
     a.qt = static_cast<uint8_t *>(qt); a.st = static_cast<uint8_t *>(st_);
@@ -1010,6 +1018,12 @@ static int rows16_types(const Fp8Args &g, const Fp8Float &fx, int fa, int fb, in
 static int rows16_run(SkmCtx *ctx, const Fp8Args &g, const Fp8Float &fx, int x_dtype, int fa, int fb, int dtype, unsigned gy,
                       hipStream_t st)
 {
+    // threads along x of the narrowest column tiles (a launch has fewer than 2^32)
+    const int groups = (g.kb1 + 3) / 4;
+    if ((((long)g.N + 15) / 16) * 64 * (groups < 8 ? groups : 8) > 0xFFFFFFFFL) {
+        skm_set_error("product of few rows: %d columns of %d blocks are too many for one launch", g.N, g.kb1);
+        return SKM_ERR_UNSUPPORTED;
+    }
     SkmProfScope ps(ctx, "k_gemm_fp8_rows16", st);
     if (g.A) {
         // two column tiles a workgroup (A's rows are read once per workgroup) where they are enough for every CU:
@@ -1082,7 +1096,7 @@ static int fp8_run(SkmCtx *ctx, Fp8Args g, int fa, int fb, int dtype, unsigned g
         return SKM_ERR_UNSUPPORTED;
     }
     const long total = (long)g.tiles_m * g.tiles_n;
-    SKM_REQUIRE(total <= 0x7FFFFFFF && gy <= 65535, "%s: too many tiles", tag);
+    SKM_REQUIRE(total <= SKM_MAX_GROUPS && gy <= 65535, "%s: too many tiles", tag);
     if (total == 0 || gy == 0) return SKM_OK;
     {
         SkmProfScope ps(ctx, tag, st);

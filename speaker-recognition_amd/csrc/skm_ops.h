@@ -11,6 +11,11 @@ static inline int skm_dt_size(int dt)
     return dt == SKM_DT_F32 ? 4 : dt == SKM_DT_BF16 || dt == SKM_DT_F16 ? 2 : dt == SKM_DT_F64 ? 8 : 0;
 }
 
+// The workgroups of 256 threads that one launch takes.  A launch has fewer than 2^32 threads along x; the runtime cuts a
+// larger grid's number of threads to 32 bits without an error, so the rows behind them would have no result.  Calls
+// of more rows are several launches.
+#define SKM_MAX_GROUPS 0xFFFFFFL
+
 // The launches go to the ctx's GPU whatever device the calling thread has current.
 struct SkmDeviceGuard {
     int prev;

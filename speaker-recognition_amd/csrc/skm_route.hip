@@ -6,6 +6,7 @@
 #define ROUTE_MAX_E 4096
 #define ROUTE_MAX_K 64
 #define ROUTE_MAX_G 64
+#define ROUTE_MAX_ROWS (SKM_MAX_GROUPS * 4)     // of one launch: a workgroup has 4 rows at least
 
 struct RouteArgs {
     const void *x;          // logits [T][ldx]
@@ -983,15 +984,18 @@ extern "C" int skm_route(void *ctx_, const void *x, int dtype, long T, int E, lo
     SkmDeviceGuard guard(ctx);
     hipStream_t st = (hipStream_t)stream;
     SkmProfScope ps(ctx, "k_route", st);
-    const RouteArgs a{x, T, ldx, E, k, bias, groups, group_k, group_top, scores == SKM_ROUTE_SIGMOID, renorm != 0, scale,
-                      ids, weights};
-    switch (dtype) {
-    case SKM_DT_F32: route_launch<float>(a, st); break;
-    case SKM_DT_BF16: route_launch<bf16_t>(a, st); break;
-    case SKM_DT_F16: route_launch<f16_t>(a, st); break;
-    default: route_launch<double>(a, st); break;
+    for (long t = 0; t < T; t += ROUTE_MAX_ROWS) {
+        const RouteArgs a{static_cast<const char *>(x) + t * ldx * skm_dt_size(dtype), T - t < ROUTE_MAX_ROWS ? T - t : ROUTE_MAX_ROWS,
+                          ldx, E, k, bias, groups, group_k, group_top, scores == SKM_ROUTE_SIGMOID, renorm != 0, scale,
+                          ids + t * k, weights + t * k};
+        switch (dtype) {
+        case SKM_DT_F32: route_launch<float>(a, st); break;
+        case SKM_DT_BF16: route_launch<bf16_t>(a, st); break;
+        case SKM_DT_F16: route_launch<f16_t>(a, st); break;
+        default: route_launch<double>(a, st); break;
+        }
+        SKM_HIP(hipGetLastError());
     }
-    SKM_HIP(hipGetLastError());
     return SKM_OK;
 }
 
@@ -1012,14 +1016,21 @@ extern "C" int skm_route_backward(void *ctx_, const void *x, int dtype, long T, 
     SkmDeviceGuard guard(ctx);
     hipStream_t st = (hipStream_t)stream;
     SkmProfScope ps(ctx, "k_route_backward", st);
-    const RouteBackArgs a{x, T, ldx, E, k, ids, dweights, scores == SKM_ROUTE_SIGMOID, renorm != 0, scale, dx};
-    switch (dtype) {
-    case SKM_DT_F32: route_back_go<float>(a, st); break;
-    case SKM_DT_BF16: route_back_go<bf16_t>(a, st); break;
-    case SKM_DT_F16: route_back_go<f16_t>(a, st); break;
-    default: hipLaunchKernelGGL((k_route_backward<double, double>), dim3((unsigned)((T + 3) / 4)), dim3(256), 0, st, a); break;
+    for (long t = 0; t < T; t += ROUTE_MAX_ROWS) {
+        const int size = skm_dt_size(dtype);
+        const RouteBackArgs a{static_cast<const char *>(x) + t * ldx * size, T - t < ROUTE_MAX_ROWS ? T - t : ROUTE_MAX_ROWS,
+                              ldx, E, k, ids + t * k, dweights + t * k, scores == SKM_ROUTE_SIGMOID, renorm != 0, scale,
+                              static_cast<char *>(dx) + t * E * size};
+        switch (dtype) {
+        case SKM_DT_F32: route_back_go<float>(a, st); break;
+        case SKM_DT_BF16: route_back_go<bf16_t>(a, st); break;
+        case SKM_DT_F16: route_back_go<f16_t>(a, st); break;
+        default:
+            hipLaunchKernelGGL((k_route_backward<double, double>), dim3((unsigned)((a.T + 3) / 4)), dim3(256), 0, st, a);
+            break;
+        }
+        SKM_HIP(hipGetLastError());
     }
-    SKM_HIP(hipGetLastError());
     return SKM_OK;
 }
 
@@ -1302,6 +1313,7 @@ struct CombineArgs {
     void *out;              // [T][N]
     const void *dout;
     float *dw;
+    long pair0;             // first pair of a launch (gradient)
 };
 
 // out[t] = sum_j w[t][j] rows[pos[t][j]], in the order of j, float32.  An empty place adds w * 0: nothing, or the NaN
@@ -1364,7 +1376,7 @@ __global__ __launch_bounds__(256) void k_route_combine_backward(CombineArgs a)
     typedef TR vr __attribute__((ext_vector_type(VEC)));
     typedef TO vo __attribute__((ext_vector_type(VEC)));
     const int lane = threadIdx.x & 63;
-    const long i = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long i = a.pair0 + (long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (i >= a.T * a.k) return;
     const int p = a.pos[i];
     float s = 0.f;
@@ -1396,14 +1408,28 @@ static void combine_launch(const CombineArgs &a, hipStream_t st)
     // 16 bytes of the narrower type a thread
     constexpr int V = sizeof(TR) == 4 && sizeof(TO) == 4 ? 4 : 8;
     const int per = (a.N + V - 1) / V, tokens = per <= 128 ? 256 / per : 1;
-    const dim3 grid((unsigned)((a.T + tokens - 1) / tokens), tokens > 1 ? 1u : (unsigned)((per + 255) / 256));
-    hipLaunchKernelGGL((k_route_combine<TR, TO, V>), grid, dim3(256), 0, st, a, per, tokens);
+    const long most = SKM_MAX_GROUPS * tokens;
+    for (long t = 0; t < a.T; t += most) {
+        CombineArgs b = a;
+        b.pos += t * a.k;
+        b.w += t * a.k;
+        b.out = static_cast<TO *>(a.out) + t * a.N;
+        b.T = a.T - t < most ? a.T - t : most;
+        const dim3 grid((unsigned)((b.T + tokens - 1) / tokens), tokens > 1 ? 1u : (unsigned)((per + 255) / 256));
+        hipLaunchKernelGGL((k_route_combine<TR, TO, V>), grid, dim3(256), 0, st, b, per, tokens);
+    }
 }
 
 template <typename TR, typename TO>
 static void combine_back_launch(const CombineArgs &a, hipStream_t st)
 {
-    hipLaunchKernelGGL((k_route_combine_backward<TR, TO>), dim3((unsigned)((a.T * a.k + 3) / 4)), dim3(256), 0, st, a);
+    const long pairs = a.T * a.k;
+    CombineArgs b = a;
+    for (b.pair0 = 0; b.pair0 < pairs; b.pair0 += SKM_MAX_GROUPS * 4) {
+        const long groups = (pairs - b.pair0 + 3) / 4;
+        hipLaunchKernelGGL((k_route_combine_backward<TR, TO>), dim3((unsigned)(groups < SKM_MAX_GROUPS ? groups : SKM_MAX_GROUPS)),
+                           dim3(256), 0, st, b);
+    }
 }
 
 #define COMBINE_TYPES(F, TR_CODE, TO_CODE)                                                                       \
@@ -1430,7 +1456,7 @@ extern "C" int skm_route_combine(void *ctx_, const void *rows, int rows_dtype, c
     SkmDeviceGuard guard(ctx);
     hipStream_t st = (hipStream_t)stream;
     SkmProfScope ps(ctx, "k_route_combine", st);
-    const CombineArgs a{rows, pos, weights, T, k, N, out, nullptr, nullptr};
+    const CombineArgs a{rows, pos, weights, T, k, N, out, nullptr, nullptr, 0};
     COMBINE_TYPES(combine_launch, rows_dtype, out_dtype)
     SKM_HIP(hipGetLastError());
     return SKM_OK;
@@ -1448,7 +1474,7 @@ extern "C" int skm_route_combine_backward(void *ctx_, const void *rows, int rows
     SkmDeviceGuard guard(ctx);
     hipStream_t st = (hipStream_t)stream;
     SkmProfScope ps(ctx, "k_route_combine_backward", st);
-    const CombineArgs a{rows, pos, nullptr, T, k, N, nullptr, dout, dweights};
+    const CombineArgs a{rows, pos, nullptr, T, k, N, nullptr, dout, dweights, 0};
     COMBINE_TYPES(combine_back_launch, rows_dtype, dout_dtype)
     SKM_HIP(hipGetLastError());
     return SKM_OK;
