@@ -951,6 +951,12 @@ class HipEngine(object):
             raise SkmError("%s: type %s" % (what, dtype))
         return code
 
+    @staticmethod
+    def _int32(n, what):
+        """a size that the C entry points take as an int (ctypes would cut a larger one to its low 32 bits)"""
+        if not 0 <= n <= 0x7FFFFFFF:
+            raise SkmError("%s: a size or option of %d is outside 0 .. 2^31 - 1" % (what, n))
+
     def _matrix(self, t, what, rows=None, cols=None, dtypes=None):
         """a device matrix with unit stride along its rows; returns the distance between them"""
         if not isinstance(t, self.torch.Tensor) or t.device != self.device or t.dim() != 2:
@@ -962,6 +968,7 @@ class HipEngine(object):
         n, m = t.shape
         if n == 0 or m == 0:
             return m
+        self._int32(m, what)
         ld = t.stride(0) if n > 1 else m
         if (m > 1 and t.stride(1) != 1) or ld < m:
             raise SkmError("%s: rows have to be contiguous (strides %s)" % (what, tuple(t.stride())))
@@ -994,13 +1001,16 @@ class HipEngine(object):
         T, E = logits.shape
         if bias is not None:
             self._vector(bias, "route: bias", E, torch.float32)
-        k = int(k)
-        ids = torch.empty((T, max(k, 0)), dtype=torch.int32, device=self.device)
-        weights = torch.empty((T, max(k, 0)), dtype=torch.float32, device=self.device)
+        k, groups, group_top = int(k), int(groups), int(group_top)
+        group_k = groups if group_k is None else int(group_k)
+        if min(k, groups, group_k, group_top) < 0 or max(k, groups, group_k, group_top) > 0x7FFFFFFF:
+            raise SkmError("route: k, groups, group_k and group_top are at least 0 and below 2^31")
+        ids = torch.empty((T, k), dtype=torch.int32, device=self.device)
+        weights = torch.empty((T, k), dtype=torch.float32, device=self.device)
         self._check(self.lib.skm_route(
             self.ctx, logits.data_ptr(), self._dt(logits.dtype, (0, 1, 2, 3), "route: logits"), T, E, ldx, k,
-            self._scores(scores), bias.data_ptr() if bias is not None else None, int(groups),
-            int(groups if group_k is None else group_k), int(group_top), 1 if renorm else 0, float(scale),
+            self._scores(scores), bias.data_ptr() if bias is not None else None, groups,
+            group_k, group_top, 1 if renorm else 0, float(scale),
             ids.data_ptr(), weights.data_ptr(), self._raw_stream()))
         return ids, weights
 
@@ -1024,6 +1034,7 @@ class HipEngine(object):
         0 .. E - 1 = no expert) chose: a RoutePlan (skm_route_plan)."""
         torch = self.torch
         E = int(E)
+        self._int32(E, "route_plan: experts")
         if not isinstance(ids, torch.Tensor) or ids.dim() != 2:
             raise SkmError("route_plan: ids T x k are wanted")
         T, k = ids.shape
@@ -1093,6 +1104,7 @@ class HipEngine(object):
         batch = tuple(w.shape[:-2])
         if N < 1 or K < 1:
             raise SkmError("fp8_tiles: shape %s" % (tuple(w.shape),))
+        self._int32(max(w.shape), "fp8_tiles: w")
         out = Fp8Matrix(self, batch + (N,), K, fmt)
         outt = Fp8Matrix(self, batch + (K,), N, fmt) if transposed else None
         self._check(self.lib.skm_fp8_tiles(
@@ -1152,6 +1164,7 @@ class HipEngine(object):
         N = B.shape[0]
         if B.shape[1] != K or B.plan is not None:
             raise SkmError("gemm_fp8: A %s and B %s do not go together" % ((M, K), B.shape))
+        self._int32(max(M, N), "gemm_fp8")
         if out is None:
             if accumulate:
                 raise SkmError("gemm_fp8: accumulate without out")
