@@ -985,6 +985,10 @@ class HipEngine(object):
             raise SkmError("%s: a contiguous %s tensor of %d on %s is wanted" % (what, dtype, n, self.device))
         return t
 
+    def _plan(self, plan, what):
+        if not isinstance(plan, RoutePlan) or plan._buf.device != self.device:
+            raise SkmError("%s: a RoutePlan on %s is wanted" % (what, self.device))
+
     @staticmethod
     def _scores(scores):
         if scores not in ("softmax", "sigmoid"):
@@ -1053,6 +1057,7 @@ class HipEngine(object):
     def route_combine(self, rows, weights, plan, dtype=None):
         """out[t] = sum_j weights[t, j] rows[the plan's row of (t, j)] in `dtype` (default: that of rows)."""
         torch = self.torch
+        self._plan(plan, "route_combine")
         N = rows.shape[-1]
         self._dense(rows, "route_combine: rows", plan.n, N, None)
         self._dense(weights, "route_combine: weights", plan.T, plan.k, (torch.float32,))
@@ -1067,6 +1072,7 @@ class HipEngine(object):
     def route_combine_backward(self, rows, dout, plan):
         """Gradient of route_combine's weights (float32 T x k)."""
         torch = self.torch
+        self._plan(plan, "route_combine_backward")
         N = rows.shape[-1]
         self._dense(rows, "route_combine_backward: rows", plan.n, N, None)
         self._dense(dout, "route_combine_backward: dout", plan.T, N, None)
@@ -1118,6 +1124,8 @@ class HipEngine(object):
         With a plan: the rows of its pairs (x holds a row per token), times `weights` (float32 T x k) if given, every
         expert's from a new block: for gemm_fp8_experts_wgrad."""
         torch = self.torch
+        if plan is not None:
+            self._plan(plan, "fp8_columns")
         ldx = self._matrix(x, "fp8_columns: x", rows=plan.T if plan is not None else None)
         R, C = x.shape
         if C < 1 or (R < 1 and plan is None):
@@ -1185,6 +1193,7 @@ class HipEngine(object):
         not written) is W[expert of r] times the row of A: of the pair's token where A has plan.T rows, of r itself
         where it has plan.n and the plan more than one place.  A: Fp8Matrix, or a float matrix that goes through 8-bit
         floats as fp8_rows makes them; W: Fp8Matrix E x N x K."""
+        self._plan(plan, "gemm_fp8_experts")
         a, sa, fa, a_dtype, lda, (M, K) = self._operand(A, "gemm_fp8_experts: A")
         self._fp8(W, "gemm_fp8_experts: W", 2)
         E, N, Kw = W.shape
@@ -1205,6 +1214,7 @@ class HipEngine(object):
     def gemm_fp8_experts_wgrad(self, A, B, plan, out=None, accumulate=False):
         """float32 E x M x N: for each expert A B' over its rows, A (M) and B (N) from fp8_columns with this plan."""
         torch = self.torch
+        self._plan(plan, "gemm_fp8_experts_wgrad")
         self._fp8(A, "gemm_fp8_experts_wgrad: A")
         self._fp8(B, "gemm_fp8_experts_wgrad: B")
         if A.plan is not plan or B.plan is not plan:
