@@ -17,7 +17,8 @@ and checks, per kernel, linearly over the instruction stream:
         any later `ds_read`) can reach before an `s_waitcnt vmcnt(n)` that covers the load: hipcc emits no such wait
         for this load kind.  (A `ds_read` in the SAME iteration belongs to the other buffer of the ring by design.)
         Kernels listed in RING_DEPTH keep their loads in flight longer -- a ring of three LDS stages filled two
-        iterations ahead: there the reads of the iteration after next are the ones that must be covered.
+        iterations ahead: there the reads of the iteration after next are the ones that must be covered.  Of a kernel
+        with loops of different depth each is held to its own.
 
 A wait state is one issued instruction; `s_nop n` counts n + 1.  One refinement over LLVM's counting (which is one per
 instruction whatever it is): the matrix pipe takes one MFMA at a time, so a second MFMA of the same kind issues no
@@ -61,11 +62,12 @@ MFMA_PASSES = [
     (re.compile(r"^v_mfma_(scale_)?f32_32x32x64_"), 16),
 ]
 STRICT = False
-# LDS-direct loads: iterations between a load and the first ds_read of its data (default 1: a ring of two buffers)
+# LDS-direct loads: iterations between a load and the first ds_read of its data (default 1: a ring of two buffers), and,
+# where a kernel holds loops of different depth, the count that the waits of the loops with this depth leave
 RING_DEPTH = [
-    (re.compile(r"k_gemm_b3"), 2),      # csrc/skm_gemm_b3.hip: three stages, loads issued two stages ahead, vmcnt(6)
-    (re.compile(r"k_gemm_fp8I"), 2),    # csrc/skm_fp8.hip: two stages; half of a stage is read in front of the wait
-    (re.compile(r"k_gemm_fp8ILi4ELi2"), 3),     # 256 x 128 tiles: three stages, vmcnt(14)
+    (re.compile(r"k_gemm_b3"), 2, None),    # csrc/skm_gemm_b3.hip: three stages, loads issued two stages ahead, vmcnt(6)
+    (re.compile(r"k_gemm_fp8I"), 2, None),  # csrc/skm_fp8.hip: two stages; half of a stage is read in front of the wait
+    (re.compile(r"k_gemm_fp8ILi4ELi2"), 3, 14),     # 256 x 128 tiles: three stages; the half tile's loop has two
 ]
 REG = re.compile(r"\b([va])(?:(\d+)|\[(\d+):(\d+)\])(?![\w\[])")
 LINE = re.compile(r"^\s+(\S+)\s*(.*?)\s*//\s*([0-9A-Fa-f]+):")
@@ -280,6 +282,21 @@ class Flow(object):
                     self.loops[key] = self.loops.get(key, set()) | body
 
 
+def vmcnt(a):
+    """the count of an s_waitcnt vmcnt(n), None for anything else"""
+    m = re.search(r"vmcnt\((\d+)\)", a.args) if a.op == "s_waitcnt" else None
+    return int(m.group(1)) if m else None
+
+
+def ring_depth(name, loop):
+    """RING_DEPTH's entry for a kernel's loop, given by its instructions"""
+    depth = 1
+    for pat, d, left in RING_DEPTH:
+        if pat.search(name) and (left is None or any(vmcnt(a) == left for a in loop)):
+            depth = d
+    return depth
+
+
 def lint_kernel(name, ins):
     found = []
     flow = Flow(ins)
@@ -341,10 +358,6 @@ def lint_kernel(name, ins):
                                 found.append("(ii)  %s @%x writes %s%d, %s @%x reads it after %d of 2 wait states"
                                              % (a.op, a.addr, r[0], r[1], b.op, b.addr, since))
     # ---- (iii) LDS-direct loads against the ds_reads of the next iteration (of the iteration `depth` later)
-    depth = 1
-    for pat, d in RING_DEPTH:
-        if pat.search(name):
-            depth = d
     for i, a in enumerate(ins):
         if not a.lds_direct:
             continue
@@ -352,6 +365,8 @@ def lint_kernel(name, ins):
         back = {e for e, body in flow.loops.items() if mine in body}
         if not back:
             continue                                        # not in a loop
+        inner = min((flow.loops[e] for e in back), key=len)
+        depth = ring_depth(name, [b for blk in inner for b in ins[flow.blocks[blk][0]:flow.blocks[blk][1] + 1]])
         # state (instruction, crossed a back edge of a loop that holds the load) -> fewest vector-memory
         # instructions issued behind the load on any path there (the fewest is the worst case for a vmcnt(n))
         best, stack, bad = {}, [(t, 0, 0) for t in succ[i]], None
@@ -361,10 +376,9 @@ def lint_kernel(name, ins):
                 continue
             best[(j, wrapped)] = later
             b = ins[j]
-            if b.op == "s_waitcnt":
-                m = re.search(r"vmcnt\((\d+)\)", b.args)
-                if m and int(m.group(1)) <= later:
-                    continue                                # this path is covered
+            n = vmcnt(b)
+            if n is not None and n <= later:
+                continue                                    # this path is covered
             if wrapped >= depth and (b.op.startswith("ds_read") or b.op.startswith("ds_load")):
                 bad = b
                 break
