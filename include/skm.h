@@ -473,7 +473,7 @@ int skm_route_combine_backward(void *ctx, const void *rows_dev, int rows_dtype, 
 
 /* Matrices of 8-bit floats with a power-of-two scale for each block of 128: a block is q * 2^e, e the smallest integer
  * (>= -110; 0 for a block of zeros) with max |x| <= top * 2^e, top = 448 (e4m3) or 57344 (e5m2), q the nearest 8-bit
- * floats to x * 2^-e, ties to even.  NaN and infinities have no part in e; they become NaN (an infinity stays one in
+ * floats to x * 2^-e, ties to even (float32's largest numbers round to 2^128, which float32 shows as infinity).  NaN and infinities have no part in e; they become NaN (an infinity stays one in
  * e5m2).
  *   q[rows][skm_fp8_row_bytes(K)]      K rounded up to 128, zeros behind K
  *   s[rows][skm_fp8_scale_bytes(K)]    e + 127 of the row's blocks
@@ -499,7 +499,10 @@ int skm_fp8_columns(void *ctx, const void *x_dev, int dtype, long R, int C, long
 
 /* C[M][ldc] (+)= A B' of two such matrices [M][K], [N][K] (any of the three block shapes, either format).
  * C float32: exact products, float32 sums.  C bf16 or f16: the 8-bit matrix instructions, which add 8 products at a time in
- * 13 bits below the largest of them (1.4e-5 of a result of random operands, under the rounding to C's type).
+ * 13 bits below the largest of them: up to 2^-10 of the sum of the products' magnitudes is lost, 1.4e-5 of the result's norm
+ * with random operands.  Where products cancel this can be more than the rounding to C's type (2^-8, 2^-11 of the result):
+ * take float32 there.  A result of more columns than one launch has threads for (N / 16 workgroups of 64 threads for every 512
+ * of K, 512 at most; 2^24 tiles) is refused.
  * accumulate adds to what is there, before the rounding to C's type.
  * a_dtype = -1: A is q, s (lda is not looked at).  a_dtype = SKM_DT_*: A is a float matrix in rows of lda that goes through
  * 8-bit floats of format fmt_a as skm_fp8_rows makes them (sA is not looked at).  q and the workspace 16-byte, s 4-byte
@@ -511,8 +514,11 @@ int skm_gemm_fp8(void *ctx, const void *A_dev, const void *sA_dev, int fmt_a, in
 
 /* The experts' products: C[row] = W_e A[row of A], W [E][N][K] (tiles), for the rows of a plan of n pairs.  A has `rows`
  * rows, as for skm_gemm_fp8.  slots = k: the row of A is the pair's token (rows * k = n); slots = 0: A is in the plan's order
- * already (rows = n).  The plan's second table, if it has one, sets the tiles: 16 rows (the weights straight into registers,
- * for up to about 16 rows an expert) or 256 (from about 256 rows an expert); 128 without it.  Rows of C behind the plan's last are left as they are.
+ * already (rows = n).  The plan's second table, if it has one, sets the tiles: 16 rows (the weights straight into registers:
+ * faster where they come from memory and an expert has a few rows, see the engine's RoutePlan) or 256 (bf16 and f16 results
+ * from about 256 rows an expert); 128 without it.  Rows of C behind the plan's last are left as they are.
+ * Rows in bf16 or f16 are rounded once here and again behind skm_route_combine's sum, which is float32; float32 rows are
+ * rounded only there, at half the rate.
  * skm_gemm_fp8_experts_wgrad: C[e] (+)= A_e B_e' (float32 [E][M][N]) over the rows of each expert, A [M], B [N] from
  * skm_fp8_columns with the same plan; an expert without rows has zeros. */
 size_t skm_gemm_fp8_experts_workspace_bytes(void *ctx, long rows, int K, int a_float, int more_rows);

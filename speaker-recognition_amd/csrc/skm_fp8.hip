@@ -408,10 +408,12 @@ typedef __attribute__((address_space(1))) const void *glb_ptr;
 //   pieces at consecutive addresses, so the exchange is made on the global side, within the line.
 //   The scales come the same way, a dword (four blocks) of every row in every fourth stage.
 //   The 8-bit matrix instructions add 8 products at a time in a window of 13 bits below the largest of the 8 (a product
-//   2^-14 of it is lost, measured): 1.4e-5 of a result of random operands.  Under a result that is rounded to bf16 or f16
-//   (2^-9, 2^-12) that is nothing; a float32 result is wanted as such (weight gradients that are added up, rows that a
-//   gradient is formed with), so there the operands become bf16 -- exactly, scale included -- and the products are exact
-//   and the sums float32, at half the rate.
+//   2^-14 of it is lost, measured), the sums of 8 in float32.  Of each 8, up to 7 lose less than 2^-13 of the largest: at
+//   worst 2^-10 of the sum of the products' magnitudes, 1.4e-5 (2^-16) of the result's norm with random operands.  A
+//   bf16 result's own rounding is 2^-8 of it, an f16 one's 2^-11; where the products cancel, what is cut off can exceed
+//   either.  That is the price of twice the rate, taken for results of 16 bits.  A float32 result is wanted for its digits
+//   (weight gradients that are added up, rows that a gradient is formed with), so there the operands become bf16 --
+//   exactly, scale included -- and the products are exact and the sums float32, at half the rate.
 //   Which of the 64 k of a product lies where in the operand registers does not matter as long as A and B agree and a
 //   scale covers all of them: a lane's 32 bytes are 32 consecutive k of its row here.
 // A stage is two halves of 64 k in two sets of fragments: while one set is multiplied, the other is read.  Stage s:
@@ -424,9 +426,9 @@ typedef __attribute__((address_space(1))) const void *glb_ptr;
 // that are under way already.
 // Why 256 x 256: a stage's 64 KB of LDS reads (128 x 128: 32 KB a quarter of the products) fit under its multiplications,
 // and every operand byte is loaded half as often.
-// Measured: 8192 x 8192 x 8192 to bf16 471 us, 2335 TFLOP/s (matrix pipe busy 62 % of the cycles at 1.95 GHz: the engine
-// clock gives way to power on random operands); 4096 x 8192 x 4096 at 2600.  To float32 887 us, 1240 TFLOP/s (60 %, 1.92
-// GHz), as fast as a plain bf16 product of the size on this GPU (1241).
+// Measured: 8192 x 8192 x 8192 to bf16 436 to 477 us by the run, 2300 to 2520 TFLOP/s (matrix pipe busy 63 % of the cycles at
+// 1.93 GHz: the engine clock gives way to power on random operands); 4096 x 8192 x 4096 at 2600.  To float32 880 us, 1250
+// TFLOP/s (63 %, 1.88 GHz), as fast as a plain bf16 product of the size on this GPU (1241).
 template <int MT, int NT> struct Fp8Lds {
     // [DEPTH stages of (BM + BN) rows of 128 bytes][two groups of four blocks of (BM + BN) scale dwords]
     // 256 x 128 has room for three stages, and a load then has two and a half to arrive.
@@ -788,8 +790,10 @@ __global__ __launch_bounds__(256, (MT * NT > 4) ? 1 : 2) void k_gemm_fp8(Fp8Args
         kb0 += (int)((long)n * z / g.slabs);
         C += z * g.zC;
     }
-    // A last tile of half the rows or less is half the work: experts of about 1000 rows often have one (8191 tokens, 4 of 32
-    // experts, 2048 x 4096, with the whole chain: 355 -> 343 us)
+    // A last tile of half the rows or less is half the work: experts of about 1000 rows often have one.  Little comes of
+    // it while the tiles are dealt in the table's order and the last round over the CUs is nearly empty (8191 tokens, 4 of
+    // 32 experts, 2048 x 4096, the whole chain in four runs of either: 377 against 383 us, runs 5 us apart; 8192 tokens, 2 of
+    // 16, a training step: 663 and 664)
     if constexpr (MT == 4)
         if (rows <= BM / 2) {
             fp8_tile<MT / 2, NT, FA, FB, TO>(g, sh, rows, row0, tn * BN, kb0, kb1, B, sB, C);
@@ -828,8 +832,11 @@ struct Fp8Float {
 // k_fp8_rows does it (16 lanes a block, so one row's four blocks at a time), into LDS -- the same work in every workgroup,
 // under the latency of B's bytes, costs less than a launch before this one.  LDS: a row's 512 bytes, the 16-byte pieces of
 // each 256 exchanged by the row, so that the 16 rows that read the same piece meet different banks.
-// Bound by the bytes of B and, for one row, by the launch: 1 x 4096 x 4096 6.7 us, 64 x 8192 x 4096 18.5 us, 8 tokens of 4
+// Bound by the bytes of B and, for one row, by the launch: 1 x 4096 x 4096 6.7 us, 64 x 8192 x 4096 18.5 us (two waves a
+// SIMD, half of their time without an instruction to issue: too little of B is in flight), 8 tokens of 4
 // places over 64 experts of 2048 x 2048 24 us (about 105 MB, 4.4 TB/s).
+// By plan every tile of 16 rows reads its expert's weights again and every workgroup quantizes the tile's float rows again:
+// 64 experts of 2048 x 4096 with 16 rows each 183 us from 8-bit rows and 276 from float ones (128-row tiles: 141 and 145).
 template <int MT, int NT, int FA, int FB, typename TO, typename XT>
 __global__ __launch_bounds__(512, 2) void k_gemm_fp8_rows16(Fp8Args g, Fp8Float fx)
 {

@@ -325,7 +325,7 @@ __device__ __forceinline__ void tile_row_max(const f32x16 (&lg)[NCT], float (&m)
 }
 
 // lg <- 2^(lg - max of the row), sm[r] = sum over the tiles; rmax = ls + 4 h holds the row maxima of this half-wave's
-// 16 rows in groups of four (stride 8).  Two rows at a time: the subtraction and the sum are packed (v_pk_add_f32).
+// 16 rows in groups of four (stride 8).  Two rows at a time.
 template <int NCT>
 __device__ __forceinline__ void tile_exp_sum(f32x16 (&lg)[NCT], const float *rmax, float (&sm)[16])
 {

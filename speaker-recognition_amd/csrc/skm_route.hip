@@ -317,9 +317,10 @@ __device__ __forceinline__ void merge_down8(unsigned *a, const unsigned *b)
 //   terms: (NV + 6) additions and the terms' errors, in all (NV + 48) 2^-24 / S bounds it; 1 / (1 + exp(-x)):
 //   p (1 - p) |x| <= 0.23 and an approximate reciprocal, 8 2^-24.  Error of c = p + bias: that and |c| 2^-24; of the key: |c| 2^-(23 - bits).
 // GROUPED: with groups of experts (without, those take registers that the rows in flight need).
-// Bound by the vector ALU (sort of the keys, k steps of the row's largest head), not by memory: 16384 x 256 float32, 8 of 8
-// groups' 4, bias: 23 us (0.8 TB/s); 32768 x 128 bf16 with a bias 18 us; 50001 x 512 float64, k = 20, 70 us (3.0
-// TB/s); one row 3.5 us, the launch.
+// Bound by the vector ALU (sort of the keys, k + 1 steps of the row's largest head, each waiting for the one before), not
+// by memory: 16384 x 256 float32, 4 of 8 groups, bias: 23 us (0.8 TB/s; vector ALU 73 % of the cycles in which a CU has
+// waves); 32768 x 128 bf16 with a bias 18 us (94 %); 50001 x 512 float64, k = 20, 70 us (3.0 TB/s); one row 3.5 us, the
+// launch.
 template <typename T, int NV, int L, bool GROUPED>
 __global__ __launch_bounds__(256, NV <= 16 ? 4 : NV == 32 ? (L == 16 ? 3 : 2) : 1) void k_route(RouteArgs a)
 {
@@ -912,6 +913,9 @@ __global__ __launch_bounds__(256) void k_route_backward16(RouteBackArgs a)
 template <typename T>
 static void route_back_go(const RouteBackArgs &a, hipStream_t st)
 {
+    // 16 lanes a row up to 512 experts: 16384 x 512 bf16, k 8, 9.7 us, a wave a row 20.5.  Softmax without renormalisation has
+    // a gradient at every expert and would be better off with a wave a row from there on (35 against 31 us; 16384 x 1024 60
+    // against 80), the others with 16 lanes for longer (16384 x 1024: 35 against 14.5).
     const dim3 grid((unsigned)((a.T + 15) / 16)), block(256);
     if (a.E <= 128) hipLaunchKernelGGL((k_route_backward16<T, 128>), grid, block, 0, st, a);
     else if (a.E <= 512) hipLaunchKernelGGL((k_route_backward16<T, 512>), grid, block, 0, st, a);
@@ -941,7 +945,8 @@ static void route_go_wide(const RouteArgs &a, hipStream_t st)
 template <typename T>
 static void route_launch(const RouteArgs &a, hipStream_t st)
 {
-    // 16 lanes a row up to 512 experts (32 of them a lane), the whole wave above.
+    // 16 lanes a row up to 512 experts (32 of them a lane), the whole wave above: 16384 x 512 float32, k 8, 15.5 us (a wave a
+    // row 20.4), 16384 x 1024 42.7 (16 lanes 54.3), bf16 12.6 (16.3) and 31.4 (35.8); 50001 x 512 float64, k 20, 69 (75).
     // In float64 throughout: probabilities of float64 logits; more groups than a row has lanes.
     const bool wide = (sizeof(T) == 8 && (a.bias || a.groups > 1 || (!a.renorm && !a.sigmoid))) || a.groups > (a.E <= 512 ? 16 : 64);
     if (wide) {
