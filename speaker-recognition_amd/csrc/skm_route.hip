@@ -456,7 +456,8 @@ __global__ __launch_bounds__(256, NV <= 16 ? 4 : NV == 32 ? (L == 16 ? 3 : 2) : 
     {                                                                                                                  \
         const float o = dpp_ror<0x120 + N>(score);                                                                     \
         const int g = dpp_ror<0x120 + N>(l);                                                                           \
-        open |= l < a.groups && g < a.groups && (dpp_ror<0x120 + N>((int)kept) != 0) != kept && fabsf(score - o) <= near; \
+        const bool okept = dpp_ror<0x120 + N>((int)kept) != 0;  /* by all lanes: one that sits out is not read */      \
+        open |= l < a.groups && g < a.groups && okept != kept && fabsf(score - o) <= near;                             \
     }
             ROUTE_TURNS(ROUTE_NEAR)
             const unsigned long long rows = __ballot(open);
