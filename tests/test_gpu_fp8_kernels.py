@@ -151,3 +151,48 @@ def test_weight_gradient_with_long_sums(eng, fa, fb, N):
     old = dw.clone()
     eng.gemm_fp8_experts_wgrad(A, B, plan, out=dw, accumulate=True)
     assert torch.equal(dw, 2 * old)
+
+
+@pytest.mark.parametrize("M,N", [(3, 60), (16, 4200), (40, 300), (130, 140), (2660, 3100)])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("fmt", ["e4m3", "e5m2"])
+def test_nan_and_infinities_stay_in_their_row(eng, M, N, dtype, fmt):
+    """on every kernel: a NaN (or infinity, which e4m3 has none of) leaves no number in its row and every number in the others"""
+    K = 1450
+    a = torch.rand(M, K, generator=torch.Generator().manual_seed(M)).cuda() + 0.5
+    b = torch.rand(N, K, generator=torch.Generator().manual_seed(N)).cuda() + 0.5       # no zeros: infinity times 0 is NaN
+    rows = torch.zeros(M, dtype=torch.bool)
+    rows[[1, M - 1]] = True
+    clean = eng.gemm_fp8(eng.fp8_rows(a, fmt), eng.fp8_tiles(b, fmt), dtype=DT[dtype])
+    a[1, K - 1], a[M - 1, 700] = float("nan"), float("inf")
+    got = eng.gemm_fp8(eng.fp8_rows(a, fmt), eng.fp8_tiles(b, fmt), dtype=DT[dtype])
+    assert torch.isnan(got[1]).all() and not torch.isfinite(got[M - 1]).any()
+    if fmt == "e5m2" and M > 2:
+        assert (got[M - 1] == float("inf")).all()
+    assert torch.equal(got[(~rows).cuda()], clean[(~rows).cuda()])
+    # and of B in their column
+    b[N - 1, 0] = float("nan")
+    other = eng.gemm_fp8(eng.fp8_rows(a, fmt), eng.fp8_rows(b, fmt), dtype=DT[dtype])
+    assert torch.isnan(other[:, N - 1]).all() and torch.isfinite(other[(~rows).cuda()][:, :N - 1]).all()
+
+
+@pytest.mark.parametrize("M", [1, 16, 40, 300])
+@pytest.mark.parametrize("every", [2, 4, 8, 16, 32, 64])
+@pytest.mark.parametrize("cancel", [False, True])
+def test_small_products_beside_large_ones(eng, M, every, cancel):
+    """the loss of the 8-bit instructions at its worst stays inside its bound, 2^-10 of the sum of the products' magnitudes
+    (see _product_close); float32 results lose nothing: sums of multiples of 2^-14 below 2^10 are exact"""
+    N, K = 140, 1024
+    k = torch.arange(K)
+    a = torch.where(k % every == 0, 1.0, 2.0 ** -7).repeat(M, 1)
+    if cancel:
+        a[:, (k % (2 * every)) == every] = -1.0              # the large products add up to nothing
+    b = torch.where(k % every == 0, 1.0, 2.0 ** -7).repeat(N, 1)
+    A, B = eng.fp8_rows(a.cuda()), eng.fp8_rows(b.cuda())
+    ref = a.double() @ b.double().t()
+    mag = a.abs().double() @ b.double().t()
+    assert torch.equal(eng.gemm_fp8(A, B, dtype=torch.float32).double().cpu(), ref)
+    for dtype in (torch.bfloat16, torch.float16):
+        c = eng.gemm_fp8(A, B, dtype=dtype).double().cpu()
+        tol = (2.0 ** -10 + rc.U32 * K) * mag + rc.half_step(dtype) * ref.abs() + 2.0 ** -25
+        assert ((c - ref).abs() <= tol).all()
